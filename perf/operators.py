@@ -405,13 +405,12 @@ def _sample(s):
     p = s["top_p"].double()[:, None]
     keep = (p >= 1) | (before < p * w.sum(1, keepdim=True)) | (at == 0)
     keep &= (w >= s["min_p"].double()[:, None]) | (at == 0)
-    w = torch.zeros_like(x).scatter_(1, index, torch.where(keep, w, 0.0))
-    upto = w.cumsum(1)
+    upto = torch.where(keep, w, 0.0).cumsum(1)
     u = s["u"].double()[:, None].clamp(0, 1)
-    past = upto > u * upto[:, -1:]
-    kept = w > 0
-    # the first token whose running mass passes u, the last kept one where rounding hides it
-    pick = torch.where(past.any(1), past.int().argmax(1), v - 1 - kept.flip(1).int().argmax(1))
+    past = keep & (upto > u * upto[:, -1:])
+    # the first token, in falling order, whose running mass passes u; the last kept one where rounding hides it
+    at = torch.where(past.any(1), past.int().argmax(1), keep.sum(1) - 1)
+    pick = index.gather(1, at[:, None])[:, 0]
     pick = torch.where(t[:, 0] > 0, pick, index[:, 0])
     return torch.where(top[:, 0] == float("-inf"), -1, pick)
 
