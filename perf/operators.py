@@ -263,7 +263,7 @@ def _assign(s):
     ends = add.cumsum(0)
     have = (lens + bs - 1) // bs
     after = (lens + add + bs - 1) // bs
-    fits = (after <= s["tables"].shape[1]) & (ends <= rows)
+    fits = (add == 0) | ((after <= s["tables"].shape[1]) & (ends <= rows))
     need = torch.where(fits, after - have, 0)
     upto = need.cumsum(0)
     served = fits & ((need == 0) | (upto <= count))
