@@ -31,6 +31,15 @@ class AffineExperts(ctypes.Structure):
     ]
 
 
+class KvCache8(ctypes.Structure):
+    """gdsllm_kv_cache8 (include/gdsllm_amd.h)."""
+
+    _fields_ = [
+        ("k", _c_vp), ("v", _c_vp), ("k_scale", _c_vp), ("v_scale", _c_vp),
+        ("num_blocks", _c_i64), ("kv_heads", _c_i64), ("block_size", _c_i64), ("head_dim", _c_i64), ("format", _c_i64),
+    ]
+
+
 # name -> (restype, argtypes); must match include/gdsllm_amd.h
 SIGNATURES = {
     "gdsllm_last_error": (ctypes.c_char_p, []),
@@ -80,6 +89,12 @@ SIGNATURES = {
     "gdsllm_moe_route_topk": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp]),
     "gdsllm_silu_mul": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "gdsllm_moe_combine": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "gdsllm_kv_assign": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64] + [_c_vp] * 6),
+    "gdsllm_kv_append": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "gdsllm_kv_attention_workspace_size": (ctypes.c_size_t, [_c_i64] * 6),
+    "gdsllm_kv_attention": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_size_t, _c_vp]),
+    "gdsllm_sample_tokens_workspace_size": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "gdsllm_sample_tokens": (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_vp]),
     "gdsllm_read_stream": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, ctypes.c_uint32, _c_vp, _c_vp]),
     "gdsllm_empty_launch": (ctypes.c_int, [_c_i64, _c_vp]),
 }

@@ -898,6 +898,204 @@ py::object fused_gate_up_silu(const Handle& gate, const Handle& up, torch::Tenso
     return py::cast(h);
 }
 
+// ---- 8-bit KV cache and sampling -------------------------------------------------
+// Not in the reference's gds_io_ext: its keys and values are fp16 torch tensors
+// (runtime/kv_cache.py) and its sampler runs torch ops behind a host sync
+// (engine.py:47-96).
+
+void check_on(const torch::Tensor& t, torch::Dtype type, int device, const char* what, const char* where) {
+    if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != type)
+        throw std::runtime_error(std::string(where) + ": " + what + " must be a " + c10::toString(type) +
+                                 " tensor on cuda:" + std::to_string(device));
+}
+
+// A 1-D tensor of `n` elements of `type` (any shape with that many), contiguous.
+torch::Tensor flat(const torch::Tensor& t, torch::Dtype type, int device, int64_t n, const char* what,
+                   const char* where) {
+    check_on(t, type, device, what, where);
+    if (t.numel() != n)
+        throw std::runtime_error(std::string(where) + ": " + what + " must hold " + std::to_string(n) +
+                                 " values, got " + std::to_string(t.numel()));
+    return t.contiguous();
+}
+
+// Block tables [requests, width] int32, rows any distance apart.
+void check_tables(const torch::Tensor& t, int device, int64_t requests, const char* where) {
+    check_on(t, torch::kInt32, device, "block_tables", where);
+    if (t.dim() != 2 || t.size(0) != requests || t.size(1) < 1 || (t.size(1) > 1 && t.stride(1) != 1) ||
+        (requests > 1 && t.stride(0) < t.size(1)))
+        throw std::runtime_error(std::string(where) + ": block_tables must be [" + std::to_string(requests) +
+                                 ", blocks] with contiguous rows");
+}
+int64_t table_stride(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+gdsllm_kv_cache8 kv_cache_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ks,
+                             const torch::Tensor& vs, const char* where) {
+    if (!k.is_cuda() || k.dim() != 4 || !k.is_contiguous() ||
+        (k.scalar_type() != torch::kFloat8_e4m3fn && k.scalar_type() != torch::kInt8))
+        throw std::runtime_error(std::string(where) + ": k_cache must be a contiguous float8_e4m3fn or int8 GPU tensor "
+                                 "[blocks, kv_heads, block_size, head_dim]");
+    const int dev = k.get_device();
+    check_on(v, k.scalar_type(), dev, "v_cache", where);
+    if (!v.sizes().equals(k.sizes()) || !v.is_contiguous())
+        throw std::runtime_error(std::string(where) + ": v_cache must have k_cache's shape and be contiguous");
+    for (const auto* t : {&ks, &vs}) {
+        check_on(*t, torch::kFloat32, dev, "the scales", where);
+        if (t->dim() != 2 || t->size(0) != k.size(0) || t->size(1) != k.size(1) || !t->is_contiguous())
+            throw std::runtime_error(std::string(where) + ": scales must be contiguous [blocks, kv_heads]");
+    }
+    return {k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), k.size(0), k.size(1), k.size(2),
+            k.size(3), k.scalar_type() == torch::kInt8 ? GDSLLM_KV_INT8 : GDSLLM_KV_E4M3};
+}
+
+// Rows [tokens, heads, dim] fp16: as they are where a row is contiguous and
+// rows start 16 bytes apart or a multiple of it, else a copy.
+torch::Tensor head_rows(const torch::Tensor& t, int device, int64_t heads, int64_t dim, const char* what,
+                        const char* where) {
+    check_on(t, torch::kFloat16, device, what, where);
+    if (t.dim() != 3 || t.size(2) != dim || (heads > 0 && t.size(1) != heads))
+        throw std::runtime_error(std::string(where) + ": " + what + " must be [tokens, " +
+                                 (heads > 0 ? std::to_string(heads) : std::string("heads")) + ", " + std::to_string(dim) + "]");
+    const bool in_place = t.numel() == 0 || (t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == dim) &&
+                                             (t.size(0) == 1 || (t.stride(0) >= t.size(1) * dim && t.stride(0) % 8 == 0)) &&
+                                             reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+    if (in_place) return t;
+    return t.is_contiguous() ? t.clone() : t.contiguous();  // clone: contiguous, but off the 16-byte grid
+}
+int64_t row_stride(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
+py::tuple kv_assign(torch::Tensor lens, torch::Tensor delta, torch::Tensor block_tables, torch::Tensor free_ring,
+                    torch::Tensor free_state, int64_t block_size, int64_t max_tokens) {
+    const char* where = "kv_assign";
+    if (!lens.is_cuda()) throw std::runtime_error("kv_assign: lens must be on a GPU");
+    const int dev = lens.get_device();
+    const int64_t n = lens.numel();
+    torch::Tensor l = flat(lens, torch::kInt32, dev, n, "lens", where), d = flat(delta, torch::kInt32, dev, n, "delta", where);
+    torch::Tensor st = flat(free_state, torch::kInt32, dev, 2, "free_state", where);
+    check_tables(block_tables, dev, n, where);
+    check_on(free_ring, torch::kInt32, dev, "free_ring", where);
+    if (free_ring.dim() != 1 || !free_ring.is_contiguous())
+        throw std::runtime_error("kv_assign: free_ring must be 1-D and contiguous");
+    if (max_tokens < 0 || max_tokens > (int64_t(1) << 30))
+        throw std::runtime_error("kv_assign: max_tokens must be in [0, 2^30]");
+    const auto opt = l.options();
+    torch::Tensor slots = torch::empty({max_tokens}, opt), positions = torch::empty({max_tokens}, opt);
+    torch::Tensor starts = torch::empty({n + 1}, opt), lens_out = torch::empty_like(l), state = torch::empty({2}, opt);
+    check(gdsllm_kv_assign(l.data_ptr<int32_t>(), d.data_ptr<int32_t>(), n, block_tables.data_ptr<int32_t>(),
+                           block_tables.size(1), table_stride(block_tables), free_ring.data_ptr<int32_t>(),
+                           free_ring.numel(), st.data_ptr<int32_t>(), block_size, max_tokens, slots.data_ptr<int32_t>(),
+                           positions.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), lens_out.data_ptr<int32_t>(),
+                           state.data_ptr<int32_t>(), OnDevice(dev).stream()),
+          where);
+    return py::make_tuple(slots, positions, starts, lens_out, state);
+}
+
+py::object kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
+                     torch::Tensor k_scale, torch::Tensor v_scale, c10::optional<torch::Tensor> q,
+                     c10::optional<torch::Tensor> positions, c10::optional<torch::Tensor> cos,
+                     c10::optional<torch::Tensor> sin) {
+    const char* where = "kv_append";
+    const gdsllm_kv_cache8 c = kv_cache_of(k_cache, v_cache, k_scale, v_scale, where);
+    const int dev = k_cache.get_device();
+    torch::Tensor kr = head_rows(k, dev, c.kv_heads, c.head_dim, "k", where);
+    torch::Tensor vr = head_rows(v, dev, c.kv_heads, c.head_dim, "v", where);
+    const int64_t n = kr.size(0);
+    if (vr.size(0) != n) throw std::runtime_error("kv_append: k and v differ in tokens");
+    torch::Tensor s = flat(slots, torch::kInt32, dev, n, "slots", where);
+    if (cos.has_value() != sin.has_value()) throw std::runtime_error("kv_append: cos and sin come together");
+    if (q.has_value() && !cos.has_value()) throw std::runtime_error("kv_append: q is given without cos and sin");
+    torch::Tensor pos, ct, sn, qr, out;
+    int64_t rotary = 0, max_pos = 0;
+    if (cos.has_value()) {
+        if (!positions.has_value()) throw std::runtime_error("kv_append: a rotation needs positions");
+        pos = flat(*positions, torch::kInt32, dev, n, "positions", where);
+        check_on(*cos, torch::kFloat32, dev, "cos", where);
+        if (cos->dim() != 2) throw std::runtime_error("kv_append: cos must be [positions, rotary / 2]");
+        ct = cos->contiguous();
+        sn = flat(*sin, torch::kFloat32, dev, ct.numel(), "sin", where);
+        if (!sn.sizes().equals(ct.sizes())) throw std::runtime_error("kv_append: cos and sin differ in shape");
+        max_pos = ct.size(0);
+        rotary = 2 * ct.size(1);
+    }
+    if (q.has_value()) {
+        qr = head_rows(*q, dev, 0, c.head_dim, "q", where);
+        if (qr.size(0) != n) throw std::runtime_error("kv_append: q and k differ in tokens");
+        out = torch::empty(qr.sizes(), qr.options());
+    }
+    const bool has_q = qr.defined(), has_r = ct.defined();
+    check(gdsllm_kv_append(&c, kr.data_ptr(), row_stride(kr), vr.data_ptr(), row_stride(vr), s.data_ptr<int32_t>(), n,
+                           has_q ? qr.data_ptr() : nullptr, has_q ? row_stride(qr) : 0, has_q ? out.data_ptr() : nullptr,
+                           has_q ? qr.size(1) : 0, has_r ? pos.data_ptr<int32_t>() : nullptr,
+                           has_r ? ct.data_ptr<float>() : nullptr, has_r ? sn.data_ptr<float>() : nullptr, rotary, max_pos,
+                           OnDevice(dev).stream()),
+          where);
+    return has_q ? py::cast(out) : py::none();
+}
+
+torch::Tensor kv_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                           torch::Tensor v_scale, torch::Tensor block_tables, torch::Tensor lens, torch::Tensor starts,
+                           double scale, int64_t max_new, int64_t max_len, c10::optional<torch::Tensor> output) {
+    const char* where = "kv_attention";
+    const gdsllm_kv_cache8 c = kv_cache_of(k_cache, v_cache, k_scale, v_scale, where);
+    const int dev = k_cache.get_device();
+    torch::Tensor qr = head_rows(q, dev, 0, c.head_dim, "q", where);
+    const int64_t n = lens.numel(), tokens = qr.size(0), heads = qr.size(1);
+    torch::Tensor l = flat(lens, torch::kInt32, dev, n, "lens", where);
+    torch::Tensor st = flat(starts, torch::kInt32, dev, n + 1, "starts", where);
+    check_tables(block_tables, dev, n, where);
+    torch::Tensor out;
+    if (output.has_value()) {
+        out = *output;
+        check_on(out, torch::kFloat16, dev, "output", where);
+        if (!out.sizes().equals(qr.sizes()) || out.stride(2) != 1 || (heads > 1 && out.stride(1) != c.head_dim) ||
+            (tokens > 1 && out.stride(0) < heads * c.head_dim))
+            throw std::runtime_error("kv_attention: output must have q's shape with contiguous rows");
+    } else {
+        out = torch::empty(qr.sizes(), qr.options());
+    }
+    const size_t bytes = gdsllm_kv_attention_workspace_size(n, heads, c.kv_heads, c.head_dim,
+                                                            max_new > 0 ? std::min(max_new, tokens) : tokens,
+                                                            max_len > 0 ? std::min(max_len, block_tables.size(1) * c.block_size)
+                                                                        : block_tables.size(1) * c.block_size);
+    torch::Tensor ws;
+    if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, qr.options().dtype(torch::kUInt8));
+    check(gdsllm_kv_attention(&c, qr.data_ptr(), row_stride(qr), out.data_ptr(), row_stride(out), tokens, heads,
+                              block_tables.data_ptr<int32_t>(), block_tables.size(1), table_stride(block_tables),
+                              l.data_ptr<int32_t>(), st.data_ptr<int32_t>(), n, static_cast<float>(scale), max_new, max_len,
+                              output.has_value() ? 0 : 1, bytes > 0 ? ws.data_ptr() : nullptr, bytes, OnDevice(dev).stream()),
+          where);
+    return out;
+}
+
+torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u, c10::optional<torch::Tensor> temperature,
+                            c10::optional<torch::Tensor> top_k, c10::optional<torch::Tensor> top_p,
+                            c10::optional<torch::Tensor> min_p) {
+    const char* where = "sample_tokens";
+    if (!logits.is_cuda() || (logits.scalar_type() != torch::kFloat16 && logits.scalar_type() != torch::kFloat32))
+        throw std::runtime_error("sample_tokens: logits must be a float16 or float32 GPU tensor");
+    if (logits.dim() < 1 || logits.size(-1) < 1) throw std::runtime_error("sample_tokens: logits must be [..., vocab]");
+    const int dev = logits.get_device();
+    const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
+    const bool strided = logits.dim() == 2 && logits.stride(1) == 1 && (rows <= 1 || logits.stride(0) >= vocab);
+    torch::Tensor l = strided ? logits : logits.contiguous();
+    torch::Tensor uu = flat(u, torch::kFloat32, dev, rows, "u", where), t, k, p, m;
+    if (temperature.has_value()) t = flat(*temperature, torch::kFloat32, dev, rows, "temperature", where);
+    if (top_k.has_value()) k = flat(*top_k, torch::kInt32, dev, rows, "top_k", where);
+    if (top_p.has_value()) p = flat(*top_p, torch::kFloat32, dev, rows, "top_p", where);
+    if (min_p.has_value()) m = flat(*min_p, torch::kFloat32, dev, rows, "min_p", where);
+    torch::Tensor out = torch::empty(logits.sizes().slice(0, logits.dim() - 1), l.options().dtype(torch::kInt64));
+    const int bits = l.scalar_type() == torch::kFloat16 ? 16 : 32;
+    const size_t bytes = bits == 16 ? gdsllm_sample_tokens_workspace_size(rows, vocab) : 0;
+    torch::Tensor ws;
+    if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, l.options().dtype(torch::kUInt8));
+    auto f = [](const torch::Tensor& x) { return x.defined() ? x.data_ptr<float>() : nullptr; };
+    check(gdsllm_sample_tokens(l.data_ptr(), bits, rows, vocab, strided && rows > 1 ? l.stride(0) : vocab, f(uu), f(t),
+                               k.defined() ? k.data_ptr<int32_t>() : nullptr, f(p), f(m), out.data_ptr<int64_t>(),
+                               bytes > 0 ? ws.data_ptr() : nullptr, bytes, OnDevice(dev).stream()),
+          where);
+    return out;
+}
+
 Handle from_tensor(const torch::Tensor& t) { return std::make_shared<GdsBufferHandle>(t); }
 
 }  // namespace
@@ -990,4 +1188,22 @@ PYBIND11_MODULE(gds_io_ext, m) {
     m.def("silu_mul", &silu_mul, "silu(gate) * up with torch fp16 semantics.", py::arg("gate"), py::arg("up"));
     m.def("moe_combine", &moe_combine, "clamp(expert_out + sigmoid(gate) * shared_out) with torch fp16 semantics.",
           py::arg("expert_out"), py::arg("shared_out"), py::arg("shared_gate_logit"));
+    m.def("kv_assign", &kv_assign,
+          "Cache blocks, slots and positions of a step from the requests' lengths: "
+          "(slots, positions, starts, lens, free_state); block_tables and free_ring are updated in place.",
+          py::arg("lens"), py::arg("delta"), py::arg("block_tables"), py::arg("free_ring"), py::arg("free_state"),
+          py::arg("block_size"), py::arg("max_tokens"));
+    m.def("kv_append", &kv_append,
+          "Rotate k (and q), write k and v to their slots of the 8-bit cache; returns the rotated q (None without q).",
+          py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
+          py::arg("v_scale"), py::arg("q") = py::none(), py::arg("positions") = py::none(), py::arg("cos") = py::none(),
+          py::arg("sin") = py::none());
+    m.def("kv_attention", &kv_attention, "Causal attention of q [T, heads, dim] over the 8-bit cache.", py::arg("q"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_tables"),
+          py::arg("lens"), py::arg("starts"), py::arg("scale"), py::arg("max_new") = 0, py::arg("max_len") = 0,
+          py::arg("output") = py::none());
+    m.def("sample_tokens", &sample_tokens,
+          "Tokens int64 [...] drawn from logits [..., vocab] with the given uniforms; per-row settings or None.",
+          py::arg("logits"), py::arg("u"), py::arg("temperature") = py::none(), py::arg("top_k") = py::none(),
+          py::arg("top_p") = py::none(), py::arg("min_p") = py::none());
 }

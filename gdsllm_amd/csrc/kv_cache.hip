@@ -1,0 +1,503 @@
+// The 8-bit KV cache of a serving loop: which blocks each request holds
+// (kv_assign) and the write of a step's keys and values into them (kv_append).
+//
+// A layer's cache is a pool of blocks of `block_size` tokens.  Codes lie as
+// [block][kv_head][token][head_dim], so that one head's block is one
+// contiguous run, and each (block, head) has one fp32 scale for its keys and
+// one for its values: element = scale * code.
+//
+// The scales this file writes are powers of two.  x / scale and scale / scale
+// are then exact, each code is one rounding of the fp16 value, and when a later
+// token makes a block's scale grow the old codes are rescaled exactly in e4m3
+// (but for codes that become subnormal) and with one more rounding in int8.
+// That costs at most one bit of the range and makes results independent of the
+// order of the arithmetic.
+
+#include <algorithm>
+
+#include "kv_cache.h"
+
+namespace gdsllm {
+
+int kv_cache_args(const gdsllm_kv_cache8* c, const std::string& where, KvCache* out) {
+    auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, where + ": " + m); };
+    if (!c) return bad("null cache");
+    if (c->format != GDSLLM_KV_E4M3 && c->format != GDSLLM_KV_INT8) return bad("unknown cache format");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return bad("head_dim must be 64, 128 or 256, got " + std::to_string(c->head_dim));
+    if (c->block_size < 16 || c->block_size > 256 || (c->block_size & (c->block_size - 1)))
+        return bad("block_size must be 16, 32, 64, 128 or 256, got " + std::to_string(c->block_size));
+    if (c->kv_heads < 1 || c->kv_heads > 1024) return bad("kv_heads must be in [1, 1024]");
+    if (c->num_blocks < 1 || c->num_blocks > ((int64_t(1) << 31) - 1) / c->block_size)
+        return bad("num_blocks must be positive and num_blocks * block_size below 2^31");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return bad("null cache pointer");
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 ||
+        (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) % 4)
+        return bad("misaligned cache pointer");
+    out->k = static_cast<uint8_t*>(c->k);
+    out->v = static_cast<uint8_t*>(c->v);
+    out->k_scale = c->k_scale;
+    out->v_scale = c->v_scale;
+    out->num_blocks = static_cast<int>(c->num_blocks);
+    out->kv_heads = static_cast<int>(c->kv_heads);
+    out->block_log2 = __builtin_ctzll(static_cast<unsigned long long>(c->block_size));
+    return GDSLLM_OK;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ kv_assign
+
+constexpr int kMaxRequests = 8192;  // three words of LDS each
+
+struct AssignArgs {
+    const int32_t* lens;
+    const int32_t* delta;
+    int32_t* tables;
+    int32_t* ring;
+    const int32_t* state;
+    int32_t *slots, *positions, *starts, *lens_out, *state_out;
+    int64_t ld_table;
+    int n, width, ring_size, block_log2, max_tokens;
+};
+
+// Inclusive sums over the workgroup of one int64 per thread.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t u = __shfl_up(static_cast<long long>(v), o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();  // part may still be read from the last scan
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) v += part[w];
+    return v;
+}
+
+// Every workgroup takes the sums over all requests for itself (two scans over
+// at most 8192 of them: cheaper than a second launch or a grid barrier) and
+// then writes its share of the tables and of the token rows.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
+    extern __shared__ int32_t lds[];
+    int32_t* ends = lds;              // tokens up to and with request r, at most max_tokens + 1
+    int32_t* first = lds + a.n;       // blocks taken before request r; -1 where it is not served
+    int32_t* given = lds + 2 * a.n;   // blocks given back before request r
+    __shared__ int64_t part[THREADS / 64];
+    __shared__ int taken, returned;
+    const int bs = 1 << a.block_log2, tid = threadIdx.x;
+    const int64_t row_tokens = static_cast<int64_t>(a.width) << a.block_log2;
+    if (tid == 0) taken = 0;
+    const int head = min(max(a.state[0], 0), a.ring_size - 1), count = min(max(a.state[1], 0), a.ring_size);
+
+    auto len_of = [&](int r) { return max(a.lens[r], 0); };
+    auto add_of = [&](int r) { return max(a.delta[r], 0); };
+    auto drop_of = [&](int r) {
+        return static_cast<int>(min(static_cast<int64_t>(len_of(r)), max(-static_cast<int64_t>(a.delta[r]), int64_t(0))));
+    };
+    auto blocks = [&](int64_t t) { return static_cast<int>((t + bs - 1) >> a.block_log2); };
+
+    const int per = (a.n + THREADS - 1) / THREADS, r0 = min(tid * per, a.n), r1 = min(r0 + per, a.n);
+    int64_t sum = 0;
+    for (int r = r0; r < r1; ++r) sum += add_of(r);
+    int64_t at = block_scan<THREADS>(sum, part) - sum;
+    const int64_t at0 = at;
+    auto need_of = [&](int r, int64_t end) {
+        const int64_t after = static_cast<int64_t>(len_of(r)) + add_of(r);
+        if (add_of(r) == 0) return 0;
+        return after <= row_tokens && end <= a.max_tokens ? blocks(after) - blocks(len_of(r)) : -1;
+    };
+    int64_t need = 0, back = 0;
+    for (int r = r0; r < r1; ++r) {
+        at += add_of(r);
+        need += max(need_of(r, at), 0);
+        back += blocks(len_of(r)) - blocks(len_of(r) - drop_of(r));
+    }
+    int64_t upto = block_scan<THREADS>(need, part) - need;
+    const int64_t back_end = block_scan<THREADS>(back, part);
+    if (tid == THREADS - 1) returned = static_cast<int>(min(back_end, static_cast<int64_t>(a.ring_size)));
+    int64_t back_at = back_end - back;
+    at = at0;
+    int most = 0;
+    for (int r = r0; r < r1; ++r) {
+        at += add_of(r);
+        const int n = need_of(r, at);
+        const bool served = n == 0 || (n > 0 && upto + n <= count);
+        ends[r] = static_cast<int32_t>(min(at, static_cast<int64_t>(a.max_tokens) + 1));
+        first[r] = served ? static_cast<int32_t>(min(upto, static_cast<int64_t>(a.ring_size))) : -1;
+        given[r] = static_cast<int32_t>(min(back_at, static_cast<int64_t>(a.ring_size)));
+        upto += max(n, 0);
+        if (served && n > 0) most = static_cast<int>(upto);
+        back_at += blocks(len_of(r)) - blocks(len_of(r) - drop_of(r));
+        if (blockIdx.x == 0) {
+            a.starts[r + 1] = min(ends[r], a.max_tokens);
+            a.lens_out[r] = len_of(r) + (served ? add_of(r) - drop_of(r) : 0);
+        }
+    }
+    if (most > 0) atomicMax(&taken, most);
+    __syncthreads();
+    const int room = a.ring_size - count;  // ring entries that a returned block may take
+    if (blockIdx.x == 0 && tid == 0) {
+        a.starts[0] = 0;
+        a.state_out[0] = (head + taken) % a.ring_size;
+        a.state_out[1] = count - taken + min(returned, room);
+    }
+
+    // new and returned blocks: one request to a wave
+    const int waves = THREADS / 64, lane = tid & 63;
+    for (int r = static_cast<int>(blockIdx.x) * waves + (tid >> 6); r < a.n; r += static_cast<int>(gridDim.x) * waves) {
+        const int len = len_of(r), add = add_of(r), have = blocks(len);
+        int32_t* row = a.tables + r * a.ld_table;
+        if (add > 0) {
+            const int n = blocks(static_cast<int64_t>(len) + add) - have;
+            if (first[r] >= 0)
+                for (int j = lane; j < n; j += 64)
+                    row[have + j] = a.ring[(static_cast<int64_t>(head) + first[r] + j) % a.ring_size];
+        } else {
+            const int keep = blocks(len - drop_of(r));
+            for (int j = lane; j < have - keep; j += 64)
+                if (keep + j < a.width && given[r] + j < room)
+                    a.ring[(static_cast<int64_t>(head) + count + given[r] + j) % a.ring_size] = row[keep + j];
+        }
+    }
+    // token rows: the request of a row is the first whose end lies past it
+    const int total = a.n > 0 ? min(ends[a.n - 1], a.max_tokens) : 0;
+    for (int t = static_cast<int>(blockIdx.x) * THREADS + tid; t < a.max_tokens; t += static_cast<int>(gridDim.x) * THREADS) {
+        int slot = -1, pos = -1;
+        if (t < total) {
+            int lo = 0, hi = a.n - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ends[mid] > t) hi = mid;
+                else lo = mid + 1;
+            }
+            if (first[lo] >= 0) {
+                const int len = len_of(lo), have = blocks(len);
+                pos = len + t - (lo > 0 ? ends[lo - 1] : 0);
+                const int b = pos >> a.block_log2;
+                const int id = b < have ? a.tables[lo * a.ld_table + b]
+                                        : a.ring[(static_cast<int64_t>(head) + first[lo] + b - have) % a.ring_size];
+                slot = (id << a.block_log2) + (pos & (bs - 1));
+            }
+        }
+        a.slots[t] = slot;
+        a.positions[t] = pos;
+    }
+}
+
+// ------------------------------------------------------------------ kv_append
+
+struct AppendArgs {
+    KvCache c;
+    const uint16_t *k, *v, *q;
+    uint16_t* q_out;
+    const int32_t *slots, *positions;
+    const float *cos, *sin;
+    int64_t ldk, ldv, ldq;
+    int tokens, q_heads, half;  // half: channels in one half of a rotated pair; 0: no rotation
+    int max_pos;
+    int rows_per_group;         // token rows of a workgroup
+    int groups;                 // ceil(tokens / rows_per_group)
+};
+
+// The slot of a row that is written, -1 for padding: a slot outside the
+// cache, or a position that the rotation's table does not have.
+__device__ __forceinline__ int64_t slot_of(const AppendArgs& a, int t) {
+    const int s = a.slots[t];
+    if (s < 0 || (s >> a.c.block_log2) >= a.c.num_blocks) return -1;
+    if (a.half > 0 && static_cast<uint32_t>(a.positions[t]) >= static_cast<uint32_t>(a.max_pos)) return -1;
+    return s;
+}
+
+// (x c - y s, y c + x s) of eight fp16 pairs.  In 64 bits: the products are
+// exact, so the one rounding that counts is the last, to fp16.
+__device__ __forceinline__ void rotate8(const uint4& x, const uint4& y, const float* c, const float* s, bool first,
+                                        uint16_t (&out)[8]) {
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double a = h2f((xs[i / 2] >> (16 * (i & 1))) & 0xFFFFu), b = h2f((ys[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+        const double cc = c[i], ss = s[i];
+        out[i] = f2h_bits(fp32_rounded(static_cast<float>(first ? a * cc - b * ss : a * cc + b * ss)));
+    }
+}
+
+// Eight channels (chunk `ch`) of a row of k, after the rotation, as fp16 bits.
+__device__ __forceinline__ void load_rotated(const AppendArgs& a, const uint16_t* row, int t, int ch,
+                                             uint16_t (&out)[8]) {
+    const uint4 own = *reinterpret_cast<const uint4*>(row + 8 * ch);
+    const int hc = a.half >> 3;
+    if (ch < 2 * hc) {
+        const bool lo = ch < hc;
+        const uint4 other = *reinterpret_cast<const uint4*>(row + 8 * (lo ? ch + hc : ch - hc));
+        const int64_t at = static_cast<int64_t>(a.positions[t]) * a.half + 8 * (lo ? ch : ch - hc);
+        rotate8(own, other, a.cos + at, a.sin + at, lo, out);
+        return;
+    }
+    const uint32_t w[4] = {own.x, own.y, own.z, own.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+}
+
+// Workgroups [0, groups * kv_heads * 2): keys (even) or values (odd) of one
+// head in rows_per_group token rows.  A page's tokens stand in consecutive
+// rows; the workgroup takes every page whose first row lies in its rows, to
+// that page's last row wherever it is, so one workgroup alone writes a page.
+template <bool E4M3, int D>
+__device__ void append_pages(const AppendArgs& a, int unit) {
+    constexpr int C = D / 8;
+    __shared__ float red[4];
+    const bool is_k = (unit & 1) == 0;
+    const int head = (unit >> 1) % a.c.kv_heads, g = (unit >> 1) / a.c.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nthreads = blockDim.x;
+    const int bl = a.c.block_log2;
+    const uint16_t* src = (is_k ? a.k : a.v) + head * D;
+    const int64_t ld = is_k ? a.ldk : a.ldv;
+    uint8_t* codes = is_k ? a.c.k : a.c.v;
+    float* scales = is_k ? a.c.k_scale : a.c.v_scale;
+    const float top = E4M3 ? kE4m3Max : kInt8Max;
+
+    const int t_end = min((g + 1) * a.rows_per_group, a.tokens);
+    for (int t0 = g * a.rows_per_group; t0 < t_end; ++t0) {
+        const int64_t s0 = slot_of(a, t0);
+        if (s0 < 0) continue;
+        const int page = static_cast<int>(s0 >> bl);
+        if (t0 > 0) {
+            const int64_t prev = slot_of(a, t0 - 1);
+            if (prev >= 0 && (prev >> bl) == page) continue;
+        }
+        // rows of the page, the lowest offset among them, and whether the
+        // offsets rise row by row (else a slot may occur twice)
+        int n = 1, low = static_cast<int>(s0) & ((1 << bl) - 1);
+        bool rising = true;
+        for (;;) {
+            const int t = t0 + n + lane;
+            const int64_t s = t < a.tokens ? slot_of(a, t) : -1;
+            const bool in = s >= 0 && (s >> bl) == page;
+            const uint64_t out = ~__ballot(in);
+            const int more = out ? __builtin_ctzll(out) : 64;
+            if (lane < more) low = min(low, static_cast<int>(s) & ((1 << bl) - 1));
+            if (__ballot(lane < more && s <= slot_of(a, t - 1))) rising = false;
+            n += more;
+            if (more < 64) break;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o));
+
+        auto load = [&](int i, uint16_t (&x)[8]) {
+            const int t = t0 + i / C;
+            const uint16_t* row = src + t * ld;
+            if (is_k && a.half > 0) {
+                load_rotated(a, row, t, i % C, x);
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4*>(row + 8 * (i % C));
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = static_cast<uint16_t>(ws[j / 2] >> (16 * (j & 1)));
+            }
+        };
+        float amax = 0.f;
+        for (int i = tid; i < n * C; i += nthreads) {
+            uint16_t x[8];
+            load(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if ((x[j] & 0x7C00u) != 0x7C00u) amax = fmaxf(amax, h2f(x[j] & 0x7FFFu));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+        if (nthreads > 64) {
+            __syncthreads();
+            if (lane == 0) red[wave] = amax;
+            __syncthreads();
+            amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        }
+        // smallest power of two with amax <= top * scale
+        float want = 0x1p-32f;
+        if (amax > 0.f) {
+            int e;
+            const float m = frexpf(amax / top, &e);
+            want = fmaxf(want, ldexpf(1.f, m == 0.5f ? e - 1 : e));
+        }
+        const int64_t sc = static_cast<int64_t>(page) * a.c.kv_heads + head;
+        const float was = low > 0 ? scales[sc] : 0.f;
+        const float now = fmaxf(was, want);
+        if (nthreads > 64) __syncthreads();  // every wave has read the old scale
+        uint8_t* base = codes + ((sc << bl) * D);
+        if (tid == 0) scales[sc] = now;
+        if (low > 0 && was != now) {
+            const float ratio = was / now;
+            for (int i = tid; i < low * C; i += nthreads) {
+                uint2* p = reinterpret_cast<uint2*>(base + 8 * static_cast<int64_t>(i));
+                const uint2 w = *p;
+                float x[4], y[4];
+                codes_to_f32<E4M3>(w.x, x);
+                codes_to_f32<E4M3>(w.y, y);
+                *p = make_uint2(to_codes<E4M3>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio),
+                                to_codes<E4M3>(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio));
+            }
+        }
+        const float inv = 1.f / now;
+        for (int i = tid; i < n * C; i += nthreads) {
+            const int t = t0 + i / C;
+            const int64_t s = slot_of(a, t);
+            if (!rising) {  // the last row of a slot that occurs twice is the one that stays
+                bool later = false;
+                for (int u = t + 1; u < t0 + n; ++u) later |= slot_of(a, u) == s;
+                if (later) continue;
+            }
+            uint16_t x[8];
+            load(i, x);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = h2f(x[j]) * inv;
+            const int64_t at = (s & ((1 << bl) - 1)) * D + 8 * (i % C);
+            *reinterpret_cast<uint2*>(base + at) =
+                make_uint2(to_codes<E4M3>(y[0], y[1], y[2], y[3]), to_codes<E4M3>(y[4], y[5], y[6], y[7]));
+        }
+    }
+}
+
+template <bool E4M3, int D>
+__global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
+    const int units = a.groups * a.c.kv_heads * 2;
+    if (static_cast<int>(blockIdx.x) < units) {
+        append_pages<E4M3, D>(a, blockIdx.x);
+        return;
+    }
+    // the rotation of q: one chunk of eight channels a thread
+    constexpr int C = D / 8;
+    const int64_t chunks = static_cast<int64_t>(a.tokens) * a.q_heads * C;
+    const int64_t step = static_cast<int64_t>(gridDim.x - units) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - units) * blockDim.x + threadIdx.x; i < chunks; i += step) {
+        const int64_t th = i / C;
+        const int t = static_cast<int>(th / a.q_heads);
+        uint16_t x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (slot_of(a, t) >= 0)
+            load_rotated(a, a.q + t * a.ldq + (th % a.q_heads) * D, t, static_cast<int>(i % C), x);
+        uint4 w;
+        w.x = x[0] | (uint32_t(x[1]) << 16);
+        w.y = x[2] | (uint32_t(x[3]) << 16);
+        w.z = x[4] | (uint32_t(x[5]) << 16);
+        w.w = x[6] | (uint32_t(x[7]) << 16);
+        *reinterpret_cast<uint4*>(a.q_out + i * 8) = w;
+    }
+}
+
+}  // namespace
+}  // namespace gdsllm
+
+using namespace gdsllm;
+
+extern "C" int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests, int32_t* block_tables,
+                                int64_t table_width, int64_t ld_table, int32_t* free_ring, int64_t ring_size,
+                                const int32_t* free_state, int64_t block_size, int64_t max_tokens, int32_t* slots,
+                                int32_t* positions, int32_t* starts, int32_t* lens_out, int32_t* state_out,
+                                void* stream) {
+    const std::string n = "kv_assign";
+    auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
+    if (requests < 1 || requests > kMaxRequests) return bad("requests must be in [1, 8192]");
+    if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1)))
+        return bad("block_size must be 16, 32, 64, 128 or 256, got " + std::to_string(block_size));
+    if (table_width < 1 || ld_table < table_width) return bad("ld_table < table_width or an empty table");
+    if (table_width > ((int64_t(1) << 31) - 1) / block_size) return bad("table_width too large");
+    if (ring_size < 1 || ring_size > ((int64_t(1) << 31) - 1) / block_size)
+        return bad("ring_size must be positive and ring_size * block_size below 2^31");
+    if (max_tokens < 0 || max_tokens > (int64_t(1) << 30)) return bad("max_tokens must be in [0, 2^30]");
+    if (!lens || !delta || !block_tables || !free_ring || !free_state || !starts || !lens_out || !state_out ||
+        (max_tokens > 0 && (!slots || !positions)))
+        return bad("null pointer");
+    if ((reinterpret_cast<uintptr_t>(lens) | reinterpret_cast<uintptr_t>(delta) |
+         reinterpret_cast<uintptr_t>(block_tables) | reinterpret_cast<uintptr_t>(free_ring) |
+         reinterpret_cast<uintptr_t>(free_state) | reinterpret_cast<uintptr_t>(slots) |
+         reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(starts) |
+         reinterpret_cast<uintptr_t>(lens_out) | reinterpret_cast<uintptr_t>(state_out)) % 4)
+        return bad("misaligned pointer");
+    if (lens_out == lens || state_out == free_state) return bad("lens_out and state_out must not be the inputs");
+    AssignArgs a{lens, delta, block_tables, free_ring, free_state, slots, positions, starts, lens_out, state_out,
+                 ld_table, static_cast<int>(requests), static_cast<int>(table_width), static_cast<int>(ring_size),
+                 __builtin_ctzll(static_cast<unsigned long long>(block_size)), static_cast<int>(max_tokens)};
+    const size_t lds = 3 * sizeof(int32_t) * static_cast<size_t>(requests);
+    const int threads = requests <= 256 ? 256 : 1024;
+    const int64_t want = std::max((max_tokens + threads - 1) / threads, (requests + 255) / 256);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(want, 1), cu_count()));
+    if (threads == 256) {
+        hipLaunchKernelGGL(kv_assign<256>, dim3(grid), dim3(256), lds, as_stream(stream), a);
+    } else {
+        if (int rc = prepare_lds(reinterpret_cast<const void*>(&kv_assign<1024>), lds)) return rc;
+        hipLaunchKernelGGL(kv_assign<1024>, dim3(grid), dim3(1024), lds, as_stream(stream), a);
+    }
+    if (int rc = check_hip(hipGetLastError(), "kv_assign launch")) return rc;
+    return ok();
+}
+
+extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                const int32_t* slots, int64_t tokens, const void* q, int64_t ldq, void* q_out,
+                                int64_t q_heads, const int32_t* positions, const float* cos, const float* sin,
+                                int64_t rotary, int64_t max_pos, void* stream) {
+    const std::string n = "kv_append";
+    auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
+    AppendArgs a{};
+    if (int rc = kv_cache_args(cache, n, &a.c)) return rc;
+    const int64_t D = cache->head_dim;
+    if (tokens < 0 || tokens > (int64_t(1) << 30)) return bad("bad token count");
+    if (rotary < 0 || rotary > D || rotary % 16)
+        return bad("rotary must be a multiple of 16 in [0, head_dim], got " + std::to_string(rotary));
+    if (q && !rotary) return bad("q is given without a rotation");
+    if (q && (q_heads < 1 || q_heads > 16384)) return bad("q_heads must be in [1, 16384]");
+    if (tokens == 0) return ok();
+    if (!k || !v || !slots || (q && !q_out)) return bad("null pointer");
+    if (rotary && (!positions || !cos || !sin)) return bad("a rotation needs positions, cos and sin");
+    if (rotary && (max_pos < 1 || max_pos > (int64_t(1) << 31) - 1)) return bad("bad number of positions");
+    if (ldk < cache->kv_heads * D || ldv < cache->kv_heads * D || (q && ldq < q_heads * D))
+        return bad("row stride smaller than a row");
+    if (ldk % 8 || ldv % 8 || (q && ldq % 8)) return bad("row strides must be multiples of 8");
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q) |
+         reinterpret_cast<uintptr_t>(q_out)) % 16)
+        return bad("k, v, q and q_out must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions) |
+         reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 4)
+        return bad("misaligned pointer");
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.slots = slots;
+    a.positions = positions;
+    a.cos = cos;
+    a.sin = sin;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldq = ldq;
+    a.tokens = static_cast<int>(tokens);
+    a.q_heads = static_cast<int>(q_heads);
+    a.half = static_cast<int>(rotary / 2);
+    a.max_pos = static_cast<int>(max_pos);
+    a.rows_per_group = tokens > 512 ? 16 : 1;
+    a.groups = static_cast<int>((tokens + a.rows_per_group - 1) / a.rows_per_group);
+    const int64_t units = static_cast<int64_t>(a.groups) * cache->kv_heads * 2;
+    const int threads = tokens > 512 ? 256 : 64;
+    int64_t q_groups = 0;
+    if (q) {
+        const int64_t chunks = tokens * q_heads * (D / 8);
+        q_groups = std::min<int64_t>((chunks + threads - 1) / threads, 16 * static_cast<int64_t>(cu_count()));
+    }
+    if (units + q_groups > (int64_t(1) << 31) - 1) return bad("too many tokens and heads for one call");
+    const dim3 grid(static_cast<unsigned>(units + q_groups)), block(threads);
+    const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
+    const hipStream_t s = as_stream(stream);
+#define GDSLLM_APPEND(DIM)                                                                   \
+    if (D == DIM) {                                                                          \
+        if (e4m3) hipLaunchKernelGGL((kv_append<true, DIM>), grid, block, 0, s, a);          \
+        else hipLaunchKernelGGL((kv_append<false, DIM>), grid, block, 0, s, a);              \
+    }
+    GDSLLM_APPEND(64)
+    GDSLLM_APPEND(128)
+    GDSLLM_APPEND(256)
+#undef GDSLLM_APPEND
+    if (int rc = check_hip(hipGetLastError(), "kv_append launch")) return rc;
+    return ok();
+}

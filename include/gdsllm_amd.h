@@ -417,6 +417,110 @@ int gdsllm_moe_prefill_affine_q4(const gdsllm_affine_experts* gate,
                                  void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                                  void* stream);
 
+/* ------------------------------------------------------ 8-bit KV cache --
+ * The state between a step's q/k/v projections and o_proj.  No counterpart
+ * kernels in the reference, which concatenates fp16 keys and values in torch
+ * (runtime/kv_cache.py) and attends with torch ops (runtime/llama.py:212-246).
+ *
+ * One layer's cache: a pool of blocks of block_size tokens (16, 32, 64, 128 or
+ * 256), codes [num_blocks][kv_heads][block_size][head_dim] (head_dim 64, 128 or
+ * 256) and one fp32 scale for each (block, kv head), [num_blocks][kv_heads];
+ * element = scale * code.  format: the codes' type.  Slot s is token
+ * s % block_size of block s / block_size.                                    */
+enum gdsllm_kv_format { GDSLLM_KV_E4M3 = 0, GDSLLM_KV_INT8 = 1 };
+typedef struct gdsllm_kv_cache8 {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t num_blocks;
+    int64_t kv_heads;
+    int64_t block_size;
+    int64_t head_dim;
+    int64_t format;
+} gdsllm_kv_cache8;
+
+/* Block tables and slot maps of a step, from the requests' lengths.
+ * Request r holds lens[r] tokens in blocks block_tables[r][0 ..] (rows
+ * ld_table apart, table_width entries) and changes by delta[r]: a positive
+ * number of tokens is added, a negative one dropped from its end (no more than
+ * it holds; all of them ends the request).  Free blocks are a ring:
+ * free_ring[(head + i) % ring_size], i < count, free_state = {head, count}.
+ * Requests take new blocks from its head in their order and dropped blocks go
+ * to its tail, for later calls.  A request is not served when its new length
+ * does not fit its table row, its tokens do not fit max_tokens, or, if it needs
+ * blocks, the blocks needed up to and with it are more than count.
+ * Written: block_tables (new entries) and free_ring (returned blocks) in place;
+ * lens_out [requests] (not served: unchanged) and state_out [2], which must not
+ * be the inputs; starts [requests + 1], the first token row of each request and
+ * the end of the last (at most max_tokens); slots and positions [max_tokens],
+ * -1 for the rows of requests not served and behind the last request.
+ * The inputs stay as they are, so the same call gives the same result.
+ * requests <= 8192.                                                         */
+int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests, int32_t* block_tables,
+                     int64_t table_width, int64_t ld_table, int32_t* free_ring, int64_t ring_size,
+                     const int32_t* free_state, int64_t block_size, int64_t max_tokens, int32_t* slots,
+                     int32_t* positions, int32_t* starts, int32_t* lens_out, int32_t* state_out, void* stream);
+
+/* Writes keys and values k, v fp16 [tokens][kv_heads * head_dim] (rows ldk, ldv
+ * apart) to their slots.  With rotary > 0 (a multiple of 16, at most head_dim)
+ * keys, and q [tokens][q_heads * head_dim] into q_out (rows contiguous; q may be
+ * null), are rotated first: channels i and i + rotary/2 of a head turn by the
+ * angle whose cosine and sine are cos, sin [max_pos][rotary/2] at positions[t];
+ * the rotated values are rounded once, to fp16.
+ * The tokens of one block stand in consecutive rows (as kv_assign numbers
+ * them); a block occurs in one such run only.  With o the lowest offset that
+ * the call writes in a block, what the block held before o stays and what it
+ * held from o on is replaced.  The (block, head)'s scale becomes the smallest
+ * power of two s >= 2^-32 with |x| <= top * s (top 448 or 127) for its new
+ * finite values, or the scale it had, if o > 0 and that is larger; older codes
+ * are rescaled to a scale that grew.  Codes are x / s to nearest even,
+ * saturated; NaN stays NaN in e4m3 and is 0 in int8.  A row whose slot lies
+ * outside the cache (-1) or whose position outside [0, max_pos) is padding:
+ * not written, zeros in q_out.  Of several rows with one slot the last counts. */
+int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                     const int32_t* slots, int64_t tokens, const void* q, int64_t ldq, void* q_out, int64_t q_heads,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t rotary, int64_t max_pos,
+                     void* stream);
+
+/* Causal attention of q fp16 [tokens][q_heads * head_dim] over the cache into
+ * o (rows ldq, ldo apart).  Request r's rows are starts[r] .. starts[r+1]-1, the
+ * last of its lens[r] tokens: row i of n sees tokens 0 .. lens[r]-n+i; a row
+ * that sees none is zero.  Query head h reads kv head h / (q_heads / kv_heads).
+ * Products of fp16 and code values in fp32, softmax in fp32, weights rounded
+ * to fp16 before the product with the values.  Scales must be positive; blocks
+ * outside the cache have no weight.
+ * max_new and max_len: bounds on a request's rows and tokens, known to the host
+ * (0: tokens, and table_width * block_size).  They set how the work is split;
+ * larger requests than they say are computed all the same, more slowly.
+ * Rows behind the last request are left as they were, or set to zero with
+ * zero_tail.  workspace_bytes >= gdsllm_kv_attention_workspace_size(...).    */
+size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t max_new, int64_t max_len);
+int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
+                        int64_t tokens, int64_t q_heads, const int32_t* block_tables, int64_t table_width,
+                        int64_t ld_table, const int32_t* lens, const int32_t* starts, int64_t requests, float scale,
+                        int64_t max_new, int64_t max_len, int zero_tail, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* -------------------------------------------------------------- sampling --
+ * One token for each row of logits [rows][vocab] (fp16 or fp32: bits 16 or 32;
+ * rows ld apart; vocab <= 2^20) from the uniform number u[row] in [0, 1).
+ * Tokens are taken in falling order of their logits, equal ones by rising index,
+ * with weights exp((l - max) / temperature).  Kept: the first top_k (<= 0: all);
+ * of those, the tokens before which less than top_p of their mass lies; of
+ * those, the ones whose weight is at least min_p of the largest; always the
+ * first.  The draw is the first kept token at which the running mass passes
+ * u times the kept mass.  temperature <= 0 (or NaN): the first token.  NaN and
+ * -inf are never drawn; a row without any other value gives -1.  temperature,
+ * top_k, top_p and min_p hold one value a row; null: 1, all, 1, 0.
+ * Weights and sums in 64 bits.  Replaces _sample (engine.py:47-96), which
+ * sorts the logits and draws on the host side of a sync.                     */
+size_t gdsllm_sample_tokens_workspace_size(int64_t rows, int64_t vocab);
+int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
+                         const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                         int64_t* tokens, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------ measurement helpers --
  * Not on the matvec path and with no counterpart in the reference: reference
  * kernels the benchmark measures the GEMV against on the same device.

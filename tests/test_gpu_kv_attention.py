@@ -1,0 +1,186 @@
+"""Attention over the 8-bit cache against the plain 64-bit form
+(oracle/serve.py attention, which derives the bound its results are held to)."""
+
+import pytest
+import torch
+
+from gdsllm_amd.runtime import ext
+from helpers import gen
+from oracle import serve as sv
+
+pytestmark = pytest.mark.gpu
+
+
+class Problem:
+    def __init__(self, dev, fmt, dim, heads, kv_heads, bs, lens, new, seed, extra_rows=0, spread=1.0, qscale=1.0):
+        g = gen(seed)
+        counts = [sv.blocks(n, bs) for n in lens]
+        pool = sum(counts) + 2
+        x = torch.randn(2, pool, kv_heads, bs, dim, generator=g) * 100
+        x = x.clamp(-sv.QMAX[fmt], sv.QMAX[fmt])
+        self.codes = (x.round() if fmt == "int8" else x).to(sv.DTYPE[fmt])
+        # any positive scale: those kv_append writes are powers of two
+        self.scales = 0.01 * torch.exp(spread * torch.randn(2, pool, kv_heads, generator=g))
+        ids = torch.randperm(pool, generator=g)
+        width = max(1, max(counts))
+        self.tables = torch.full((len(lens), width), -1, dtype=torch.int32)
+        at = 0
+        for b, c in enumerate(counts):
+            self.tables[b, :c] = ids[at:at + c].int()
+            at += c
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        self.starts = torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        self.q = (torch.randn(sum(new) + extra_rows, heads, dim, generator=g) * qscale).half()
+        self.scale, self.dev, self.fmt, self.bs = dim ** -0.5, dev, fmt, bs
+        self.new, self.longest = max(new), max(lens)
+
+    def poison(self):
+        """Everything behind a request's last token, and blocks nobody holds, is no number (e4m3) or large."""
+        held = torch.zeros(self.codes.shape[1], self.bs, dtype=torch.bool)
+        for row, n in zip(self.tables.tolist(), self.lens.tolist()):
+            for i in range(n):
+                held[row[i // self.bs], i % self.bs] = True
+        bad = 0x7F
+        c = self.codes.view(torch.uint8)
+        c.copy_(torch.where(held[None, :, None, :, None], c, torch.tensor(bad, dtype=torch.uint8)))
+        free = ~held.any(1)
+        self.scales[:, free] = float("nan")
+
+    def run(self, max_new=None, max_len=None, **kw):
+        d = lambda t: t.to(self.dev)  # noqa: E731
+        return ext().kv_attention(d(self.q), d(self.codes[0]), d(self.codes[1]), d(self.scales[0]), d(self.scales[1]),
+                                  d(self.tables), d(self.lens), d(self.starts), self.scale,
+                                  self.new if max_new is None else max_new,
+                                  self.longest if max_len is None else max_len, **kw)
+
+    def check(self, got):
+        s = self.scales.double().nan_to_num(1.0)
+        vals = self.codes.double() * s[..., None, None]
+        want, bound = sv.attention(self.q, vals[0], vals[1], s[1], self.tables, self.lens, self.starts, self.scale)
+        err = (got.cpu().double() - want).abs()
+        assert bool((err <= bound).all()), f"worst {float((err / bound.clamp(min=2.0 ** -25)).max()):.3f} of the bound"
+
+
+HEADS = [(64, 4, 4), (128, 8, 1), (128, 6, 2), (256, 16, 1), (128, 7, 7), (64, 40, 2)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,kv_heads", HEADS, ids=[f"d{d}_{h}x{k}" for d, h, k in HEADS])
+@pytest.mark.parametrize("bs", [16, 32, 64, 256])
+def test_decode(gpu, fmt, dim, heads, kv_heads, bs):
+    """One new token a request: lengths about a block's and a tile's edge, an idle slot among them."""
+    lens = [1, 15, 16, 17, 0, 31, 33, 63, 64, 65, 127, 129, 255, 257, 300]
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, lens, [0 if n == 0 else 1 for n in lens], 200 + dim + bs)
+    p.poison()
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,kv_heads,bs", [(128, 4, 1, 64), (64, 8, 8, 16), (256, 4, 2, 128)])
+def test_decode_split(gpu, fmt, dim, heads, kv_heads, bs):
+    """Sequences long enough to be split, the last unit short; the bound on the length loose, right and too small."""
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, [2100, 513, 5, 1024], [1, 1, 1, 1], 300 + dim)
+    p.poison()
+    outs = [p.run(), p.run(max_len=0), p.run(max_len=300), p.run(max_new=0)]
+    for o in outs:
+        p.check(o)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,kv_heads,bs", [(128, 4, 1, 64), (64, 3, 3, 16), (256, 4, 2, 128), (128, 14, 2, 32)])
+@pytest.mark.parametrize("lens,new", [([5, 300, 64, 129], [5, 2, 64, 100]), ([200], [200]), ([17, 0, 40], [1, 0, 33]),
+                                      ([400, 3], [3, 3])], ids=["ragged", "whole", "mixed", "few"])
+def test_prompts(gpu, fmt, dim, heads, kv_heads, bs, lens, new):
+    """Several new tokens a request, behind what its cache holds; rows see the tokens up to their own."""
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, lens, new, 400 + dim + bs)
+    p.poison()
+    p.check(p.run())
+
+
+def test_rows_that_see_nothing_and_rows_behind_the_last(gpu):
+    """More rows than tokens (a request that was not served): the first rows see nothing and are zero.  Rows behind
+    the last request are zero in a new tensor and left alone in a given one."""
+    p = Problem(gpu, "e4m3", 128, 4, 2, 16, [3, 0, 20], [5, 2, 1], 500, extra_rows=6)
+    p.poison()
+    got = p.run()
+    p.check(got)
+    assert bool((got[:2] == 0).all()) and bool((got[5:7] == 0).all()) and bool((got[8:] == 0).all())
+    wide = torch.full((14, 4 * 128 + 64), 7.0, dtype=torch.float16, device=gpu)
+    out = wide[:, :4 * 128].unflatten(1, (4, 128))
+    assert p.run(output=out).data_ptr() == out.data_ptr()
+    p.check(torch.cat([out[:8], torch.zeros_like(out[8:])]))
+    assert bool((wide[8:] == 7).all()) and bool((wide[:, 512:] == 7).all())
+
+
+def test_scales_far_apart(gpu):
+    """Value scales of neighbouring blocks 2^40 apart, a block of zeros with a tiny scale, large scores."""
+    p = Problem(gpu, "e4m3", 64, 2, 1, 16, [200, 64], [1, 3], 600, spread=0.0, qscale=6.0)
+    e = torch.arange(p.scales.shape[1]) % 3
+    p.scales[1] *= torch.exp2(torch.tensor([0.0, -40.0, -20.0]))[e][:, None]
+    p.codes[1].view(torch.uint8)[p.tables[0, 3]] = 0
+    p.check(p.run())
+
+
+def test_blocks_outside_the_cache_have_no_weight(gpu):
+    p = Problem(gpu, "int8", 64, 2, 1, 16, [40], [1], 700)
+    want = Problem(gpu, "int8", 64, 2, 1, 16, [40], [1], 700)
+    keep = p.tables.clone()
+    p.tables[0, 1] = 10 ** 9
+    got = p.run()
+    # the same as with the block's tokens left out: one softmax over the rest
+    vals = want.codes.double() * want.scales.double()[..., None, None]
+    ids = keep[0].long()
+    ids = torch.stack([ids[0], ids[2]])
+    k, v = (vals[i][ids, 0].reshape(-1, 64)[:24] for i in range(2))
+    for h in range(2):
+        o = torch.softmax((k @ want.q[0, h].double()) * want.scale, 0) @ v
+        assert float((got[0, h].cpu().double() - o).norm() / o.norm()) < 2e-3
+
+
+def test_special_values(gpu):
+    """A NaN key reaches its row alone; q without any number gives none; int8 zeros give zeros."""
+    p = Problem(gpu, "e4m3", 64, 2, 2, 16, [20, 20], [1, 1], 800)
+    p.codes[0].view(torch.uint8)[p.tables[0, 0], 0, 3, 5] = 0x7F
+    got = p.run()
+    assert bool(got[0, 0].isnan().all()) and bool(got[0, 1].isfinite().all()) and bool(got[1].isfinite().all())
+    z = Problem(gpu, "int8", 64, 2, 2, 16, [20, 20], [1, 1], 801)
+    z.codes.zero_()
+    assert bool((z.run() == 0).all())
+
+
+def test_strided_q_and_tables_on_another_stream(gpu):
+    """q inside a fused projection's rows, tables inside a wider tensor, on a stream of the caller's."""
+    p = Problem(gpu, "e4m3", 128, 4, 2, 32, [100, 7], [2, 1], 900)
+    wide = torch.randn(3, 8 * 128).half().to(gpu)
+    wide[:, :512] = p.q.flatten(1).to(gpu)
+    tabs = torch.full((2, 9), -3, dtype=torch.int32, device=gpu)
+    tabs[:, :p.tables.shape[1]] = p.tables.to(gpu)
+    d = lambda t: t.to(gpu)  # noqa: E731
+    args = [wide[:, :512].unflatten(1, (4, 128)), d(p.codes[0]), d(p.codes[1]), d(p.scales[0]), d(p.scales[1]),
+            tabs[:, :p.tables.shape[1]], d(p.lens), d(p.starts)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ext().kv_attention(*args, p.scale)
+    s.synchronize()
+    p.check(got)
+
+
+def test_long_cache_past_32_bits(gpu):
+    """Blocks whose bytes lie behind 4 GiB."""
+    dim, bs, heads = 256, 256, 8
+    blocks = (2 ** 32) // (heads * bs * dim) + 2
+    codes = [torch.zeros(blocks, heads, bs, dim, dtype=torch.int8, device=gpu) for _ in range(2)]
+    x = torch.randint(-127, 128, (2, heads, bs, dim), generator=gen(1000)).to(torch.int8)
+    for c, y in zip(codes, x):
+        c[-1] = y.to(gpu)
+    scale = torch.full((blocks, heads), 0.01, device=gpu)
+    q = torch.randn(1, heads, dim, generator=gen(1001)).half()
+    got = ext().kv_attention(q.to(gpu), *codes, scale, scale, torch.tensor([[blocks - 1]], dtype=torch.int32, device=gpu),
+                             torch.tensor([200], dtype=torch.int32, device=gpu),
+                             torch.tensor([0, 1], dtype=torch.int32, device=gpu), dim ** -0.5)
+    s = torch.full((1, heads), 0.01).double()
+    vals = x.double() * scale[0, 0].cpu().double()
+    want, bound = sv.attention(q, vals[:1], vals[1:], s, torch.tensor([[0]]), torch.tensor([200]), torch.tensor([0, 1]),
+                               dim ** -0.5)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
