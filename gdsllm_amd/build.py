@@ -39,6 +39,11 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
+# Flags of single sources.  kv_attention.hip: accumulators of matrix instructions
+# in ordinary registers, which its running maximum rescales (in accumulation
+# registers every rescaling moves them there and back).
+SOURCE_FLAGS = {"kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
@@ -65,7 +70,7 @@ def build_library(verbose: bool = False, jobs: int = 0) -> Path:
     cc = hipcc()
     jobs = jobs or min(len(sources), os.cpu_count() or 4, 16)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        futs = [ex.submit(_run, [cc, *HIPCC_FLAGS, "-c", str(s), "-o", str(o)], verbose) for s, o in zip(sources, objs)]
+        futs = [ex.submit(_run, [cc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(s.name, []), "-c", str(s), "-o", str(o)], verbose) for s, o in zip(sources, objs)]
         for f in futs:
             f.result()
     tmp = LIB.with_suffix(".so.tmp")

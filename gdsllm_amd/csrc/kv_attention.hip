@@ -24,32 +24,34 @@ namespace gdsllm {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSegment = 4096;       // tokens whose block table a workgroup holds in LDS
-constexpr int kMaxPages = kSegment / 16;
-constexpr int kWaves = 4;
+constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
+constexpr int kMaxPages = kSegment / 16;   // segments begin on a block of 64 tokens
+constexpr int kBlock = 64;                 // tokens of a unit of work
 
 struct AttendArgs {
     KvCache c;
     const uint16_t* q;
     uint16_t* o;
     const int32_t *tables, *lens, *starts;
-    float* part_o;   // [unit][16][D]
-    float* part_ml;  // [unit][16][2]
+    float* part_o;        // [2 * groups][16][D]: sums of a sequence's parts
+    float2* part_ml;      // [2 * groups][16]: maximum and weight sum of each row
+    int2* parts;          // [requests][tiles][kv_heads]: first part and their number (0: none)
     int64_t ldq, ldo, ld_table;
-    float scale_log2;  // scale * log2 e
+    float scale_log2;     // scale * log2 e
     int tokens, requests, q_heads, group, width;
-    int chunk, splits, tiles;  // tokens of a unit; units along a sequence; row tiles of a request that have units
-    int zero_tail;             // rows behind the last request are set to zero
+    int tiles;            // row tiles of a request that the grids have
+    int groups;           // workgroups that share the work evenly
+    int zero_tail;        // rows behind the last request are set to zero
 };
 
-// What this workgroup computes: a request's rows and the keys they may see.
+// A request's rows and the keys they may see.
 struct Rows {
     int start, n, len, rows;
     __device__ __forceinline__ Rows(const AttendArgs& a, int b) {
-        start = min(max(a.starts[b], 0), a.tokens);
-        n = min(max(a.starts[b + 1] - start, 0), a.tokens - start);
-        const int64_t most = static_cast<int64_t>(a.width) << a.c.block_log2;
-        len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), most));
+        const int s0 = a.starts[b], s1 = a.starts[b + 1], held = a.lens[b];
+        start = min(max(s0, 0), a.tokens);
+        n = min(max(s1 - start, 0), a.tokens - start);
+        len = min(max(held, 0), a.width << a.c.block_log2);
         rows = n * a.group;
     }
     // Keys that the last of rows [r0, r0 + count) sees.
@@ -57,58 +59,99 @@ struct Rows {
         const int last = (min(r0 + count, rows) - 1) / a.group;
         return max(len - n + last + 1, 0);
     }
+    __device__ __forceinline__ int tiles() const { return (rows + 15) / 16; }
+    // Blocks of kBlock tokens to each of its sequences (row tile and kv head).
+    __device__ __forceinline__ int blocks() const { return max((len + kBlock - 1) / kBlock, 1); }
+    __device__ __forceinline__ int work(const AttendArgs& a) const { return min(tiles(), a.tiles) * a.c.kv_heads * blocks(); }
 };
 
-__device__ __forceinline__ int chunks_of(const AttendArgs& a, int tile, int keys) {
-    if (tile >= a.tiles) return 1;
-    return min(max((keys + a.chunk - 1) / a.chunk, 1), a.splits);
-}
-
-// v from the other half of the wave (lanes l and l + 32), and from the other
-// 16 lanes of each half, combined with f.
+// f over the values of lanes l % 16 + {0, 16, 32, 48}: every lane gets the result.
 template <class F>
 __device__ __forceinline__ float over_groups(float v, F f) {
-    v = f(v, __shfl_xor(v, 16));
-    return f(v, __shfl_xor(v, 32));
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = f(a, b);
+    a = v, b = v;
+    swap32(a, b);
+    return f(a, b);
 }
 
-// Units (split, kv head and row tile, request): 16 rows over one chunk of
-// tokens.  Matrix tiles are 16x16x32 and nothing passes through LDS but the
-// block table:
+__device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
+
+__device__ __forceinline__ void zero_rows_behind(const AttendArgs& a, int D) {
+    if (!a.zero_tail) return;
+    for (int64_t t = min(max(a.starts[a.requests], 0), a.tokens) + blockIdx.x; t < a.tokens; t += gridDim.x)
+        for (int i = threadIdx.x; i < a.q_heads * D / 8; i += blockDim.x)
+            *reinterpret_cast<uint4*>(a.o + t * a.ldo + 8 * i) = make_uint4(0, 0, 0, 0);
+}
+
+// 16 rows over blocks [block0, block1) of a sequence, by NW waves.  Matrix tiles
+// are 16x16x32 and nothing passes through LDS but the block table and the waves'
+// sums:
 //  * scores S^T = K Q^T: lane l gives key row l % 16 and 16 of each 64 channels
-//    (one 16-byte load; Q's operand takes the same order), and receives, for query l % 16, tokens 4 * group .. + 3 of each 16;
+//    (one 16-byte load; Q's operand takes the same order), and receives, for
+//    query l % 16, tokens 4 * group .. + 3 of each 16;
 //  * O^T = V^T P^T: its B operand is exactly those eight weights of two score
 //    tiles, in place; V's operand needs eight tokens of one channel in a lane:
 //    lanes load D/16 channels of the eight tokens and transpose 4x4 bytes with
 //    v_perm.
-template <bool E4M3, int D>
-__global__ __launch_bounds__(kWaves * 64) void attend_rows(AttendArgs a) {
-    constexpr int KS = D / 32;               // score steps of 32 channels
-    constexpr int DB = D / 16;               // channels of V a lane holds
-    constexpr int VW = DB / 4;               // the same in dwords
-    constexpr int NT = D == 256 ? 2 : 4;     // score tiles of 16 tokens in an iteration
-    constexpr int TT = 16 * NT;
-    __shared__ int s_id[kMaxPages];
-    __shared__ float s_c[kMaxPages], s_e[kMaxPages], s_inv[kMaxPages];
-    __shared__ float s_o[2][16][D];
-    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+template <bool E4M3, int D, int NW_>
+struct RowTile {
+    static constexpr int NT = 2;        // score tiles of an iteration
+    static constexpr int NW = NW_;
+    static constexpr int KS = D / 32;   // score steps of 32 channels
+    static constexpr int DB = D / 16;   // channels of V a lane holds
+    static constexpr int VW = DB / 4;   // the same in dwords
+    static constexpr int TT = 16 * NT;  // tokens of an iteration
+    struct Codes {
+        uint32_t k[NT][D / 16];
+        uint32_t v[NT][4][VW];
+    };
+    struct Lds {
+        int id[kMaxPages];
+        float c[kMaxPages], e[kMaxPages], inv[kMaxPages];
+        float m[NW][16], l[NW][16];
+        float o[NW][16][D + 4];
+    };
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x, head = blockIdx.y % a.c.kv_heads, tile0 = blockIdx.y / a.c.kv_heads, b = blockIdx.z;
-    const int bl = a.c.block_log2;
-    if (a.zero_tail) {
-        const int64_t id = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * gridDim.x + split;
-        const int64_t groups = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z;
-        for (int64_t t = min(max(a.starts[a.requests], 0), a.tokens) + id; t < a.tokens; t += groups)
-            for (int i = tid; i < a.q_heads * D / 8; i += kWaves * 64)
-                *reinterpret_cast<uint4*>(a.o + t * a.ldo + 8 * i) = make_uint4(0, 0, 0, 0);
+    // Codes of 16 tokens from `kb` (`vb`) on, wave-uniform, into slot t.
+    __device__ __forceinline__ static void load_k(Codes& w, int t, const uint8_t* kb, uint32_t klane) {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + klane + 64 * i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.k[t][4 * i + j] = x[j];
+        }
     }
-    const Rows R(a, b);
-    for (int tile = tile0; tile * 16 < R.rows; tile += gridDim.y / a.c.kv_heads) {
-        const int keys = R.keys(a, tile * 16, 16);
-        const int chunks = chunks_of(a, tile, keys);
-        if (split >= chunks) continue;
-        const int k0 = split * a.chunk, k1 = split == chunks - 1 ? keys : min(k0 + a.chunk, keys);
+    __device__ __forceinline__ static void load_v(Codes& w, int t, const uint8_t* vb, uint32_t vlane) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint8_t* p = vb + vlane + i * D;
+            if constexpr (VW == 1) {
+                w.v[t][i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+            } else if constexpr (VW == 2) {
+                const uint64_t x = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(p));
+                w.v[t][i][0] = static_cast<uint32_t>(x);
+                w.v[t][i][1] = static_cast<uint32_t>(x >> 32);
+            } else {
+                const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w.v[t][i][j] = x[j];
+            }
+        }
+    }
+
+    // `slot` < 0: the sequence is whole, its rows are written to o; else its sums
+    // go to that part.  `early`: entry threadIdx.x of the request's block table,
+    // loaded ahead of its length (only where block0 is 0 and a thread has each
+    // entry of a segment), else -2.
+    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows& R, int tile, int head, int block0,
+                               int block1, int slot, int early) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15,
+                  g = lane >> 4;
+        const int bl = a.c.block_log2;
+        const uint32_t klane = col * D + 16 * g, vlane = 4 * g * D + col * DB;
+        const int k0 = block0 * kBlock, k1 = min(block1 * kBlock, R.keys(a, tile * 16, 16));
         const int r = tile * 16 + col;
         const bool valid = r < R.rows;
         const int t_row = R.start + (valid ? r / a.group : 0), h_row = head * a.group + (valid ? r % a.group : 0);
@@ -117,94 +160,101 @@ __global__ __launch_bounds__(kWaves * 64) void attend_rows(AttendArgs a) {
 
         half8_t qf[KS];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
+        for (int i = 0; i < KS; ++i) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (valid) w = *reinterpret_cast<const uint4*>(a.q + t_row * a.ldq + h_row * D + 64 * (s / 2) + 16 * g + 8 * (s & 1));
-            qf[s] = __builtin_bit_cast(half8_t, w);
+            if (valid) w = *reinterpret_cast<const uint4*>(a.q + t_row * a.ldq + h_row * D + 64 * (i / 2) + 16 * g + 8 * (i & 1));
+            qf[i] = __builtin_bit_cast(half8_t, w);
         }
         float4_t acc[DB];
 #pragma unroll
         for (int j = 0; j < DB; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
 
+        if (k1 <= k0) lds_barrier();
         for (int seg = k0; seg < k1; seg += kSegment) {
             const int seg_end = min(seg + kSegment, k1);
-            __syncthreads();
-            const int pages = ((min(seg + kSegment, (k1 + TT - 1) & ~(TT - 1)) - seg) + (1 << bl) - 1) >> bl;
+            const int p0 = seg >> bl, pages = ((min(seg + kSegment, (k1 + TT - 1) & ~(TT - 1)) - 1) >> bl) - p0 + 1;
+            lds_barrier();  // the last segment's table, or the last sequence's sums, have been read
             bool lost = false;
-            for (int p = tid; p < pages; p += kWaves * 64) {
-                const int page = (seg >> bl) + p;
-                const int id = page < a.width && (page << bl) < k1 ? a.tables[b * a.ld_table + page] : -1;
+            for (int p = tid; p < pages; p += NW * 64) {
+                const int page = p0 + p;
+                int id = -1;
+                if (page < a.width && (page << bl) < k1) id = early != -2 && seg == 0 ? early : a.tables[b * a.ld_table + page];
                 const bool ok = id >= 0 && id < a.c.num_blocks;
-                const int64_t sc = static_cast<int64_t>(ok ? id : 0) * a.c.kv_heads + head;
-                const float vs = fmaxf(a.c.v_scale[sc], 0x1p-64f);
-                s_id[p] = ok ? id : 0;
-                s_c[p] = a.c.k_scale[sc] * a.scale_log2;
-                s_e[p] = log2f(vs);
-                s_inv[p] = ok ? 1.f / vs : 0.f;
+                s.id[p] = ok ? id : 0;
+                s.inv[p] = ok ? 1.f : 0.f;
                 lost |= !ok && (page << bl) < k1;
             }
             const bool some_lost = __syncthreads_or(lost);
-            for (int base = seg + wave * TT; base < seg_end; base += kWaves * TT) {
-                uint32_t kw[NT][D / 16];
-                uint32_t vw[NT][4][VW];
+            auto row_of = [&](int token) {
+                const int id = __builtin_amdgcn_readfirstlane(s.id[(token >> bl) - p0]);
+                return (((static_cast<int64_t>(id) * a.c.kv_heads + head) << bl) + (token & ((1 << bl) - 1))) * D;
+            };
+            constexpr int step = NW * TT;
+            int base = seg + wave * TT;
+            // the scales, and behind them the first codes
+            float ks = 0.f, vs = 0.f;
+            int64_t sc = 0;
+            if (tid < pages) {
+                sc = static_cast<int64_t>(s.id[tid]) * a.c.kv_heads + head;
+                ks = a.c.k_scale[sc];
+                vs = a.c.v_scale[sc];
+            }
+            Codes w;
+            if (base < seg_end) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const int p = (base - seg + 16 * t) >> bl, off = (base + 16 * t) & ((1 << bl) - 1);
-                    const int64_t row = ((static_cast<int64_t>(s_id[p]) * a.c.kv_heads + head) << bl) + off;
-                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.c.k + (row + col) * D + 16 * g);
+                for (int t = 0; t < NT; ++t) load_k(w, t, a.c.k + row_of(base + 16 * t), klane);
 #pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const u32x4_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + 16 * i));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) kw[t][4 * i + j] = w[j];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint8_t* vp = a.c.v + (row + 4 * g + i) * D + col * DB;
-                        if constexpr (VW == 1) {
-                            vw[t][i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vp));
-                        } else if constexpr (VW == 2) {
-                            const uint64_t w = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(vp));
-                            vw[t][i][0] = static_cast<uint32_t>(w);
-                            vw[t][i][1] = static_cast<uint32_t>(w >> 32);
-                        } else {
-                            const u32x4_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vp));
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) vw[t][i][j] = w[j];
-                        }
-                    }
+                for (int t = 0; t < NT; ++t) load_v(w, t, a.c.v + row_of(base + 16 * t), vlane);
+            }
+            for (int p = tid; p < pages; p += NW * 64) {
+                if (p != tid) {
+                    sc = static_cast<int64_t>(s.id[p]) * a.c.kv_heads + head;
+                    ks = a.c.k_scale[sc];
+                    vs = a.c.v_scale[sc];
                 }
+                vs = fmaxf(vs, 0x1p-64f);
+                s.c[p] = ks * a.scale_log2;
+                s.e[p] = log2f(vs);
+                s.inv[p] = s.inv[p] / vs;
+            }
+            lds_barrier();
+            for (; base < seg_end; base += step) {
+                const bool more = base + step < seg_end;
                 float x[NT][4];
                 float mx = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    float4_t s = {0.f, 0.f, 0.f, 0.f};
+                    float4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
                         uint32_t f[4];
-                        codes_to_f16<E4M3>(kw[t][2 * i], f[0], f[1]);
-                        codes_to_f16<E4M3>(kw[t][2 * i + 1], f[2], f[3]);
+                        codes_to_f16<E4M3>(w.k[t][2 * i], f[0], f[1]);
+                        codes_to_f16<E4M3>(w.k[t][2 * i + 1], f[2], f[3]);
                         const half8_t kf = __builtin_bit_cast(half8_t, make_uint4(f[0], f[1], f[2], f[3]));
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i], s, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i], sum, 0, 0, 0);
                     }
-                    const int p = (base - seg + 16 * t) >> bl;
-                    const float c = s_c[p], e = s_e[p];
+                    const int p = ((base + 16 * t) >> bl) - p0;
+                    const float c = s.c[p], e = s.e[p];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[t][i] = fmaf(s[i], c, e);
+                    for (int i = 0; i < 4; ++i) x[t][i] = fmaf(sum[i], c, e);
+                }
+                if (more) {  // the keys' registers are free: the next tile's
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) load_k(w, t, a.c.k + row_of(base + step + 16 * t), klane);
                 }
                 if (base + TT - 1 > all_see || base + TT > k1 || some_lost) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         // a block outside the cache has no weight
-                        const bool none = s_inv[(base - seg + 16 * t) >> bl] == 0.f;
+                        const bool none = s.inv[((base + 16 * t) >> bl) - p0] == 0.f;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int j = base + 16 * t + 4 * g + i;
                             if (j > last || j >= k1 || none) x[t][i] = -INFINITY;
                             if (j >= k1 || none) {  // what lies there may be no number
 #pragma unroll
-                                for (int w = 0; w < VW; ++w) vw[t][i][w] = 0;
+                                for (int u = 0; u < VW; ++u) w.v[t][i][u] = 0;
                             }
                         }
                     }
@@ -226,7 +276,7 @@ __global__ __launch_bounds__(kWaves * 64) void attend_rows(AttendArgs a) {
                 half8_t pf[NT / 2];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const float inv = s_inv[(base - seg + 16 * t) >> bl];
+                    const float inv = s.inv[((base + 16 * t) >> bl) - p0];
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -239,146 +289,260 @@ __global__ __launch_bounds__(kWaves * 64) void attend_rows(AttendArgs a) {
 #pragma unroll
                 for (int u = 0; u < NT / 2; ++u)
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        // pairs[k]: tokens 2k, 2k+1 of the eight, channels 0, 1 (lo) and 2, 3 (hi)
+                    for (int c = 0; c < VW; ++c) {
                         uint32_t f[4][4];  // [channel][token pair]
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t t0 = vw[2 * u + k / 2][2 * (k & 1)][w], t1 = vw[2 * u + k / 2][2 * (k & 1) + 1][w];
+                            const uint32_t t0 = w.v[2 * u + k / 2][2 * (k & 1)][c], t1 = w.v[2 * u + k / 2][2 * (k & 1) + 1][c];
                             codes_to_f16<E4M3>(__builtin_amdgcn_perm(t1, t0, 0x05010400u), f[0][k], f[1][k]);
                             codes_to_f16<E4M3>(__builtin_amdgcn_perm(t1, t0, 0x07030602u), f[2][k], f[3][k]);
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const half8_t vf = __builtin_bit_cast(half8_t, make_uint4(f[j][0], f[j][1], f[j][2], f[j][3]));
-                            acc[4 * w + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[u], acc[4 * w + j], 0, 0, 0);
+                            acc[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[u], acc[4 * c + j], 0, 0, 0);
                         }
                     }
+                if (more) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) load_v(w, t, a.c.v + row_of(base + step + 16 * t), vlane);
+                }
             }
         }
         l = over_groups(l, [](float u, float v) { return u + v; });
 
-        // the four waves' sums, in a fixed order: (0 + 2) + (1 + 3)
+        // the waves' sums meet in LDS; every thread adds four channels of a row
         if (g == 0) {
-            s_m[wave][col] = m;
-            s_l[wave][col] = l;
+            s.m[wave][col] = m;
+            s.l[wave][col] = l;
         }
-        __syncthreads();
-        float mw = s_m[0][col];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) mw = fmaxf(mw, s_m[w][col]);
-        const float ref = mw == -INFINITY ? 0.f : mw;
-        const float f = __builtin_amdgcn_exp2f(m - ref);
-        l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) l = fmaf(s_l[w][col], __builtin_amdgcn_exp2f(s_m[w][col] - ref), l);
-#pragma unroll
-        for (int j = 0; j < DB; ++j) acc[j] *= f;
-        auto put = [&](float (*o)[D]) {
+        if (valid) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < DB; j += 4)
-                    *reinterpret_cast<float4_t*>(&o[col][(4 * g + i) * DB + j]) =
+                    *reinterpret_cast<float4_t*>(&s.o[wave][col][(4 * g + i) * DB + j]) =
                         float4_t{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
-        };
-        auto add = [&](float (*o)[D]) {
+        }
+        lds_barrier();
+        const int count = min(16, R.rows - tile * 16);
+        for (int i = tid; i < count * (D / 4); i += NW * 64) {
+            const int rr = i / (D / 4), d = 4 * (i % (D / 4));
+            float mw = s.m[0][rr];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int w = 1; w < NW; ++w) mw = fmaxf(mw, s.m[w][rr]);
+            const float ref = mw == -INFINITY ? 0.f : mw;
+            float lw = 0.f;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < DB; ++j) acc[j][i] += o[col][(4 * g + i) * DB + j];
-        };
-        if (wave >= 2) put(s_o[wave - 2]);
-        __syncthreads();
-        if (wave < 2) add(s_o[wave]);
-        __syncthreads();
-        if (wave == 1) put(s_o[0]);
-        __syncthreads();
-        if (wave == 0) {
-            add(s_o[0]);
-            if (chunks == 1) {
-                if (valid) {
-                    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-                    uint16_t* o = a.o + t_row * a.ldo + h_row * D;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < DB; j += 4) {
-                            uint2 w;
-                            w.x = pack_h2(static_cast<half_t>(acc[j][i] * inv), static_cast<half_t>(acc[j + 1][i] * inv));
-                            w.y = pack_h2(static_cast<half_t>(acc[j + 2][i] * inv), static_cast<half_t>(acc[j + 3][i] * inv));
-                            *reinterpret_cast<uint2*>(o + (4 * g + i) * DB + j) = w;
-                        }
-                }
-            } else if (valid) {
-                const int64_t unit = ((static_cast<int64_t>(b) * a.tiles + tile) * a.c.kv_heads + head) * a.splits + split;
-                float* o = a.part_o + (unit * 16 + col) * D;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < DB; j += 4)
-                        *reinterpret_cast<float4_t*>(o + (4 * g + i) * DB + j) =
-                            float4_t{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
-                if (g == 0) {
-                    a.part_ml[(unit * 16 + col) * 2] = mw;
-                    a.part_ml[(unit * 16 + col) * 2 + 1] = l;
-                }
+            for (int w = 0; w < NW; ++w) {
+                const float f = __builtin_amdgcn_exp2f(s.m[w][rr] - ref);
+                lw = fmaf(s.l[w][rr], f, lw);
+                o += *reinterpret_cast<const float4_t*>(&s.o[w][rr][d]) * f;
+            }
+            if (slot < 0) {
+                const float inv = inverse(lw);
+                const int row = tile * 16 + rr;
+                uint2 w;
+                w.x = pack_h2(static_cast<half_t>(o[0] * inv), static_cast<half_t>(o[1] * inv));
+                w.y = pack_h2(static_cast<half_t>(o[2] * inv), static_cast<half_t>(o[3] * inv));
+                *reinterpret_cast<uint2*>(a.o + (R.start + row / a.group) * a.ldo + (head * a.group + row % a.group) * D + d) = w;
+            } else {
+                *reinterpret_cast<float4_t*>(a.part_o + (static_cast<int64_t>(slot) * 16 + rr) * D + d) = o;
+                if (d == 0) a.part_ml[slot * 16 + rr] = make_float2(mw, lw);
             }
         }
     }
+};
+
+// One workgroup to a sequence (grid: row tiles times kv heads, requests).
+template <bool E4M3, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void attend_whole(AttendArgs a) {
+    using RT = RowTile<E4M3, D, NW>;
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    typename RT::Lds& s = *reinterpret_cast<typename RT::Lds*>(raw);
+    const int b = blockIdx.y, tid = threadIdx.x;
+    const int early = NW * 64 < kMaxPages ? -2 : tid < a.width ? a.tables[b * a.ld_table + tid] : -1;
+    const Rows R(a, b);
+    const int head = blockIdx.x % a.c.kv_heads;
+    for (int tile = blockIdx.x / a.c.kv_heads; tile < R.tiles(); tile += a.tiles)
+        RT::run(a, s, b, R, tile, head, 0, R.blocks(), -1, early);
+    if (b == 0) zero_rows_behind(a, D);
 }
 
-// Rows whose tokens were split: their units' sums joined in order.
-template <int D>
-__global__ __launch_bounds__(256) void attend_join(AttendArgs a) {
-    constexpr int TPR = D / 4;  // threads of a row
-    const int head = blockIdx.x % a.c.kv_heads, tile = blockIdx.x / a.c.kv_heads, b = blockIdx.y;
-    const Rows R(a, b);
-    if (tile * 16 >= R.rows) return;
-    const int chunks = chunks_of(a, tile, R.keys(a, tile * 16, 16));
-    if (chunks == 1) return;
-    const int64_t unit = ((static_cast<int64_t>(b) * a.tiles + tile) * a.c.kv_heads + head) * a.splits;
-    const int d = 4 * (threadIdx.x % TPR);
-    for (int r = threadIdx.x / TPR; r < 16 && tile * 16 + r < R.rows; r += 256 / TPR) {
-        const float* ml = a.part_ml + (unit * 16 + r) * 2;
-        float m = -INFINITY;
-        for (int s = 0; s < chunks; ++s) m = fmaxf(m, ml[s * 32]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < chunks; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[s * 32] - ref);
-            l = fmaf(ml[s * 32 + 1], f, l);
-            const float4_t p = *reinterpret_cast<const float4_t*>(a.part_o + ((unit + s) * 16 + r) * D + d);
-            o += p * f;
+// The work as one line of blocks: request after request, in each its row tiles,
+// kv heads and blocks of tokens, innermost last; `groups` workgroups take even
+// shares of it, so none waits for a long sequence.  Each sums the requests'
+// work for itself, 256 a step, and looks up where its share begins.  A sequence
+// that lies in several shares leaves a part in each: a workgroup has at most
+// two, the one its share begins with and the one it ends in.
+// Workgroups of attend_shared that a compute unit holds at once (registers: 16
+// rows of accumulators, a tile of codes and Q grow with D).  At D = 256 one, so
+// that a long sequence leaves half as many parts: 131072 tokens 36.8 us against
+// 41.1 with two.
+constexpr int per_cu(int64_t D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
+
+
+template <bool E4M3, int D>
+__global__ __launch_bounds__(256, per_cu(D)) void attend_shared(AttendArgs a) {
+    using RT = RowTile<E4M3, D, 4>;
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    typename RT::Lds& s = *reinterpret_cast<typename RT::Lds*>(raw);
+    __shared__ int s_part[4], s_request, s_begin;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wg = blockIdx.x;
+    zero_rows_behind(a, D);
+    int total = 0, share = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        int carry = 0;
+        for (int b0 = 0; b0 < a.requests; b0 += 256) {
+            const int b = b0 + tid, w = b < a.requests ? Rows(a, b).work(a) : 0;
+            int upto = w;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int u = __shfl_up(upto, o);
+                if (lane >= o) upto += u;
+            }
+            __syncthreads();
+            if (lane == 63) s_part[wave] = upto;
+            __syncthreads();
+            for (int i = 0; i < wave; ++i) upto += s_part[i];
+            const int begin = carry + upto - w;
+            carry += s_part[0] + s_part[1] + s_part[2] + s_part[3];
+            if (a.requests <= 256) {  // one step: the sum is all here
+                total = carry;
+                share = max((total + a.groups - 1) / a.groups, 4);
+            }
+            const int at = wg * share;
+            if (share > 0 && w > 0 && begin <= at && at < begin + w) s_request = b, s_begin = begin;
         }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int row = tile * 16 + r;
-        uint16_t* out = a.o + (R.start + row / a.group) * a.ldo + (head * a.group + row % a.group) * D + d;
-        uint2 w;
-        w.x = pack_h2(static_cast<half_t>(o[0] * inv), static_cast<half_t>(o[1] * inv));
-        w.y = pack_h2(static_cast<half_t>(o[2] * inv), static_cast<half_t>(o[3] * inv));
-        *reinterpret_cast<uint2*>(out) = w;
+        if (a.requests <= 256) break;
+        total = carry;
+        share = max((total + a.groups - 1) / a.groups, 4);
+    }
+    __syncthreads();
+    int at = wg * share, b = s_request, begin = s_begin;
+    const int end = min(at + share, total);
+    if (at >= end) return;
+    bool first = true;
+    while (at < end) {
+        Rows R(a, b);
+        while (at >= begin + R.work(a)) {
+            begin += R.work(a);
+            R = Rows(a, ++b);
+        }
+        const int blocks = R.blocks(), sequence = (at - begin) / blocks, block0 = at - begin - sequence * blocks;
+        const int block1 = min(blocks, block0 + end - at);
+        const int head = sequence % a.c.kv_heads, tile = sequence / a.c.kv_heads;
+        const bool whole = block0 == 0 && block1 == blocks;
+        const int slot = 2 * wg + (first ? 0 : 1);
+        if (block0 == 0 && tid == 0)
+            a.parts[(static_cast<int64_t>(b) * a.tiles + tile) * a.c.kv_heads + head] =
+                make_int2(slot, whole ? 0 : 1 + (blocks - block1 + share - 1) / share);
+        RT::run(a, s, b, R, tile, head, block0, block1, whole ? -1 : slot, -2);
+        if (block0 == 0)  // more rows than the caller said: whole, by whoever begins the tile below
+            for (int t = tile + a.tiles; t < R.tiles(); t += a.tiles) RT::run(a, s, b, R, t, head, 0, blocks, -1, -2);
+        at += block1 - block0;
+        first = false;
     }
 }
 
+// Sequences that several workgroups had a part of: one workgroup to a row adds
+// their sums.  Part 0 lies in slot `first`, part i in slot 2 * (first / 2 + i).
+// Its threads first take the parts' maxima and turn them into factors, then D/4
+// threads of four channels in each of NG groups run over every NGth part, and the groups' sums meet in LDS in a fixed order.
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
+    constexpr int TPR = D / 4, NG = THREADS / TPR, NWV = THREADS / 64, EARLY = 2;
+    __shared__ float s_f[THREADS], s_m[NWV], s_l[NWV];
+    __shared__ __attribute__((aligned(16))) float4_t s_o[THREADS];
+    const int b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
+    const int r = blockIdx.x % rows, sequence = blockIdx.x / rows;
+    const int head = sequence % a.c.kv_heads, row = sequence / a.c.kv_heads * 16 + r;
+    const int2 d = a.parts[static_cast<int64_t>(b) * a.tiles * a.c.kv_heads + sequence];
+    const Rows R(a, b);
+    if (row >= R.rows || d.y == 0) return;  // no such row (d is not set), or whole
+    const int parts = d.y;
+    auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * 16 + r; };
+    auto sums = [&](int i) { return *reinterpret_cast<const float4_t*>(a.part_o + at(i) * D + 4 * (tid % TPR)); };
+    // the first parts' sums come in while the factors are made
+    float4_t early[EARLY];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) {
+        const int i = tid / TPR + k * NG;
+        early[k] = i < parts ? sums(i) : float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const float2 mine = tid < parts ? a.part_ml[at(tid)] : make_float2(-INFINITY, 0.f);
+    float m = mine.x;
+    for (int i = tid + THREADS; i < parts; i += THREADS) m = fmaxf(m, a.part_ml[at(i)].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((tid & 63) == 0) s_m[wave] = m;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) m = fmaxf(m, s_m[i]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < parts; i0 += THREADS) {
+        if (i0 > 0) __syncthreads();
+        float w = 0.f;
+        if (i0 + tid < parts) {
+            const float2 x = i0 == 0 ? mine : a.part_ml[at(i0 + tid)];
+            w = __builtin_amdgcn_exp2f(x.x - ref);
+            l = fmaf(x.y, w, l);
+        }
+        s_f[tid] = w;
+        lds_barrier();
+        int i = tid / TPR;
+        if (i0 == 0) {
+#pragma unroll
+            for (int k = 0; k < EARLY; ++k, i += NG)
+                if (i < parts) acc += early[k] * s_f[i];
+        }
+        const int n = min(THREADS, parts - i0);
+#pragma unroll 8
+        for (; i < n; i += NG) acc += sums(i0 + i) * s_f[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    if ((tid & 63) == 0) s_l[wave] = l;
+    s_o[tid] = acc;
+    __syncthreads();
+    if (tid >= TPR) return;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) l += s_l[i];
+#pragma unroll
+    for (int i = 1; i < NG; ++i) acc += s_o[tid + i * TPR];
+    const float inv = inverse(l);
+    uint16_t* out = a.o + (R.start + row / a.group) * a.ldo + (head * a.group + row % a.group) * D + 4 * tid;
+    uint2 w;
+    w.x = pack_h2(static_cast<half_t>(acc[0] * inv), static_cast<half_t>(acc[1] * inv));
+    w.y = pack_h2(static_cast<half_t>(acc[2] * inv), static_cast<half_t>(acc[3] * inv));
+    *reinterpret_cast<uint2*>(out) = w;
+}
+
 struct Plan {
-    int tiles, splits, chunk;
-    int64_t units;
+    int64_t sequences;  // (request, row tile, kv head)
+    int groups;         // workgroups that share them; 0: one to a sequence
+    int tiles;
 };
 
-// Row tiles, chunk length and units of a call.  Enough units to give every
-// compute unit a few workgroups, none shorter than 256 tokens.
-Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_new, int64_t max_len) {
+constexpr int kCus = 256;  // compute units of the device: the workspace's size goes by it
+constexpr int64_t kWholeTokens = 2048;
+// One workgroup to a sequence where none is long or there are many of them, else
+// as many workgroups as the device holds at once, with even shares.
+Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
     Plan p;
     p.tiles = static_cast<int>(std::max<int64_t>(1, (max_new * (q_heads / kv_heads) + 15) / 16));
-    const int64_t lanes = requests * kv_heads * p.tiles;
-    int64_t chunk = (max_len * lanes / 1024 + 255) / 256 * 256;
-    chunk = std::min<int64_t>(std::max<int64_t>(chunk, 256), kSegment);
-    p.chunk = static_cast<int>(chunk);
-    p.splits = static_cast<int>(std::max<int64_t>(1, (max_len + chunk - 1) / chunk));
-    p.units = p.splits > 1 ? lanes * p.splits : 0;
+    p.sequences = requests * kv_heads * p.tiles;
+    const int64_t resident = per_cu(head_dim) * static_cast<int64_t>(kCus);
+    const bool whole = max_len <= kWholeTokens || p.sequences >= 8 * resident;
+    p.groups = whole ? 0 : static_cast<int>(std::min<int64_t>(resident, p.sequences * ((max_len + 255) / 256)));
     return p;
+}
+size_t attend_bytes(const Plan& p, int64_t head_dim) {
+    return p.groups ? static_cast<size_t>(p.groups) * 2 * 16 * (head_dim + 2) * sizeof(float) + p.sequences * sizeof(int2) : 0;
 }
 
 bool attend_sizes(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
@@ -395,8 +559,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return static_cast<size_t>(plan_attend(requests, q_heads, kv_heads, max_new, max_len).units) * 16 *
-           (head_dim + 2) * sizeof(float);
+    return attend_bytes(plan_attend(requests, q_heads, kv_heads, head_dim, max_new, max_len), head_dim);
 }
 
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
@@ -429,8 +592,8 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     if (max_len == 0 || max_len > most) max_len = most;
     if (!attend_sizes(requests, q_heads, cache->kv_heads, D, max_new, max_len)) return bad("sizes out of range");
     if (requests == 0) return bad("no requests for the tokens");
-    const Plan p = plan_attend(requests, q_heads, cache->kv_heads, max_new, max_len);
-    const size_t need = static_cast<size_t>(p.units) * 16 * (D + 2) * sizeof(float);
+    const Plan p = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len);
+    const size_t need = attend_bytes(p, D);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return bad("workspace of " + std::to_string(need) + " bytes needed, got " + std::to_string(workspace_bytes));
     a.q = static_cast<const uint16_t*>(q);
@@ -439,7 +602,8 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.lens = lens;
     a.starts = starts;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + p.units * 16 * D;
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<int64_t>(p.groups) * 2 * 16 * D);
+    a.parts = reinterpret_cast<int2*>(a.part_ml + static_cast<int64_t>(p.groups) * 2 * 16);
     a.ldq = ldq;
     a.ldo = ldo;
     a.ld_table = ld_table;
@@ -449,21 +613,40 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.q_heads = static_cast<int>(q_heads);
     a.group = static_cast<int>(q_heads / cache->kv_heads);
     a.width = static_cast<int>(table_width);
-    a.chunk = p.chunk;
-    a.splits = p.splits;
     a.tiles = p.tiles;
     a.zero_tail = zero_tail;
-    const int64_t y = std::min<int64_t>(p.tiles, 65535 / cache->kv_heads) * cache->kv_heads;
-    const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(y), static_cast<unsigned>(requests));
+    // the line of blocks is counted in 32 bits
+    const int64_t line = ((tokens * a.group + 15) / 16 + requests) * cache->kv_heads * (most / kBlock + 1);
+    a.groups = line < (int64_t(1) << 31) ? p.groups : 0;
+    const int64_t per_request = static_cast<int64_t>(p.tiles) * cache->kv_heads;
+    const int rows = static_cast<int>(std::min<int64_t>(16, max_new * a.group));
+    if (per_request * 16 > (int64_t(1) << 31) - 1) return bad("too many rows for one call");
+    const dim3 whole(static_cast<unsigned>(per_request), static_cast<unsigned>(requests));
+    const dim3 join(static_cast<unsigned>(per_request * rows), static_cast<unsigned>(requests));
+    const bool few = p.sequences * rows <= kCus;  // long sequences in many parts each
     const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
     const hipStream_t s = as_stream(stream);
-#define GDSLLM_ATTEND(DIM)                                                                            \
-    if (D == DIM) {                                                                                   \
-        if (e4m3) hipLaunchKernelGGL((attend_rows<true, DIM>), grid, dim3(kWaves * 64), 0, s, a);     \
-        else hipLaunchKernelGGL((attend_rows<false, DIM>), grid, dim3(kWaves * 64), 0, s, a);         \
-        if (p.splits > 1)                                                                             \
-            hipLaunchKernelGGL(attend_join<DIM>, dim3(static_cast<unsigned>(p.tiles * cache->kv_heads), \
-                                                      static_cast<unsigned>(requests)), dim3(256), 0, s, a); \
+    auto launch = [&](auto kernel, dim3 grid, int threads, size_t lds) {
+        if (int rc = prepare_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, a);
+        return static_cast<int>(GDSLLM_OK);
+    };
+    int rc = GDSLLM_OK;
+#define GDSLLM_ATTEND(DIM)                                                                                     \
+    if (D == DIM) {                                                                                            \
+        if (a.groups) {                                                                                        \
+            const size_t lds = sizeof(RowTile<true, DIM, 4>::Lds);                                         \
+            rc = e4m3 ? launch(attend_shared<true, DIM>, dim3(a.groups), 256, lds)                         \
+                      : launch(attend_shared<false, DIM>, dim3(a.groups), 256, lds);                       \
+            if (rc) return rc;                                                                                 \
+            if (few) hipLaunchKernelGGL((attend_join<DIM, 1024>), join, dim3(1024), 0, s, a, rows);            \
+            else hipLaunchKernelGGL((attend_join<DIM, 256>), join, dim3(256), 0, s, a, rows);                  \
+        } else {                                                                                               \
+            const size_t lds = sizeof(RowTile<true, DIM, 8>::Lds);                                       \
+            rc = e4m3 ? launch(attend_whole<true, DIM, 8>, whole, 512, lds)                          \
+                      : launch(attend_whole<false, DIM, 8>, whole, 512, lds);                        \
+            if (rc) return rc;                                                                                 \
+        }                                                                                                      \
     }
     GDSLLM_ATTEND(64)
     GDSLLM_ATTEND(128)
