@@ -17,11 +17,14 @@
 // the 16 columns of one matrix tile (row r = token r / G, head r % G).
 
 #include <algorithm>
+#include <climits>
 
 #include "kv_cache.h"
 
 namespace gdsllm {
 namespace {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
@@ -33,18 +36,20 @@ struct AttendArgs {
     const uint16_t* q;
     uint16_t* o;
     const int32_t *tables, *lens, *starts;
-    float* part_o;        // [2 * groups][16][D]: sums of a sequence's parts
-    float2* part_ml;      // [2 * groups][16]: maximum and weight sum of each row
-    int2* parts;          // [requests][tiles][kv_heads]: first part and their number (0: none)
+    float* part_o;           // [2 * groups][rows of a tile][D]: sums of a sequence's parts
+    float2* part_ml;         // [2 * groups][rows of a tile]: maximum and weight sum of each row
+    int2* parts;             // [requests][tiles][kv_heads]: first part and their number (0: none)
     int64_t ldq, ldo, ld_table;
-    float scale_log2;     // scale * log2 e
+    float scale_log2;        // scale * log2 e
     int tokens, requests, q_heads, group, width;
-    int tiles;            // row tiles of a request that the grids have
-    int groups;           // workgroups that share the work evenly
-    int zero_tail;        // rows behind the last request are set to zero
+    int min_rows, max_rows;  // requests with other numbers of rows are left to another launch
+    int tiles;               // row tiles of a request that the grids have
+    int groups;              // workgroups that share the work evenly
+    int zero_tail;           // rows behind the last request are set to zero
 };
 
-// A request's rows and the keys they may see.
+// A request's rows, in tiles of RT, and the keys they may see.
+template <int RT>
 struct Rows {
     int start, n, len, rows;
     __device__ __forceinline__ Rows(const AttendArgs& a, int b) {
@@ -53,13 +58,14 @@ struct Rows {
         n = min(max(s1 - start, 0), a.tokens - start);
         len = min(max(held, 0), a.width << a.c.block_log2);
         rows = n * a.group;
+        if (rows < a.min_rows || rows > a.max_rows) rows = 0;
     }
     // Keys that the last of rows [r0, r0 + count) sees.
     __device__ __forceinline__ int keys(const AttendArgs& a, int r0, int count) const {
         const int last = (min(r0 + count, rows) - 1) / a.group;
         return max(len - n + last + 1, 0);
     }
-    __device__ __forceinline__ int tiles() const { return (rows + 15) / 16; }
+    __device__ __forceinline__ int tiles() const { return (rows + RT - 1) / RT; }
     // Blocks of kBlock tokens to each of its sequences (row tile and kv head).
     __device__ __forceinline__ int blocks() const { return max((len + kBlock - 1) / kBlock, 1); }
     __device__ __forceinline__ int work(const AttendArgs& a) const { return min(tiles(), a.tiles) * a.c.kv_heads * blocks(); }
@@ -75,6 +81,12 @@ __device__ __forceinline__ float over_groups(float v, F f) {
     swap32(a, b);
     return f(a, b);
 }
+
+// Workgroups of attend_shared that a compute unit holds at once (registers: 16
+// rows of accumulators, a tile of codes and Q grow with D).  At D = 256 one, so
+// that a long sequence leaves half as many parts: 131072 tokens 36.8 us against
+// 41.1 with two.
+constexpr int per_cu(int64_t D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
 
 __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
 
@@ -97,6 +109,8 @@ __device__ __forceinline__ void zero_rows_behind(const AttendArgs& a, int D) {
 //    v_perm.
 template <bool E4M3, int D, int NW_>
 struct RowTile {
+    static constexpr int kRows = 16, kD = D, kPerCu = per_cu(D);
+    static constexpr int kThreads = NW_ * 64;
     static constexpr int NT = 2;        // score tiles of an iteration
     static constexpr int NW = NW_;
     static constexpr int KS = D / 32;   // score steps of 32 channels
@@ -145,7 +159,7 @@ struct RowTile {
     // go to that part.  `early`: entry threadIdx.x of the request's block table,
     // loaded ahead of its length (only where block0 is 0 and a thread has each
     // entry of a segment), else -2.
-    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows& R, int tile, int head, int block0,
+    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows<16>& R, int tile, int head, int block0,
                                int block1, int slot, int early) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15,
                   g = lane >> 4;
@@ -355,19 +369,266 @@ struct RowTile {
     }
 };
 
-// One workgroup to a sequence (grid: row tiles times kv heads, requests).
-template <bool E4M3, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void attend_whole(AttendArgs a) {
-    using RT = RowTile<E4M3, D, NW>;
+// 128 rows over blocks [block0, block1) of a sequence, 32 rows to each of four
+// waves, for prompts.  BN tokens at a time are converted to fp16 once, into LDS
+// (two buffers, one barrier a tile), while the tile before is worked on; matrix
+// tiles are 32x32x16:
+//  * S^T = K Q^T: K [token][channel] from LDS, Q in registers; lane l receives,
+//    for query l % 32, tokens 8b + 4h + j of each 32 (h = l / 32);
+//  * O^T = V^T P^T: again those weights are the B operand in place, eight tokens
+//    16u + 8(i/4) + 4h + i%4 to a lane, and V lies in LDS transposed, [channel]
+//    [token], with its tokens in that order, so its operand is one 16-byte read.
+// The four-token pieces of V^T come from 4x4 byte transposes of the codes.  Rows
+// of both tiles are 16 bytes longer than their data: reads and writes touch
+// every bank once.
+template <bool E4M3, int D>
+struct PromptTile {
+    static constexpr int kRows = 128, kThreads = 256, kD = D, kPerCu = D == 256 ? 1 : 2;
+    static constexpr int BN = D == 256 ? 32 : 64;
+    static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
+    static constexpr int KC = BN * D / 16 / 256;                  // 16-code chunks of K a thread converts
+    static constexpr int VQ = BN / 4, VC = VQ * (D / 8), VN = (VC + 255) / 256;  // token quads; (quad, 8 channels) pieces
+    struct Page {
+        float c, e, inv;
+        int id;
+    };
+    struct Lds {
+        Page page[kMaxPages];
+        uint16_t k[2][BN][D + 8];
+        uint16_t v[2][D][BN + 8];
+    };
+    struct Codes {
+        u32x4_t k[KC];
+        uint64_t v[VN][4];
+    };
+
+    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows<128>& R, int tile, int head, int block0,
+                               int block1, int slot, int early) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31,
+                  h = lane >> 5;
+        const int bl = a.c.block_log2;
+        const int k0 = block0 * kBlock, k1 = min(block1 * kBlock, R.keys(a, tile * 128, 128));
+        const int w0 = tile * 128 + wave * 32;  // this wave's rows
+        const int r = w0 + col;
+        const bool valid = r < R.rows;
+        const int t_row = R.start + (valid ? r / a.group : 0), h_row = head * a.group + (valid ? r % a.group : 0);
+        const int last = valid ? R.len - R.n + r / a.group : -1;
+        const int all_see = R.len - R.n + w0 / a.group;
+        const int k1w = w0 < R.rows ? min(k1, R.keys(a, w0, 32)) : 0;  // keys that this wave's rows see
+
+        half8_t qf[KS];
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (valid) w = *reinterpret_cast<const uint4*>(a.q + t_row * a.ldq + h_row * D + 16 * i + 8 * h);
+            qf[i] = __builtin_bit_cast(half8_t, w);
+        }
+        float16_t acc[DT];
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
+        float m = -INFINITY, l = 0.f;
+
+        if (k1 <= k0) lds_barrier();
+        for (int seg = k0; seg < k1; seg += kSegment) {
+            const int seg_end = min(seg + kSegment, k1);
+            const int p0 = seg >> bl, pages = ((min(seg + kSegment, (k1 + BN - 1) & ~(BN - 1)) - 1) >> bl) - p0 + 1;
+            lds_barrier();
+            bool lost = false;
+            for (int p = tid; p < pages; p += kThreads) {
+                const int page = p0 + p;
+                int id = -1;
+                if (page < a.width && (page << bl) < k1) id = early != -2 && seg == 0 ? early : a.tables[b * a.ld_table + page];
+                const bool ok = id >= 0 && id < a.c.num_blocks;
+                const int64_t sc = static_cast<int64_t>(ok ? id : 0) * a.c.kv_heads + head;
+                const float vs = fmaxf(a.c.v_scale[sc], 0x1p-64f);
+                s.page[p] = {fmaxf(a.c.k_scale[sc], 0x1p-64f) * a.scale_log2, log2f(vs), ok ? 1.f / vs : 0.f, ok ? id : 0};
+                lost |= !ok && (page << bl) < k1;
+            }
+            const bool some_lost = __syncthreads_or(lost);
+
+            auto load = [&](Codes& w, int base) {
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    const int c = tid + 256 * i, token = base + c / (D / 16);
+                    const int64_t row = ((static_cast<int64_t>(s.page[(token >> bl) - p0].id) * a.c.kv_heads + head) << bl) +
+                                        (token & ((1 << bl) - 1));
+                    w.k[i] = *reinterpret_cast<const u32x4_t*>(a.c.k + row * D + 16 * (c % (D / 16)));
+                }
+#pragma unroll
+                for (int i = 0; i < VN; ++i) {
+                    const int c = tid + 256 * i, token = base + 4 * (c % VQ);
+                    if (VC % 256 == 0 || c < VC) {
+                        const int64_t row = ((static_cast<int64_t>(s.page[(token >> bl) - p0].id) * a.c.kv_heads + head) << bl) +
+                                            (token & ((1 << bl) - 1));
+                        const uint8_t* p = a.c.v + row * D + 8 * (c / VQ);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w.v[i][j] = *reinterpret_cast<const uint64_t*>(p + j * D);
+                    }
+                }
+            };
+            auto store = [&](Codes& w, int base, int buf) {
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    const int c = tid + 256 * i;
+                    uint32_t f[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) codes_to_f16<E4M3>(w.k[i][j], f[2 * j], f[2 * j + 1]);
+                    uint4* p = reinterpret_cast<uint4*>(&s.k[buf][c / (D / 16)][16 * (c % (D / 16))]);
+                    p[0] = make_uint4(f[0], f[1], f[2], f[3]);
+                    p[1] = make_uint4(f[4], f[5], f[6], f[7]);
+                }
+                const bool tail = base + BN > k1 || some_lost;
+#pragma unroll
+                for (int i = 0; i < VN; ++i) {
+                    const int c = tid + 256 * i, quad = c % VQ;
+                    if (VC % 256 == 0 || c < VC) {
+                        if (tail) {  // what lies behind the last token, or in a lost block, may be no number
+                            const int token = base + 4 * quad;
+                            const bool none = s.page[(token >> bl) - p0].inv == 0.f;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (none || token + j >= k1) w.v[i][j] = 0;
+                        }
+                        const int pos = 16 * (quad / 4) + 8 * (quad & 1) + 4 * ((quad >> 1) & 1);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t t[4], f[4][2];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) t[j] = static_cast<uint32_t>(w.v[i][j] >> (32 * x));
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                codes_to_f16<E4M3>(__builtin_amdgcn_perm(t[2 * k + 1], t[2 * k], 0x05010400u), f[0][k], f[1][k]);
+                                codes_to_f16<E4M3>(__builtin_amdgcn_perm(t[2 * k + 1], t[2 * k], 0x07030602u), f[2][k], f[3][k]);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                *reinterpret_cast<uint2*>(&s.v[buf][8 * (c / VQ) + 4 * x + j][pos]) = make_uint2(f[j][0], f[j][1]);
+                        }
+                    }
+                }
+            };
+
+            Codes w;
+            load(w, seg);
+            store(w, seg, 0);
+            lds_barrier();
+            int buf = 0;
+            for (int base = seg; base < seg_end; base += BN, buf ^= 1) {
+                const bool more = base + BN < seg_end;
+                if (more) load(w, base + BN);
+                if (base < k1w) {
+                    float16_t x[ST];
+#pragma unroll
+                    for (int t = 0; t < ST; ++t) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) {
+                            const half8_t kf = *reinterpret_cast<const half8_t*>(&s.k[buf][32 * t + col][16 * i + 8 * h]);
+                            x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[t], 0, 0, 0);
+                        }
+                    }
+                    if (base + BN - 1 > all_see || base + BN > k1 || some_lost) {
+#pragma unroll
+                        for (int t = 0; t < ST; ++t)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int j = base + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
+                                if (j > last || j >= k1 || (some_lost && s.page[(j >> bl) - p0].inv == 0.f)) x[t][i] = -INFINITY;
+                            }
+                    }
+                    Page pg[U];
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        pg[u] = s.page[((base + 16 * u) >> bl) - p0];
+                        const float16_t& y = x[u / 2];
+                        const int o = 8 * (u & 1);
+                        const float g = fmaxf(fmaxf(fmaxf(y[o], y[o + 1]), fmaxf(y[o + 2], y[o + 3])),
+                                              fmaxf(fmaxf(y[o + 4], y[o + 5]), fmaxf(y[o + 6], y[o + 7])));
+                        mx = fmaxf(mx, fmaf(g, pg[u].c, pg[u].e));
+                    }
+                    {
+                        float p = mx, q = mx;
+                        swap32(p, q);
+                        mx = fmaxf(p, q);
+                    }
+                    const float m_new = fmaxf(m, mx);
+                    const float ref = m_new == -INFINITY ? 0.f : m_new;
+                    if (__any(m_new > m)) {
+                        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+                        l *= alpha;
+#pragma unroll
+                        for (int j = 0; j < DT; ++j) acc[j] *= alpha;
+                        m = m_new;
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const float er = pg[u].e - ref;
+                        half8_t pf;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            pf[i] = static_cast<half_t>(__builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u & 1) + i], pg[u].c, er)));
+                        const uint4 pw = __builtin_bit_cast(uint4, pf);
+                        constexpr uint32_t ones = 0x3C003C00u;
+                        l = fmaf(dot2(pw.x, ones, dot2(pw.y, ones, dot2(pw.z, ones, dot2(pw.w, ones, 0.f)))), pg[u].inv, l);
+#pragma unroll
+                        for (int j = 0; j < DT; ++j) {
+                            const half8_t vf = *reinterpret_cast<const half8_t*>(&s.v[buf][32 * j + col][16 * u + 8 * h]);
+                            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, acc[j], 0, 0, 0);
+                        }
+                    }
+                }
+                if (more) store(w, base + BN, buf ^ 1);
+                lds_barrier();
+            }
+        }
+        {
+            float p = l, q = l;
+            swap32(p, q);
+            l = p + q;
+        }
+        if (!valid) return;
+        if (slot < 0) {
+            const float inv = inverse(l);
+            uint16_t* o = a.o + t_row * a.ldo + h_row * D;
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    uint2 w;
+                    w.x = pack_h2(static_cast<half_t>(acc[j][i] * inv), static_cast<half_t>(acc[j][i + 1] * inv));
+                    w.y = pack_h2(static_cast<half_t>(acc[j][i + 2] * inv), static_cast<half_t>(acc[j][i + 3] * inv));
+                    *reinterpret_cast<uint2*>(o + 32 * j + 2 * i + 4 * h) = w;
+                }
+        } else {
+            const int64_t row = static_cast<int64_t>(slot) * 128 + wave * 32 + col;
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4_t*>(a.part_o + row * D + 32 * j + 2 * i + 4 * h) =
+                        float4_t{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]};
+            if (h == 0) a.part_ml[row] = make_float2(m, l);
+        }
+    }
+};
+
+// One workgroup to a sequence (grid: row tiles times kv heads, requests).  Later
+// tiles see more keys: they are dealt first.
+template <class T>
+__global__ __launch_bounds__(T::kThreads) void attend_whole(AttendArgs a) {
     extern __shared__ __attribute__((aligned(16))) char raw[];
-    typename RT::Lds& s = *reinterpret_cast<typename RT::Lds*>(raw);
+    typename T::Lds& s = *reinterpret_cast<typename T::Lds*>(raw);
     const int b = blockIdx.y, tid = threadIdx.x;
-    const int early = NW * 64 < kMaxPages ? -2 : tid < a.width ? a.tables[b * a.ld_table + tid] : -1;
-    const Rows R(a, b);
+    const int early = T::kThreads < kMaxPages ? -2 : tid < a.width ? a.tables[b * a.ld_table + tid] : -1;
+    const Rows<T::kRows> R(a, b);
     const int head = blockIdx.x % a.c.kv_heads;
-    for (int tile = blockIdx.x / a.c.kv_heads; tile < R.tiles(); tile += a.tiles)
-        RT::run(a, s, b, R, tile, head, 0, R.blocks(), -1, early);
-    if (b == 0) zero_rows_behind(a, D);
+    for (int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / a.c.kv_heads; tile < R.tiles(); tile += a.tiles)
+        T::run(a, s, b, R, tile, head, 0, R.blocks(), -1, early);
+    if (b == 0) zero_rows_behind(a, T::kD);
 }
 
 // The work as one line of blocks: request after request, in each its row tiles,
@@ -376,26 +637,20 @@ __global__ __launch_bounds__(NW * 64) void attend_whole(AttendArgs a) {
 // work for itself, 256 a step, and looks up where its share begins.  A sequence
 // that lies in several shares leaves a part in each: a workgroup has at most
 // two, the one its share begins with and the one it ends in.
-// Workgroups of attend_shared that a compute unit holds at once (registers: 16
-// rows of accumulators, a tile of codes and Q grow with D).  At D = 256 one, so
-// that a long sequence leaves half as many parts: 131072 tokens 36.8 us against
-// 41.1 with two.
-constexpr int per_cu(int64_t D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
 
-
-template <bool E4M3, int D>
-__global__ __launch_bounds__(256, per_cu(D)) void attend_shared(AttendArgs a) {
-    using RT = RowTile<E4M3, D, 4>;
+template <class T>
+__global__ __launch_bounds__(256, T::kPerCu) void attend_shared(AttendArgs a) {
+    static_assert(T::kThreads == 256, "the sums over requests go 256 a step");
     extern __shared__ __attribute__((aligned(16))) char raw[];
-    typename RT::Lds& s = *reinterpret_cast<typename RT::Lds*>(raw);
+    typename T::Lds& s = *reinterpret_cast<typename T::Lds*>(raw);
     __shared__ int s_part[4], s_request, s_begin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wg = blockIdx.x;
-    zero_rows_behind(a, D);
+    zero_rows_behind(a, T::kD);
     int total = 0, share = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int carry = 0;
         for (int b0 = 0; b0 < a.requests; b0 += 256) {
-            const int b = b0 + tid, w = b < a.requests ? Rows(a, b).work(a) : 0;
+            const int b = b0 + tid, w = b < a.requests ? Rows<T::kRows>(a, b).work(a) : 0;
             int upto = w;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -425,10 +680,10 @@ __global__ __launch_bounds__(256, per_cu(D)) void attend_shared(AttendArgs a) {
     if (at >= end) return;
     bool first = true;
     while (at < end) {
-        Rows R(a, b);
+        Rows<T::kRows> R(a, b);
         while (at >= begin + R.work(a)) {
             begin += R.work(a);
-            R = Rows(a, ++b);
+            R = Rows<T::kRows>(a, ++b);
         }
         const int blocks = R.blocks(), sequence = (at - begin) / blocks, block0 = at - begin - sequence * blocks;
         const int block1 = min(blocks, block0 + end - at);
@@ -438,9 +693,9 @@ __global__ __launch_bounds__(256, per_cu(D)) void attend_shared(AttendArgs a) {
         if (block0 == 0 && tid == 0)
             a.parts[(static_cast<int64_t>(b) * a.tiles + tile) * a.c.kv_heads + head] =
                 make_int2(slot, whole ? 0 : 1 + (blocks - block1 + share - 1) / share);
-        RT::run(a, s, b, R, tile, head, block0, block1, whole ? -1 : slot, -2);
+        T::run(a, s, b, R, tile, head, block0, block1, whole ? -1 : slot, -2);
         if (block0 == 0)  // more rows than the caller said: whole, by whoever begins the tile below
-            for (int t = tile + a.tiles; t < R.tiles(); t += a.tiles) RT::run(a, s, b, R, t, head, 0, blocks, -1, -2);
+            for (int t = tile + a.tiles; t < R.tiles(); t += a.tiles) T::run(a, s, b, R, t, head, 0, blocks, -1, -2);
         at += block1 - block0;
         first = false;
     }
@@ -450,19 +705,19 @@ __global__ __launch_bounds__(256, per_cu(D)) void attend_shared(AttendArgs a) {
 // their sums.  Part 0 lies in slot `first`, part i in slot 2 * (first / 2 + i).
 // Its threads first take the parts' maxima and turn them into factors, then D/4
 // threads of four channels in each of NG groups run over every NGth part, and the groups' sums meet in LDS in a fixed order.
-template <int D, int THREADS>
+template <int RT, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
     constexpr int TPR = D / 4, NG = THREADS / TPR, NWV = THREADS / 64, EARLY = 2;
     __shared__ float s_f[THREADS], s_m[NWV], s_l[NWV];
     __shared__ __attribute__((aligned(16))) float4_t s_o[THREADS];
     const int b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const int r = blockIdx.x % rows, sequence = blockIdx.x / rows;
-    const int head = sequence % a.c.kv_heads, row = sequence / a.c.kv_heads * 16 + r;
+    const int head = sequence % a.c.kv_heads, row = sequence / a.c.kv_heads * RT + r;
     const int2 d = a.parts[static_cast<int64_t>(b) * a.tiles * a.c.kv_heads + sequence];
-    const Rows R(a, b);
+    const Rows<RT> R(a, b);
     if (row >= R.rows || d.y == 0) return;  // no such row (d is not set), or whole
     const int parts = d.y;
-    auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * 16 + r; };
+    auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * RT + r; };
     auto sums = [&](int i) { return *reinterpret_cast<const float4_t*>(a.part_o + at(i) * D + 4 * (tid % TPR)); };
     // the first parts' sums come in while the factors are made
     float4_t early[EARLY];
@@ -522,27 +777,101 @@ __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
     *reinterpret_cast<uint2*>(out) = w;
 }
 
+// One launch of a call: the requests with min_rows to max_rows rows, in tiles of
+// `rows` of them.
+struct Part {
+    bool on = false;
+    int rows = 0, min_rows = 0, max_rows = INT_MAX, tiles = 0;
+    int64_t sequences = 0;  // (request, row tile, kv head)
+    int groups = 0;         // workgroups that share them; 0: one to a sequence
+    size_t sums = 0, bytes = 0;
+};
 struct Plan {
-    int64_t sequences;  // (request, row tile, kv head)
-    int groups;         // workgroups that share them; 0: one to a sequence
-    int tiles;
+    Part few, many;
+    size_t bytes() const { return few.bytes + many.bytes; }
 };
 
 constexpr int kCus = 256;  // compute units of the device: the workspace's size goes by it
+// Requests with more rows than this take 128-row tiles, the others 16-row ones.
+constexpr int kFewRows = 32;
 constexpr int64_t kWholeTokens = 2048;
+
+void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int64_t max_len,
+                 int64_t resident, bool whole) {
+    p->on = true;
+    p->tiles = static_cast<int>(std::max<int64_t>(1, (max_rows + p->rows - 1) / p->rows));
+    p->sequences = requests * kv_heads * p->tiles;
+    p->groups = whole ? 0 : static_cast<int>(std::min<int64_t>(resident, p->sequences * ((max_len + 255) / 256)));
+    p->sums = static_cast<size_t>(p->groups) * 2 * p->rows;
+    p->bytes = p->groups ? p->sums * (head_dim + 2) * sizeof(float) + p->sequences * sizeof(int2) : 0;
+    p->bytes = (p->bytes + 15) / 16 * 16;
+}
+
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.
 Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
     Plan p;
-    p.tiles = static_cast<int>(std::max<int64_t>(1, (max_new * (q_heads / kv_heads) + 15) / 16));
-    p.sequences = requests * kv_heads * p.tiles;
-    const int64_t resident = per_cu(head_dim) * static_cast<int64_t>(kCus);
-    const bool whole = max_len <= kWholeTokens || p.sequences >= 8 * resident;
-    p.groups = whole ? 0 : static_cast<int>(std::min<int64_t>(resident, p.sequences * ((max_len + 255) / 256)));
+    const int64_t rows = max_new * (q_heads / kv_heads);
+    const bool many = rows > kFewRows;
+    if (!many || requests > 1) {
+        p.few.rows = 16;
+        if (many) p.few.max_rows = kFewRows;
+        const int64_t most = many ? kFewRows : rows, resident = per_cu(head_dim) * static_cast<int64_t>(kCus);
+        const int64_t sequences = requests * kv_heads * ((most + 15) / 16);
+        finish_part(&p.few, requests, kv_heads, head_dim, most, max_len, resident,
+                    max_len <= kWholeTokens || sequences >= 8 * resident);
+    }
+    if (many) {
+        p.many.rows = 128;
+        if (p.few.on) p.many.min_rows = kFewRows + 1;
+        const int64_t resident = (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus);
+        const int64_t sequences = requests * kv_heads * ((rows + 127) / 128);
+        finish_part(&p.many, requests, kv_heads, head_dim, rows, max_len, resident,
+                    max_len <= kWholeTokens || 2 * sequences >= resident);
+    }
     return p;
 }
-size_t attend_bytes(const Plan& p, int64_t head_dim) {
-    return p.groups ? static_cast<size_t>(p.groups) * 2 * 16 * (head_dim + 2) * sizeof(float) + p.sequences * sizeof(int2) : 0;
+
+// Launches one part of a call: W where a workgroup has a whole sequence, S where
+// the work is shared out.
+template <class W, class S>
+int launch_part(AttendArgs a, const Part& p, int64_t line, int64_t max_rows, char* workspace, hipStream_t s) {
+    if (!p.on) return GDSLLM_OK;
+    a.min_rows = p.min_rows;
+    a.max_rows = p.max_rows;
+    a.tiles = p.tiles;
+    a.part_o = reinterpret_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.sums * S::kD);
+    a.parts = reinterpret_cast<int2*>(a.part_ml + p.sums);
+    a.groups = line < (int64_t(1) << 31) ? p.groups : 0;  // the line of blocks is counted in 32 bits
+    const unsigned per_request = static_cast<unsigned>(p.tiles) * a.c.kv_heads, requests = a.requests;
+    if (a.groups == 0) {
+        const size_t lds = sizeof(typename W::Lds);
+        if (int rc = prepare_lds(reinterpret_cast<const void*>(&attend_whole<W>), lds)) return rc;
+        hipLaunchKernelGGL(attend_whole<W>, dim3(per_request, requests), dim3(W::kThreads), lds, s, a);
+        return check_hip(hipGetLastError(), "kv_attention launch");
+    }
+    const size_t lds = sizeof(typename S::Lds);
+    if (int rc = prepare_lds(reinterpret_cast<const void*>(&attend_shared<S>), lds)) return rc;
+    hipLaunchKernelGGL(attend_shared<S>, dim3(a.groups), dim3(256), lds, s, a);
+    const int rows = static_cast<int>(std::min<int64_t>(S::kRows, std::max<int64_t>(1, max_rows)));
+    const dim3 join(per_request * rows, requests);
+    // few sequences are long, in many parts each
+    if (p.sequences * rows <= kCus)
+        hipLaunchKernelGGL((attend_join<S::kRows, S::kD, 1024>), join, dim3(1024), 0, s, a, rows);
+    else
+        hipLaunchKernelGGL((attend_join<S::kRows, S::kD, 256>), join, dim3(256), 0, s, a, rows);
+    return check_hip(hipGetLastError(), "kv_attention launch");
+}
+
+template <bool E4M3, int D>
+int launch_attend(AttendArgs a, const Plan& p, int64_t line, int64_t max_rows, char* workspace, hipStream_t s) {
+    const int zero_tail = a.zero_tail;
+    a.zero_tail = p.few.on ? zero_tail : 0;
+    if (int rc = launch_part<RowTile<E4M3, D, 8>, RowTile<E4M3, D, 4>>(a, p.few, line, p.many.on ? kFewRows : max_rows, workspace, s))
+        return rc;
+    a.zero_tail = p.few.on ? 0 : zero_tail;
+    return launch_part<PromptTile<E4M3, D>, PromptTile<E4M3, D>>(a, p.many, line, max_rows, workspace + p.few.bytes, s);
 }
 
 bool attend_sizes(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
@@ -559,7 +888,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return attend_bytes(plan_attend(requests, q_heads, kv_heads, head_dim, max_new, max_len), head_dim);
+    return plan_attend(requests, q_heads, kv_heads, head_dim, max_new, max_len).bytes();
 }
 
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
@@ -578,6 +907,7 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     if (table_width < 1 || ld_table < table_width) return bad("ld_table < table_width or an empty table");
     if (table_width > ((int64_t(1) << 31) - 1) / cache->block_size) return bad("table_width too large");
     if (max_new < 0 || max_len < 0) return bad("negative max_new or max_len");
+    if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
     if (tokens == 0) return ok();
     if (!q || !o || !starts || (requests > 0 && (!block_tables || !lens))) return bad("null pointer");
     if (ldq < q_heads * D || ldo < q_heads * D) return bad("row stride smaller than a row");
@@ -593,7 +923,7 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     if (!attend_sizes(requests, q_heads, cache->kv_heads, D, max_new, max_len)) return bad("sizes out of range");
     if (requests == 0) return bad("no requests for the tokens");
     const Plan p = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len);
-    const size_t need = attend_bytes(p, D);
+    const size_t need = p.bytes();
     if (need > 0 && (!workspace || workspace_bytes < need))
         return bad("workspace of " + std::to_string(need) + " bytes needed, got " + std::to_string(workspace_bytes));
     a.q = static_cast<const uint16_t*>(q);
@@ -601,9 +931,6 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.tables = block_tables;
     a.lens = lens;
     a.starts = starts;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<int64_t>(p.groups) * 2 * 16 * D);
-    a.parts = reinterpret_cast<int2*>(a.part_ml + static_cast<int64_t>(p.groups) * 2 * 16);
     a.ldq = ldq;
     a.ldo = ldo;
     a.ld_table = ld_table;
@@ -613,45 +940,21 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.q_heads = static_cast<int>(q_heads);
     a.group = static_cast<int>(q_heads / cache->kv_heads);
     a.width = static_cast<int>(table_width);
-    a.tiles = p.tiles;
     a.zero_tail = zero_tail;
-    // the line of blocks is counted in 32 bits
+    const int64_t max_rows = max_new * a.group;
+    if (max_rows / 16 * 16 * cache->kv_heads > (int64_t(1) << 30)) return bad("too many rows for one call");
     const int64_t line = ((tokens * a.group + 15) / 16 + requests) * cache->kv_heads * (most / kBlock + 1);
-    a.groups = line < (int64_t(1) << 31) ? p.groups : 0;
-    const int64_t per_request = static_cast<int64_t>(p.tiles) * cache->kv_heads;
-    const int rows = static_cast<int>(std::min<int64_t>(16, max_new * a.group));
-    if (per_request * 16 > (int64_t(1) << 31) - 1) return bad("too many rows for one call");
-    const dim3 whole(static_cast<unsigned>(per_request), static_cast<unsigned>(requests));
-    const dim3 join(static_cast<unsigned>(per_request * rows), static_cast<unsigned>(requests));
-    const bool few = p.sequences * rows <= kCus;  // long sequences in many parts each
     const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
     const hipStream_t s = as_stream(stream);
-    auto launch = [&](auto kernel, dim3 grid, int threads, size_t lds) {
-        if (int rc = prepare_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
-        hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, a);
-        return static_cast<int>(GDSLLM_OK);
-    };
+    char* ws = static_cast<char*>(workspace);
     int rc = GDSLLM_OK;
-#define GDSLLM_ATTEND(DIM)                                                                                     \
-    if (D == DIM) {                                                                                            \
-        if (a.groups) {                                                                                        \
-            const size_t lds = sizeof(RowTile<true, DIM, 4>::Lds);                                         \
-            rc = e4m3 ? launch(attend_shared<true, DIM>, dim3(a.groups), 256, lds)                         \
-                      : launch(attend_shared<false, DIM>, dim3(a.groups), 256, lds);                       \
-            if (rc) return rc;                                                                                 \
-            if (few) hipLaunchKernelGGL((attend_join<DIM, 1024>), join, dim3(1024), 0, s, a, rows);            \
-            else hipLaunchKernelGGL((attend_join<DIM, 256>), join, dim3(256), 0, s, a, rows);                  \
-        } else {                                                                                               \
-            const size_t lds = sizeof(RowTile<true, DIM, 8>::Lds);                                       \
-            rc = e4m3 ? launch(attend_whole<true, DIM, 8>, whole, 512, lds)                          \
-                      : launch(attend_whole<false, DIM, 8>, whole, 512, lds);                        \
-            if (rc) return rc;                                                                                 \
-        }                                                                                                      \
-    }
+#define GDSLLM_ATTEND(DIM)                                                          \
+    if (D == DIM)                                                                   \
+        rc = e4m3 ? launch_attend<true, DIM>(a, p, line, max_rows, ws, s)           \
+                  : launch_attend<false, DIM>(a, p, line, max_rows, ws, s);
     GDSLLM_ATTEND(64)
     GDSLLM_ATTEND(128)
     GDSLLM_ATTEND(256)
 #undef GDSLLM_ATTEND
-    if (int rc = check_hip(hipGetLastError(), "kv_attention launch")) return rc;
-    return ok();
+    return rc ? rc : ok();
 }

@@ -488,8 +488,8 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * last of its lens[r] tokens: row i of n sees tokens 0 .. lens[r]-n+i; a row
  * that sees none is zero.  Query head h reads kv head h / (q_heads / kv_heads).
  * Products of fp16 and code values in fp32, softmax in fp32, weights rounded
- * to fp16 before the product with the values.  Scales must be positive; blocks
- * outside the cache have no weight.
+ * to fp16 before the product with the values.  scale and the cache's scales must
+ * be positive; blocks outside the cache have no weight.
  * max_new and max_len: bounds on a request's rows and tokens, known to the host
  * (0: tokens, and table_width * block_size).  They set how the work is split;
  * larger requests than they say are computed all the same, more slowly.

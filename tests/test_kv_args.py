@@ -68,8 +68,8 @@ def test_append_refusals():
 
 def test_attention_refusals():
     def call(c=None, q=16, ldq=128, o=16, ldo=128, n=1, hq=2, tab=16, w=1, ldt=1, lens=16, st=16, b=1, new=1, ml=16, ws=None,
-             wb=0):
-        return capi().gdsllm_kv_attention(c or _cache(), q, ldq, o, ldo, n, hq, tab, w, ldt, lens, st, b, 1.0, new, ml, 0,
+             wb=0, scale=1.0):
+        return capi().gdsllm_kv_attention(c or _cache(), q, ldq, o, ldo, n, hq, tab, w, ldt, lens, st, b, scale, new, ml, 0,
                                           ws, wb, None)
 
     assert call(n=0) == 0
@@ -86,6 +86,8 @@ def test_attention_refusals():
     assert call(b=70000) == BAD and "requests" in _err()
     assert call(b=0) == BAD and "requests" in _err()
     assert call(new=-1) == BAD and call(ml=-1) == BAD
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert call(scale=scale) == BAD and "scale" in _err()
     # a sequence long enough to be split needs its workspace
     lib = capi()
     need = lib.gdsllm_kv_attention_workspace_size(1, 2, 2, 64, 1, 16 * 1000)
