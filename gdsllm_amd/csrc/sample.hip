@@ -35,15 +35,38 @@ struct SampleArgs {
     int vocab;
 };
 
+// 2^y for y <= 0 in 64 bits: the nearest whole number goes to the exponent, the
+// rest f (|f| <= 1/2) through sum (f ln 2)^k / k!, k <= 13, whose remainder is
+// below 2^-57 of the result.
+__device__ __forceinline__ double exp2_neg(double y) {
+    y = fmax(y, -1100.0);
+    const double n = __builtin_rint(y), f = y - n;
+    double p = 1.3691488853904128e-12;   // ln2^13 / 13!, and down
+    p = fma(p, f, 2.5678435993488206e-11);
+    p = fma(p, f, 4.4455382718708116e-10);
+    p = fma(p, f, 7.0549116208011234e-09);
+    p = fma(p, f, 1.0178086009239699e-07);
+    p = fma(p, f, 1.3215486790144309e-06);
+    p = fma(p, f, 1.5252733804059841e-05);
+    p = fma(p, f, 1.5403530393381609e-04);
+    p = fma(p, f, 1.3333558146428443e-03);
+    p = fma(p, f, 9.6181291076284772e-03);
+    p = fma(p, f, 5.5504108664821580e-02);
+    p = fma(p, f, 2.4022650695910072e-01);
+    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, static_cast<int>(n));
+}
+
 struct RowParams {
-    double u, t, top_p, min_p;
+    double u, c, top_p, min_p;  // c: log2 e / temperature
     int top_k;
     bool greedy;
     __device__ __forceinline__ RowParams(const SampleArgs& a, int row) {
-        const float temperature = a.temperature ? a.temperature[row] : 1.f;
-        greedy = !(temperature > 0.f);
-        t = temperature;
-        const float uu = a.u ? a.u[row] : 0.f;
+        const float t = a.temperature ? a.temperature[row] : 1.f;
+        greedy = !(t > 0.f);
+        c = 1.4426950408889634074 / static_cast<double>(t);
+        const float uu = a.u[row];
         u = uu > 0.f ? (uu < 1.f ? static_cast<double>(uu) : 1.0) : 0.0;
         top_k = a.top_k ? a.top_k[row] : 0;
         const float p = a.top_p ? a.top_p[row] : 1.f;
@@ -51,28 +74,41 @@ struct RowParams {
         const float mp = a.min_p ? a.min_p[row] : 0.f;
         min_p = mp > 0.f ? static_cast<double>(mp) : 0.0;
     }
+    // exp((l - m) / temperature), m the largest logit: 1 at l = m, also where both are infinite.
     __device__ __forceinline__ double weight(float l, float m) const {
-        if (l == m) return 1.0;
-        return m == INFINITY ? 0.0 : exp((static_cast<double>(l) - static_cast<double>(m)) / t);
+        if (m == INFINITY) return l == m ? 1.0 : 0.0;
+        return exp2_neg((static_cast<double>(l) - static_cast<double>(m)) * c);
     }
 };
 
-// Inclusive sums over a wave.
-template <class T>
-__device__ __forceinline__ T wave_scan(T v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
+// Inclusive sums over a wave, in 16-lane rows (DPP shifts) and then across them
+// (DPP broadcasts of lanes 15 and 31).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_shift(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_shift(uint64_t v) {
+    const uint32_t lo = dpp_shift<CTRL, ROWS>(static_cast<int>(v)), hi = dpp_shift<CTRL, ROWS>(static_cast<int>(v >> 32));
+    return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_shift(double v) {
+    return __builtin_bit_cast(double, dpp_shift<CTRL, ROWS>(__builtin_bit_cast(uint64_t, v)));
 }
 template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp_shift<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_shift<0x112, 0xF>(v);
+    v += dpp_shift<0x114, 0xF>(v);
+    v += dpp_shift<0x118, 0xF>(v);
+    v += dpp_shift<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += dpp_shift<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
     return v;
 }
+// Lane 63's value, in every lane.
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ int wave_sum(int v) { return last_lane(wave_scan(v)); }
 
 // Rank of an fp16 value among all of them, 0 for +inf, rising as the value
 // falls; +0 and -0 share one.  No token: NaN and -inf.
@@ -158,14 +194,14 @@ __device__ int nth_index(const R& rd, int which, uint32_t none, F match, int* wa
 #pragma unroll
                 for (int j = 0; j < R::N; ++j) c += match(x[j]) ? 1 : 0;
             }
-            const int upto = wave_scan(c, lane);
+            const int upto = wave_scan(c);
             if (left >= upto - c && left < upto) {
                 int k = left - (upto - c);
 #pragma unroll
                 for (int j = 0; j < R::N; ++j)
                     if (match(x[j]) && k-- == 0) *answer = rd.index(gr) + j;
             }
-            left -= __shfl(upto, 63);
+            left -= last_lane(upto);
             if (left < 0) break;
         }
     }
@@ -241,31 +277,30 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a, int* overfl
     if (!P.greedy) {
         const float top = value16(first);
         auto bin_count = [&](uint32_t bin) { return static_cast<int>((s.hist[bin >> 1] >> (16 * (bin & 1))) & 0xFFFFu); };
-        // counts and masses of the rows of bins, and the tokens that min_p keeps
-        int kept = 0;
-        for (int r = wave; r < kBinRows; r += kWaves) {
-            const int c = bin_count(64 * r + lane);
-            double w = 0.0;
-            if (__any(c > 0)) {
-                if (c > 0) w = P.weight(value16(64 * r + lane), top);
+        // Counts and masses of the rows of bins, a row to a thread (each starts at
+        // a word of its own, so the threads of a wave read different banks), and the
+        // tokens that min_p keeps.
+        int kept = 0, row_n = 0;
+        double row_w = 0.0;
+        for (int i = 0; i < 32; ++i) {
+            const int j = (i + tid) & 31;
+            const uint32_t two = s.hist[32 * tid + j];
+            if (!two) continue;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = (two >> (16 * k)) & 0xFFFFu;
+                if (!c) continue;
+                const double w = P.weight(value16(64 * tid + 2 * j + k), top);
                 if (w >= P.min_p) kept += c;
-                w *= c;
-                w = wave_sum(w);
-            }
-            const int n = wave_sum(c);
-            if (lane == 0) {
-                s.mass[r] = w;
-                s.count[r] = n;
+                row_n += c;
+                row_w = fma(w, static_cast<double>(c), row_w);
             }
         }
         kept = wave_sum(kept);
         if (lane == 0) atomicAdd(&s.kept, kept);
-        __syncthreads();
-        // inclusive sums over the rows, one row a thread
-        const int row_n = s.count[tid];
-        const double row_w = s.mass[tid];
-        int upto_n = wave_scan(row_n, lane);
-        double upto_w = wave_scan(row_w, lane);
+        // inclusive sums over the rows
+        int upto_n = wave_scan(row_n);
+        double upto_w = wave_scan(row_w);
         if (lane == 63) {
             s.part_count[wave] = upto_n;
             s.part_mass[wave] = upto_w;
@@ -306,8 +341,8 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a, int* overfl
             }
             const int c = bin_count(64 * r + lane);
             const double w = c > 0 ? P.weight(value16(64 * r + lane), top) : 0.0;
-            const int cu = wave_scan(c, lane) + (r > 0 ? s.count[r - 1] : 0);
-            const double wu = wave_scan(w * c, lane) + (r > 0 ? s.mass[r - 1] : 0.0);
+            const int cu = wave_scan(c) + (r > 0 ? s.count[r - 1] : 0);
+            const double wu = wave_scan(w * c) + (r > 0 ? s.mass[r - 1] : 0.0);
             const bool hit = c > 0 && !miss && (by_count ? cu >= n : past ? wu > m : wu >= m);
             const uint64_t some = __ballot(hit), any = __ballot(c > 0);
             const int l = some ? __builtin_ctzll(some) : 63 - __builtin_clzll(any);
@@ -325,27 +360,41 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a, int* overfl
             }
             return p;
         };
-        int n = total;
+        int n = total, cut = total;
         double mass = all;
-        if (P.top_k > 0 && P.top_k < n) {
-            n = P.top_k;
-            const Place p = find(true, n, 0.0, false);
-            mass = p.mass + p.in_bin * p.w;
-        }
-        int cut = n;
-        if (P.top_p < 1.0) {
-            const Place p = find(false, 0, P.top_p * mass, false);
-            cut = min(cut, max(p.count + p.in_bin, 1));
-        }
-        cut = max(min(cut, s.kept), 1);
-        if (cut < n) {
-            const Place p = find(true, cut, 0.0, false);
-            mass = p.mass + p.in_bin * p.w;
-        }
-        at = find(false, 0, P.u * mass, true);
-        if (at.count + at.in_bin >= cut) {
-            at = find(true, cut, 0.0, false);
-            at.in_bin -= 1;
+#pragma nounroll
+        for (int stage = 0; stage < 5; ++stage) {
+            bool by_count = true, past = false;
+            int number = 0;
+            double amount = 0.0;
+            if (stage == 0) {  // the first top_k and their mass
+                if (P.top_k <= 0 || P.top_k >= n) continue;
+                number = n = cut = P.top_k;
+            } else if (stage == 1) {  // of those, top_p of their mass
+                if (P.top_p >= 1.0) continue;
+                by_count = false;
+                amount = P.top_p * mass;
+            } else if (stage == 2) {  // of those, what min_p keeps; the mass of the kept
+                cut = max(min(cut, s.kept), 1);
+                if (cut == n) continue;
+                number = cut;
+            } else if (stage == 3) {  // the draw
+                by_count = false;
+                past = true;
+                amount = P.u * mass;
+            } else {  // rounding put it behind the last kept token
+                if (at.count + at.in_bin < cut) continue;
+                number = cut;
+            }
+            const Place p = find(by_count, number, amount, past);
+            if (stage == 1) {
+                cut = min(cut, max(p.count + p.in_bin, 1));
+            } else if (stage < 3) {
+                mass = p.mass + p.in_bin * p.w;
+            } else {
+                at = p;
+                at.in_bin -= stage == 4 ? 1 : 0;
+            }
         }
     }
     const int i = nth_index(rd, at.in_bin, none, [&](uint32_t x) { return !no_token16(x) && rank16(x) == at.bin; },
@@ -357,36 +406,37 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a, int* overfl
 
 constexpr int kLevel1 = 4096;  // rank >> 20
 constexpr int kLevel2 = 1024;  // (rank >> 10) & 1023; rank & 1023 the third
+constexpr int kListed = 12288;
 
 struct Lds32 {
-    uint64_t mass[kLevel1];
-    uint32_t count[kLevel1];
-    uint64_t part_mass[kWaves];
-    int part_count[kWaves];
-    int kept, found, answer, counted;
+    uint64_t mass1[kLevel1], mass2[kLevel2];
+    uint64_t part_mass[kWaves], before_mass, sum;
+    uint32_t count1[kLevel1], count2[kLevel2];
+    uint32_t list[kListed];  // ranks of the tokens in level-1 bin `listed`
     uint32_t first;
-    uint64_t before_mass;
-    int before_count;
+    int part_count[kWaves], before_count, kept, found, answer, counted, length;
 };
 
 // One row over 32-bit ranks.  Masses are sums of w in units of 2^-shift, whole
-// numbers, so that atomics may add them in any order.
+// numbers, so that atomics may add them in any order.  The tokens are counted by
+// the upper 12 bits of their rank once; a place is then looked for in its bin
+// alone, whose ranks are listed in LDS where they fit.
 template <class E>
 __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* only_rows, int shift) {
-    __shared__ Lds32 s;
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    Lds32& s = *reinterpret_cast<Lds32*>(raw);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
     if (only_rows && only_rows[row] == 0) return;
     const RowReader<E, 4> rd(static_cast<const E*>(a.logits) + row * a.ld, a.vocab);
     const RowParams P(a, row);
-    constexpr int N = 4;
     constexpr uint32_t none = sizeof(E) == 2 ? 0xFFFFu : 0xFFFFFFFFu;  // a NaN
     auto bits = [](uint32_t x) { return sizeof(E) == 2 ? __builtin_bit_cast(uint32_t, h2f(x)) : x; };
     auto each = [&](auto f) {
         for (int gr = tid; gr < rd.granules(); gr += kThreads) {
-            uint32_t x[N];
+            uint32_t x[4];
             rd.load(gr, none, x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const uint32_t b = bits(x[j]);
                 if (!no_token32(b)) f(rank32(b));
             }
@@ -396,7 +446,9 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
         s.first = 0xFFFFFFFFu;
         s.kept = 0;
         s.counted = 0;
+        s.sum = 0;
     }
+    for (int i = tid; i < kLevel1; i += kThreads) s.count1[i] = 0, s.mass1[i] = 0;
     __syncthreads();
     uint32_t first = 0xFFFFFFFFu;
     int counted = 0;
@@ -422,45 +474,68 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
     if (!P.greedy) {
         const float top = value32(first);
         const double unit = ldexp(1.0, shift), back = ldexp(1.0, -shift);
-        auto fixed = [&](uint32_t r) {
-            return static_cast<unsigned long long>(P.weight(value32(r), top) * unit + 0.5);
+        auto add = [&](uint32_t bin, uint32_t r, uint32_t* count, uint64_t* mass) {
+            const double w = P.weight(value32(r), top);
+            const unsigned long long m = static_cast<unsigned long long>(w * unit + 0.5);
+            atomicAdd(&count[bin], 1u);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), m);
+            return w;
         };
-        // Fills the histogram of one level: ranks whose bits above `low + width`
-        // equal those of `prefix`.
-        auto fill = [&](int low, int bins, uint32_t prefix, bool all_ranks, bool with_mass) {
+        int kept = 0;
+        each([&](uint32_t r) { kept += add(r >> 20, r, s.count1, s.mass1) >= P.min_p ? 1 : 0; });
+        kept = wave_sum(kept);
+        if (lane == 0) atomicAdd(&s.kept, kept);
+        __syncthreads();
+        for (int i = tid; i < kLevel1; i += kThreads)
+            if (s.mass1[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sum), static_cast<unsigned long long>(s.mass1[i]));
+        __syncthreads();
+        int listed = -1;
+        // Brings the ranks of level-1 bin `bin` into the list.
+        auto list = [&](int bin) {
+            if (bin == listed) return;
+            listed = bin;
             __syncthreads();
-            for (int i = tid; i < bins; i += kThreads) {
-                s.count[i] = 0;
-                s.mass[i] = 0;
-            }
+            if (tid == 0) s.length = 0;
             __syncthreads();
-            each([&](uint32_t r) {
-                if (!all_ranks && (r >> (low + 10)) != prefix) return;
-                const uint32_t bin = (r >> low) & (bins - 1);
-                atomicAdd(&s.count[bin], 1u);
-                if (with_mass) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), fixed(r));
-            });
+            if (s.count1[bin] <= kListed)
+                each([&](uint32_t r) {
+                    if (static_cast<int>(r >> 20) == bin) s.list[atomicAdd(&s.length, 1)] = r;
+                });
+        };
+        // Counts the tokens whose rank above bit low + 10 is `prefix` by the ten bits from `low` on.
+        auto fill = [&](int low, uint32_t prefix, int bin) {
+            __syncthreads();
+            for (int i = tid; i < kLevel2; i += kThreads) s.count2[i] = 0, s.mass2[i] = 0;
+            __syncthreads();
+            auto one = [&](uint32_t r) {
+                if ((r >> (low + 10)) == prefix) add((r >> low) & (kLevel2 - 1), r, s.count2, s.mass2);
+            };
+            if (s.count1[bin] <= kListed)
+                for (int i = tid; i < s.length; i += kThreads) one(s.list[i]);
+            else each(one);
             __syncthreads();
         };
         // The bin of this level in which the place lies, and what lies before it
-        // (added to n0, m0).  The histogram is left as it was.
-        auto search = [&](int bins, bool by_count, int n, uint64_t m, bool past, int& n0, uint64_t& m0) {
-            const int per = bins / kThreads > 0 ? bins / kThreads : 1;
+        // (added to n0, m0).
+        auto search = [&](const uint32_t* count, const uint64_t* mass, int bins, bool by_count, int n, uint64_t m,
+                          bool past, int& n0, uint64_t& m0) {
+            const int per = bins / kThreads;
             int c = 0;
             uint64_t w = 0;
-            const bool on = tid * per < bins;
-            if (on)
-                for (int i = 0; i < per; ++i) {
-                    c += s.count[tid * per + i];
-                    w += s.mass[tid * per + i];
-                }
-            int cu = wave_scan(c, lane);
-            uint64_t wu = wave_scan(static_cast<unsigned long long>(w), lane);
+            for (int i = 0; i < per; ++i) {
+                c += count[tid * per + i];
+                w += mass[tid * per + i];
+            }
+            int cu = wave_scan(c);
+            uint64_t wu = wave_scan(w);
             if (lane == 63) {
                 s.part_count[wave] = cu;
                 s.part_mass[wave] = wu;
             }
-            if (tid == 0) s.found = -1;
+            if (tid == 0) {
+                s.found = -1;
+                s.answer = -1;
+            }
             __syncthreads();
             for (int v = 0; v < wave; ++v) {
                 cu += s.part_count[v];
@@ -470,38 +545,34 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
             uint64_t wa = m0 + wu - w;
             int last = -1, last_c = 0;  // the place if no bin reaches it: the last that has tokens
             uint64_t last_w = 0;
-            if (on)
-                for (int i = 0; i < per; ++i) {
-                    const int bc = s.count[tid * per + i];
-                    const uint64_t bw = s.mass[tid * per + i];
-                    if (bc > 0) {
-                        const bool before = by_count ? ca < n : past ? wa <= m : (wa < m || ca == 0);
-                        const bool reached = by_count ? ca + bc >= n : past ? wa + bw > m : wa + bw >= m;
-                        if (before && reached && atomicCAS(&s.found, -1, tid * per + i) == -1) {
-                            s.before_count = ca;
-                            s.before_mass = wa;
-                        }
-                        last = tid * per + i;
-                        last_c = ca;
-                        last_w = wa;
+            for (int i = 0; i < per; ++i) {
+                const int bc = count[tid * per + i];
+                const uint64_t bw = mass[tid * per + i];
+                if (bc > 0) {
+                    const bool before = by_count ? ca < n : past ? wa <= m : (wa < m || ca == 0);
+                    const bool reached = by_count ? ca + bc >= n : past ? wa + bw > m : wa + bw >= m;
+                    if (before && reached && atomicCAS(&s.found, -1, tid * per + i) == -1) {
+                        s.before_count = ca;
+                        s.before_mass = wa;
                     }
-                    ca += bc;
-                    wa += bw;
+                    last = tid * per + i;
+                    last_c = ca;
+                    last_w = wa;
                 }
+                ca += bc;
+                wa += bw;
+            }
+            if (last >= 0) atomicMax(&s.answer, last);
             __syncthreads();
-            if (s.found < 0) {
-                if (tid == 0) s.answer = -1;
-                __syncthreads();
-                if (last >= 0) atomicMax(&s.answer, last);
-                __syncthreads();
+            int f = s.found;
+            if (f < 0) {
                 if (last >= 0 && s.answer == last) {
-                    s.found = last;
                     s.before_count = last_c;
                     s.before_mass = last_w;
                 }
+                f = s.answer;
                 __syncthreads();
             }
-            const int f = s.found;
             n0 = s.before_count;
             m0 = s.before_mass;
             __syncthreads();
@@ -511,13 +582,13 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
             const uint64_t m = static_cast<uint64_t>(fmax(mass, 0.0) * unit + (past ? 0.0 : 0.5));
             int n0 = 0;
             uint64_t m0 = 0;
-            fill(20, kLevel1, 0, true, true);
-            uint32_t bin = search(kLevel1, by_count, n, m, past, n0, m0);
-            fill(10, kLevel2, bin, false, true);
-            bin = (bin << 10) | search(kLevel2, by_count, n, m, past, n0, m0);
-            fill(0, kLevel2, bin, false, true);
-            const uint32_t low = search(kLevel2, by_count, n, m, past, n0, m0);
-            const int bc = s.count[low];
+            const uint32_t high = search(s.count1, s.mass1, kLevel1, by_count, n, m, past, n0, m0);
+            list(high);
+            fill(10, high, high);
+            const uint32_t bin = (high << 10) | search(s.count2, s.mass2, kLevel2, by_count, n, m, past, n0, m0);
+            fill(0, bin, high);
+            const uint32_t low = search(s.count2, s.mass2, kLevel2, by_count, n, m, past, n0, m0);
+            const int bc = s.count2[low];
             Place p;
             p.bin = (bin << 10) | low;
             p.w = P.weight(value32(p.bin), top);
@@ -529,44 +600,41 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
                                  : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(bc)));
             return p;
         };
-        // the mass of all tokens, and how many min_p keeps
-        int kept = 0;
-        unsigned long long sum = 0;
-        each([&](uint32_t r) {
-            const double w = P.weight(value32(r), top);
-            if (w >= P.min_p) ++kept;
-            sum += static_cast<unsigned long long>(w * unit + 0.5);
-        });
-        kept = wave_sum(kept);
-        sum = wave_sum(sum);
-        if (lane == 0) {
-            atomicAdd(&s.kept, kept);
-            s.part_mass[wave] = sum;
-        }
-        __syncthreads();
-        uint64_t all = 0;
-        for (int w = 0; w < kWaves; ++w) all += s.part_mass[w];
-        int n = total;
-        double mass = static_cast<double>(all) * back;
-        if (P.top_k > 0 && P.top_k < n) {
-            n = P.top_k;
-            const Place p = find(true, n, 0.0, false);
-            mass = p.mass + p.in_bin * p.w;
-        }
-        int cut = n;
-        if (P.top_p < 1.0) {
-            const Place p = find(false, 0, P.top_p * mass, false);
-            cut = min(cut, max(p.count + p.in_bin, 1));
-        }
-        cut = max(min(cut, s.kept), 1);
-        if (cut < n) {
-            const Place p = find(true, cut, 0.0, false);
-            mass = p.mass + p.in_bin * p.w;
-        }
-        at = find(false, 0, P.u * mass, true);
-        if (at.count + at.in_bin >= cut) {
-            at = find(true, cut, 0.0, false);
-            at.in_bin -= 1;
+        int n = total, cut = total;
+        double mass = static_cast<double>(s.sum) * back;
+#pragma nounroll
+        for (int stage = 0; stage < 5; ++stage) {
+            bool by_count = true, past = false;
+            int number = 0;
+            double amount = 0.0;
+            if (stage == 0) {  // the first top_k and their mass
+                if (P.top_k <= 0 || P.top_k >= n) continue;
+                number = n = cut = P.top_k;
+            } else if (stage == 1) {  // of those, top_p of their mass
+                if (P.top_p >= 1.0) continue;
+                by_count = false;
+                amount = P.top_p * mass;
+            } else if (stage == 2) {  // of those, what min_p keeps; the mass of the kept
+                cut = max(min(cut, s.kept), 1);
+                if (cut == n) continue;
+                number = cut;
+            } else if (stage == 3) {  // the draw
+                by_count = false;
+                past = true;
+                amount = P.u * mass;
+            } else {  // rounding put it behind the last kept token
+                if (at.count + at.in_bin < cut) continue;
+                number = cut;
+            }
+            const Place p = find(by_count, number, amount, past);
+            if (stage == 1) {
+                cut = min(cut, max(p.count + p.in_bin, 1));
+            } else if (stage < 3) {
+                mass = p.mass + p.in_bin * p.w;
+            } else {
+                at = p;
+                at.in_bin -= stage == 4 ? 1 : 0;
+            }
         }
     }
     const int i = nth_index(rd, at.in_bin, none,
@@ -624,9 +692,13 @@ extern "C" int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, 
                                static_cast<int>(rows));
         hipLaunchKernelGGL(sample_f16, grid, block, sizeof(Lds16), s, a, over);
         // over 65535 tokens a 16-bit counter can overflow; such rows are left to this
-        if (over) hipLaunchKernelGGL(sample_any<uint16_t>, grid, block, 0, s, a, static_cast<const int*>(over), shift);
+        if (over) {
+            if (int rc = prepare_lds(reinterpret_cast<const void*>(&sample_any<uint16_t>), sizeof(Lds32))) return rc;
+            hipLaunchKernelGGL(sample_any<uint16_t>, grid, block, sizeof(Lds32), s, a, static_cast<const int*>(over), shift);
+        }
     } else {
-        hipLaunchKernelGGL(sample_any<uint32_t>, grid, block, 0, s, a, static_cast<const int*>(nullptr), shift);
+        if (int rc = prepare_lds(reinterpret_cast<const void*>(&sample_any<uint32_t>), sizeof(Lds32))) return rc;
+        hipLaunchKernelGGL(sample_any<uint32_t>, grid, block, sizeof(Lds32), s, a, static_cast<const int*>(nullptr), shift);
     }
     if (int rc = check_hip(hipGetLastError(), "sample_tokens launch")) return rc;
     return ok();
