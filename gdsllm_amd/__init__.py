@@ -93,8 +93,7 @@ SIGNATURES = {
     "gdsllm_kv_append": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
     "gdsllm_kv_attention_workspace_size": (ctypes.c_size_t, [_c_i64] * 6),
     "gdsllm_kv_attention": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_size_t, _c_vp]),
-    "gdsllm_sample_tokens_workspace_size": (ctypes.c_size_t, [_c_i64, _c_i64]),
-    "gdsllm_sample_tokens": (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_vp]),
+    "gdsllm_sample_tokens": (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64, _c_i64] + [_c_vp] * 7),
     "gdsllm_read_stream": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, ctypes.c_uint32, _c_vp, _c_vp]),
     "gdsllm_empty_launch": (ctypes.c_int, [_c_i64, _c_vp]),
 }

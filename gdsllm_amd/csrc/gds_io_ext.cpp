@@ -1085,13 +1085,10 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u, c10::optional
     if (min_p.has_value()) m = flat(*min_p, torch::kFloat32, dev, rows, "min_p", where);
     torch::Tensor out = torch::empty(logits.sizes().slice(0, logits.dim() - 1), l.options().dtype(torch::kInt64));
     const int bits = l.scalar_type() == torch::kFloat16 ? 16 : 32;
-    const size_t bytes = bits == 16 ? gdsllm_sample_tokens_workspace_size(rows, vocab) : 0;
-    torch::Tensor ws;
-    if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, l.options().dtype(torch::kUInt8));
     auto f = [](const torch::Tensor& x) { return x.defined() ? x.data_ptr<float>() : nullptr; };
     check(gdsllm_sample_tokens(l.data_ptr(), bits, rows, vocab, strided && rows > 1 ? l.stride(0) : vocab, f(uu), f(t),
                                k.defined() ? k.data_ptr<int32_t>() : nullptr, f(p), f(m), out.data_ptr<int64_t>(),
-                               bytes > 0 ? ws.data_ptr() : nullptr, bytes, OnDevice(dev).stream()),
+                               OnDevice(dev).stream()),
           where);
     return out;
 }

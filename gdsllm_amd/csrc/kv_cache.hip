@@ -205,186 +205,254 @@ struct AppendArgs {
 
 // The slot of a row that is written, -1 for padding: a slot outside the
 // cache, or a position that the rotation's table does not have.
-__device__ __forceinline__ int64_t slot_of(const AppendArgs& a, int t) {
+__device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
     const int s = a.slots[t];
     if (s < 0 || (s >> a.c.block_log2) >= a.c.num_blocks) return -1;
     if (a.half > 0 && static_cast<uint32_t>(a.positions[t]) >= static_cast<uint32_t>(a.max_pos)) return -1;
     return s;
 }
 
-// (x c - y s, y c + x s) of eight fp16 pairs.  In 64 bits: the products are
-// exact, so the one rounding that counts is the last, to fp16.
-__device__ __forceinline__ void rotate8(const uint4& x, const uint4& y, const float* c, const float* s, bool first,
-                                        uint16_t (&out)[8]) {
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+// Cosines and sines of eight channels, and their product with eight pairs: in 64
+// bits, where the products are exact, so the one rounding that counts is the
+// last, to fp16.
+struct Turn {
+    float4_t c[2], s[2];
+    __device__ __forceinline__ void load(const float* cos, const float* sin) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const double a = h2f((xs[i / 2] >> (16 * (i & 1))) & 0xFFFFu), b = h2f((ys[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
-        const double cc = c[i], ss = s[i];
-        out[i] = f2h_bits(fp32_rounded(static_cast<float>(first ? a * cc - b * ss : a * cc + b * ss)));
+        for (int i = 0; i < 2; ++i) {
+            c[i] = *reinterpret_cast<const float4_t*>(cos + 4 * i);
+            s[i] = *reinterpret_cast<const float4_t*>(sin + 4 * i);
+        }
     }
+    // own c - other s of the first half's channels, own c + other s of the second's
+    __device__ __forceinline__ uint4 apply(const uint4& own, const uint4& other, bool first) const {
+        const uint32_t xs[4] = {own.x, own.y, own.z, own.w}, ys[4] = {other.x, other.y, other.z, other.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint16_t h[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const double a = h2f((xs[i] >> (16 * j)) & 0xFFFFu), b = h2f((ys[i] >> (16 * j)) & 0xFFFFu);
+                const double bs = b * static_cast<double>(s[i / 2][2 * (i & 1) + j]);
+                h[j] = f2h_bits(fp32_rounded(static_cast<float>(fma(a, static_cast<double>(c[i / 2][2 * (i & 1) + j]), first ? -bs : bs))));
+            }
+            r[i] = h[0] | (static_cast<uint32_t>(h[1]) << 16);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+};
+
+__device__ __forceinline__ uint4 load16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// Eight channels (chunk `ch`) of a row of keys, after the rotation.
+__device__ __forceinline__ uint4 load_rotated(const AppendArgs& a, const uint16_t* row, int t, int ch) {
+    const uint4 own = load16(row + 8 * ch);
+    const int hc = a.half >> 3;
+    if (ch >= 2 * hc) return own;
+    const bool lo = ch < hc;
+    const uint4 other = load16(row + 8 * (lo ? ch + hc : ch - hc));
+    const int64_t at = static_cast<int64_t>(a.positions[t]) * a.half + 8 * (lo ? ch : ch - hc);
+    Turn turn;
+    turn.load(a.cos + at, a.sin + at);
+    return turn.apply(own, other, lo);
 }
 
-// Eight channels (chunk `ch`) of a row of k, after the rotation, as fp16 bits.
-__device__ __forceinline__ void load_rotated(const AppendArgs& a, const uint16_t* row, int t, int ch,
-                                             uint16_t (&out)[8]) {
-    const uint4 own = *reinterpret_cast<const uint4*>(row + 8 * ch);
-    const int hc = a.half >> 3;
-    if (ch < 2 * hc) {
-        const bool lo = ch < hc;
-        const uint4 other = *reinterpret_cast<const uint4*>(row + 8 * (lo ? ch + hc : ch - hc));
-        const int64_t at = static_cast<int64_t>(a.positions[t]) * a.half + 8 * (lo ? ch : ch - hc);
-        rotate8(own, other, a.cos + at, a.sin + at, lo, out);
-        return;
-    }
-    const uint32_t w[4] = {own.x, own.y, own.z, own.w};
+// New rows t0 .. t0 + n - 1 of one page and head; `low`: the lowest offset that
+// they write; `rising`: their offsets rise row by row (else a slot may occur twice).
+struct Run {
+    const AppendArgs* a;
+    const uint16_t* src;
+    uint8_t* codes;
+    float* scales;
+    int64_t ld;
+    int t0, n, page, low, head;
+    bool is_k, rising;
+};
+
+// A run by `WAVES` waves (tid: this thread's number
+// among theirs): the largest finite magnitude, the scale, the old codes where it
+// grew, the new codes.  The rotated rows stay in registers between the two
+// passes, up to kKeep chunks of eight channels to a thread.
+template <bool E4M3, int D, int WAVES>
+__device__ void append_run(const Run& r, int tid, float* red) {
+    constexpr int C = D / 8, N = 64 * WAVES, kKeep = 4;
+    const AppendArgs& a = *r.a;
+    const int bl = a.c.block_log2;
+    const float top = E4M3 ? kE4m3Max : kInt8Max;
+    const int chunks = r.n * C;
+    auto load = [&](int i) {
+        const int t = r.t0 + i / C;
+        const uint16_t* row = r.src + t * r.ld;
+        return r.is_k && a.half > 0 ? load_rotated(a, row, t, i % C) : load16(row + 8 * (i % C));
+    };
+    float amax = 0.f;
+    auto largest = [&](const uint4& x) {
+        const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h = (ws[j / 2] >> (16 * (j & 1))) & 0x7FFFu;
+            amax = fmaxf(amax, h < 0x7C00u ? h2f(h) : 0.f);
+        }
+    };
+    uint4 keep[kKeep];
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+        if (tid + N * j < chunks) {
+            keep[j] = load(tid + N * j);
+            largest(keep[j]);
+        }
+    for (int i = tid + N * kKeep; i < chunks; i += N) largest(load(i));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) amax = fmaxf(amax, red[w]);
+    }
+    // smallest power of two with amax <= top * scale
+    float want = 0x1p-32f;
+    if (amax > 0.f) {
+        int e;
+        const float m = frexpf(amax / top, &e);
+        want = fmaxf(want, ldexpf(1.f, m == 0.5f ? e - 1 : e));
+    }
+    const int64_t sc = static_cast<int64_t>(r.page) * a.c.kv_heads + r.head;
+    const float was = r.low > 0 ? r.scales[sc] : 0.f;
+    const float now = fmaxf(was, want);
+    if constexpr (WAVES > 1) __syncthreads();  // every wave has read the old scale
+    uint8_t* base = r.codes + ((sc << bl) * D);
+    if (tid == 0) r.scales[sc] = now;
+    if (r.low > 0 && was != now) {
+        const float ratio = was / now;
+        for (int i = tid; i < r.low * C; i += N) {
+            uint2* p = reinterpret_cast<uint2*>(base + 8 * static_cast<int64_t>(i));
+            const uint2 w = *p;
+            float x[4], y[4];
+            codes_to_f32<E4M3>(w.x, x);
+            codes_to_f32<E4M3>(w.y, y);
+            *p = make_uint2(to_codes<E4M3>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio),
+                            to_codes<E4M3>(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio));
+        }
+    }
+    const float inv = 1.f / now;
+    auto store = [&](int i, const uint4& x) {
+        const int t = r.t0 + i / C, s = a.slots[t];
+        if (!r.rising) {  // the last row of a slot that occurs twice is the one that stays
+            for (int u = t + 1; u < r.t0 + r.n; ++u)
+                if (a.slots[u] == s) return;
+        }
+        const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = h2f((ws[j / 2] >> (16 * (j & 1))) & 0xFFFFu) * inv;
+        *reinterpret_cast<uint2*>(base + (s & ((1 << bl) - 1)) * D + 8 * (i % C)) =
+            make_uint2(to_codes<E4M3>(y[0], y[1], y[2], y[3]), to_codes<E4M3>(y[4], y[5], y[6], y[7]));
+    };
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+        if (tid + N * j < chunks) store(tid + N * j, keep[j]);
+    for (int i = tid + N * kKeep; i < chunks; i += N) store(i, load(i));
 }
 
 // Workgroups [0, groups * kv_heads * 2): keys (even) or values (odd) of one
-// head in rows_per_group token rows.  A page's tokens stand in consecutive
-// rows; the workgroup takes every page whose first row lies in its rows, to
-// that page's last row wherever it is, so one workgroup alone writes a page.
-template <bool E4M3, int D>
+// head in `rows_per_group` (at most 62) token rows.  A page's tokens stand in
+// consecutive rows; the workgroup takes every page whose first row lies in its
+// rows, to that page's last row wherever it is, so one workgroup alone writes a
+// page.  Pages with few new rows go to one wave each, others to all four.
+template <bool E4M3, int D, int WAVES>
 __device__ void append_pages(const AppendArgs& a, int unit) {
-    constexpr int C = D / 8;
-    __shared__ float red[4];
-    const bool is_k = (unit & 1) == 0;
-    const int head = (unit >> 1) % a.c.kv_heads, g = (unit >> 1) / a.c.kv_heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nthreads = blockDim.x;
-    const int bl = a.c.block_log2;
-    const uint16_t* src = (is_k ? a.k : a.v) + head * D;
-    const int64_t ld = is_k ? a.ldk : a.ldv;
-    uint8_t* codes = is_k ? a.c.k : a.c.v;
-    float* scales = is_k ? a.c.k_scale : a.c.v_scale;
-    const float top = E4M3 ? kE4m3Max : kInt8Max;
-
-    const int t_end = min((g + 1) * a.rows_per_group, a.tokens);
-    for (int t0 = g * a.rows_per_group; t0 < t_end; ++t0) {
-        const int64_t s0 = slot_of(a, t0);
-        if (s0 < 0) continue;
-        const int page = static_cast<int>(s0 >> bl);
-        if (t0 > 0) {
-            const int64_t prev = slot_of(a, t0 - 1);
-            if (prev >= 0 && (prev >> bl) == page) continue;
-        }
-        // rows of the page, the lowest offset among them, and whether the
-        // offsets rise row by row (else a slot may occur twice)
-        int n = 1, low = static_cast<int>(s0) & ((1 << bl) - 1);
-        bool rising = true;
-        for (;;) {
-            const int t = t0 + n + lane;
-            const int64_t s = t < a.tokens ? slot_of(a, t) : -1;
-            const bool in = s >= 0 && (s >> bl) == page;
-            const uint64_t out = ~__ballot(in);
-            const int more = out ? __builtin_ctzll(out) : 64;
-            if (lane < more) low = min(low, static_cast<int>(s) & ((1 << bl) - 1));
-            if (__ballot(lane < more && s <= slot_of(a, t - 1))) rising = false;
-            n += more;
-            if (more < 64) break;
+    __shared__ float red[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), bl = a.c.block_log2;
+    Run r;
+    r.a = &a;
+    r.is_k = (unit & 1) == 0;
+    r.head = (unit >> 1) % a.c.kv_heads;
+    r.src = (r.is_k ? a.k : a.v) + r.head * D;
+    r.ld = r.is_k ? a.ldk : a.ldv;
+    r.codes = r.is_k ? a.c.k : a.c.v;
+    r.scales = r.is_k ? a.c.k_scale : a.c.v_scale;
+    const int base = (unit >> 1) / a.c.kv_heads * a.rows_per_group - 1;  // lane 0's row: the one before the group
+    const int t = base + lane, mask = (1 << bl) - 1;
+    const int s = t >= 0 && t < a.tokens ? slot_of(a, t) : -1, before = __shfl_up(s, 1);
+    const bool goes_on = lane > 0 && s >= 0 && before >= 0 && (s >> bl) == (before >> bl);
+    const uint64_t same = __ballot(goes_on), falls = __ballot(goes_on && s <= before);
+    uint64_t heads = __ballot(lane > 0 && lane <= a.rows_per_group && s >= 0 && !goes_on);
+    for (int k = 0; heads; ++k, heads &= heads - 1) {
+        const int l = __builtin_ctzll(heads);
+        const uint64_t rest = l < 63 ? ~(same >> (l + 1)) : 1ull;
+        const int more = min(__builtin_ctzll(rest), 63 - l);
+        const uint64_t run = (more == 63 ? ~0ull : ((1ull << (more + 1)) - 1)) << l;
+        r.t0 = base + l;
+        r.n = more + 1;
+        r.page = __builtin_amdgcn_readlane(s, l) >> bl;
+        int low = run >> lane & 1 ? s & mask : mask;
+        r.rising = !(falls & run);
+        if (l + more == 63) {  // past the rows that the wave holds
+            for (;;) {
+                const int u = r.t0 + r.n + lane, v = u < a.tokens ? slot_of(a, u) : -1, w = u <= a.tokens ? slot_of(a, u - 1) : -1;
+                const uint64_t out = ~__ballot(v >= 0 && (v >> bl) == r.page);
+                const int got = out ? __builtin_ctzll(out) : 64;
+                if (lane < got) low = min(low, v & mask);
+                if (__ballot(lane < got && v <= w)) r.rising = false;
+                r.n += got;
+                if (got < 64) break;
+            }
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o));
+        r.low = __builtin_amdgcn_readfirstlane(low);
+        if (WAVES == 1 || r.n * (D / 8) > 4 * 64) append_run<E4M3, D, WAVES>(r, tid, red);
+        else if (k % WAVES == wave) append_run<E4M3, D, 1>(r, lane, red);
+    }
+}
 
-        auto load = [&](int i, uint16_t (&x)[8]) {
-            const int t = t0 + i / C;
-            const uint16_t* row = src + t * ld;
-            if (is_k && a.half > 0) {
-                load_rotated(a, row, t, i % C, x);
-            } else {
-                const uint4 w = *reinterpret_cast<const uint4*>(row + 8 * (i % C));
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = static_cast<uint16_t>(ws[j / 2] >> (16 * (j & 1)));
+// The rotation of q, a token to a workgroup at a time; a thread keeps to one
+// chunk of the heads' channels.
+template <int D>
+__device__ void rotate_q(const AppendArgs& a, int first, int step) {
+    constexpr int C = D / 8;
+    const int tid = threadIdx.x, ch = tid % C, hc = a.half >> 3, per = blockDim.x / C;
+    const bool turns = ch < 2 * hc, lo = ch < hc;
+    for (int t = first; t < a.tokens; t += step) {
+        const bool live = slot_of(a, t) >= 0;
+        Turn turn;
+        if (turns && live) {
+            const int64_t at = static_cast<int64_t>(a.positions[t]) * a.half + 8 * (lo ? ch : ch - hc);
+            turn.load(a.cos + at, a.sin + at);
+        }
+        const uint16_t* row = a.q + t * a.ldq + 8 * ch;
+        uint16_t* out = a.q_out + static_cast<int64_t>(t) * a.q_heads * D + 8 * ch;
+#pragma unroll 2
+        for (int h = tid / C; h < a.q_heads; h += per) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (live) {
+                x = load16(row + h * D);
+                if (turns) x = turn.apply(x, load16(row + h * D + 8 * (lo ? hc : -hc)), lo);
             }
-        };
-        float amax = 0.f;
-        for (int i = tid; i < n * C; i += nthreads) {
-            uint16_t x[8];
-            load(i, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if ((x[j] & 0x7C00u) != 0x7C00u) amax = fmaxf(amax, h2f(x[j] & 0x7FFFu));
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-        if (nthreads > 64) {
-            __syncthreads();
-            if (lane == 0) red[wave] = amax;
-            __syncthreads();
-            amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        }
-        // smallest power of two with amax <= top * scale
-        float want = 0x1p-32f;
-        if (amax > 0.f) {
-            int e;
-            const float m = frexpf(amax / top, &e);
-            want = fmaxf(want, ldexpf(1.f, m == 0.5f ? e - 1 : e));
-        }
-        const int64_t sc = static_cast<int64_t>(page) * a.c.kv_heads + head;
-        const float was = low > 0 ? scales[sc] : 0.f;
-        const float now = fmaxf(was, want);
-        if (nthreads > 64) __syncthreads();  // every wave has read the old scale
-        uint8_t* base = codes + ((sc << bl) * D);
-        if (tid == 0) scales[sc] = now;
-        if (low > 0 && was != now) {
-            const float ratio = was / now;
-            for (int i = tid; i < low * C; i += nthreads) {
-                uint2* p = reinterpret_cast<uint2*>(base + 8 * static_cast<int64_t>(i));
-                const uint2 w = *p;
-                float x[4], y[4];
-                codes_to_f32<E4M3>(w.x, x);
-                codes_to_f32<E4M3>(w.y, y);
-                *p = make_uint2(to_codes<E4M3>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio),
-                                to_codes<E4M3>(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio));
-            }
-        }
-        const float inv = 1.f / now;
-        for (int i = tid; i < n * C; i += nthreads) {
-            const int t = t0 + i / C;
-            const int64_t s = slot_of(a, t);
-            if (!rising) {  // the last row of a slot that occurs twice is the one that stays
-                bool later = false;
-                for (int u = t + 1; u < t0 + n; ++u) later |= slot_of(a, u) == s;
-                if (later) continue;
-            }
-            uint16_t x[8];
-            load(i, x);
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = h2f(x[j]) * inv;
-            const int64_t at = (s & ((1 << bl) - 1)) * D + 8 * (i % C);
-            *reinterpret_cast<uint2*>(base + at) =
-                make_uint2(to_codes<E4M3>(y[0], y[1], y[2], y[3]), to_codes<E4M3>(y[4], y[5], y[6], y[7]));
+            *reinterpret_cast<uint4*>(out + h * D) = x;
         }
     }
 }
 
-template <bool E4M3, int D>
-__global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
-    const int units = a.groups * a.c.kv_heads * 2;
-    if (static_cast<int>(blockIdx.x) < units) {
-        append_pages<E4M3, D>(a, blockIdx.x);
+template <int D>
+__global__ __launch_bounds__(256) void kv_rotate(AppendArgs a) {
+    rotate_q<D>(a, blockIdx.x, gridDim.x);
+}
+
+template <bool E4M3, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 3 : 4) void kv_append(AppendArgs a) {
+    // workgroups go to the eight XCDs in turn: each XCD takes a run of units, so
+    // that those in which a page begins (every fourth, say) fall to all of them
+    const int per = (a.groups * a.c.kv_heads * 2 + 7) / 8, b = blockIdx.x;
+    if (b >= 8 * per) {
+        rotate_q<D>(a, b - 8 * per, gridDim.x - 8 * per);
         return;
     }
-    // the rotation of q: one chunk of eight channels a thread
-    constexpr int C = D / 8;
-    const int64_t chunks = static_cast<int64_t>(a.tokens) * a.q_heads * C;
-    const int64_t step = static_cast<int64_t>(gridDim.x - units) * blockDim.x;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x - units) * blockDim.x + threadIdx.x; i < chunks; i += step) {
-        const int64_t th = i / C;
-        const int t = static_cast<int>(th / a.q_heads);
-        uint16_t x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (slot_of(a, t) >= 0)
-            load_rotated(a, a.q + t * a.ldq + (th % a.q_heads) * D, t, static_cast<int>(i % C), x);
-        uint4 w;
-        w.x = x[0] | (uint32_t(x[1]) << 16);
-        w.y = x[2] | (uint32_t(x[3]) << 16);
-        w.z = x[4] | (uint32_t(x[5]) << 16);
-        w.w = x[6] | (uint32_t(x[7]) << 16);
-        *reinterpret_cast<uint4*>(a.q_out + i * 8) = w;
-    }
+    const int unit = b % 8 * per + b / 8;
+    if (unit < a.groups * a.c.kv_heads * 2) append_pages<E4M3, D, WAVES>(a, unit);
 }
 
 }  // namespace
@@ -458,9 +526,9 @@ extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, in
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q) |
          reinterpret_cast<uintptr_t>(q_out)) % 16)
         return bad("k, v, q and q_out must be 16-byte aligned");
-    if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions) |
-         reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 4)
-        return bad("misaligned pointer");
+    if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) % 4 ||
+        (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
+        return bad("misaligned pointer (cos and sin: 16 bytes)");
     a.k = static_cast<const uint16_t*>(k);
     a.v = static_cast<const uint16_t*>(v);
     a.q = static_cast<const uint16_t*>(q);
@@ -476,27 +544,37 @@ extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, in
     a.q_heads = static_cast<int>(q_heads);
     a.half = static_cast<int>(rotary / 2);
     a.max_pos = static_cast<int>(max_pos);
-    a.rows_per_group = tokens > 512 ? 16 : 1;
+    // as many waves as hold a page of one head in registers; most of a prompt's
+    // rows begin no page, a decoding batch's all do
+    const int64_t chunks = cache->block_size * D / 8;
+    const int waves = chunks <= 256 ? 1 : chunks <= 1024 ? 4 : 16;
+    const int64_t share = tokens * cache->kv_heads * 2 / 512;  // rows that leave two workgroups to a compute unit
+    a.rows_per_group = static_cast<int>(std::min<int64_t>(std::max<int64_t>(share, 1), std::min<int64_t>(cache->block_size, 62)));
     a.groups = static_cast<int>((tokens + a.rows_per_group - 1) / a.rows_per_group);
-    const int64_t units = static_cast<int64_t>(a.groups) * cache->kv_heads * 2;
-    const int threads = tokens > 512 ? 256 : 64;
-    int64_t q_groups = 0;
-    if (q) {
-        const int64_t chunks = tokens * q_heads * (D / 8);
-        q_groups = std::min<int64_t>((chunks + threads - 1) / threads, 16 * static_cast<int64_t>(cu_count()));
-    }
+    const int64_t units = (static_cast<int64_t>(a.groups) * cache->kv_heads * 2 + 7) / 8 * 8;
+    // q rides along, but not in workgroups of 1024 threads, which turn a token at a
+    // time too slowly (8192 tokens of 32 heads of 256: 93 us against 54)
+    const int64_t q_tokens = q ? std::min<int64_t>(tokens, 16 * static_cast<int64_t>(cu_count())) : 0;
+    const bool apart = q_tokens > 256 && waves == 16;
+    const int64_t q_groups = apart ? 0 : q_tokens;
     if (units + q_groups > (int64_t(1) << 31) - 1) return bad("too many tokens and heads for one call");
-    const dim3 grid(static_cast<unsigned>(units + q_groups)), block(threads);
+    const dim3 grid(static_cast<unsigned>(units + q_groups));
     const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
     const hipStream_t s = as_stream(stream);
-#define GDSLLM_APPEND(DIM)                                                                   \
-    if (D == DIM) {                                                                          \
-        if (e4m3) hipLaunchKernelGGL((kv_append<true, DIM>), grid, block, 0, s, a);          \
-        else hipLaunchKernelGGL((kv_append<false, DIM>), grid, block, 0, s, a);              \
+#define GDSLLM_APPEND(DIM, W)                                                                    \
+    if (D == DIM && waves == W) {                                                                \
+        if (e4m3) hipLaunchKernelGGL((kv_append<true, DIM, W>), grid, dim3(64 * W), 0, s, a);    \
+        else hipLaunchKernelGGL((kv_append<false, DIM, W>), grid, dim3(64 * W), 0, s, a);        \
+        if (apart) hipLaunchKernelGGL(kv_rotate<DIM>, dim3(static_cast<unsigned>(q_tokens)), dim3(256), 0, s, a); \
     }
-    GDSLLM_APPEND(64)
-    GDSLLM_APPEND(128)
-    GDSLLM_APPEND(256)
+    GDSLLM_APPEND(64, 1)
+    GDSLLM_APPEND(64, 4)
+    GDSLLM_APPEND(64, 16)
+    GDSLLM_APPEND(128, 1)
+    GDSLLM_APPEND(128, 4)
+    GDSLLM_APPEND(128, 16)
+    GDSLLM_APPEND(256, 4)
+    GDSLLM_APPEND(256, 16)
 #undef GDSLLM_APPEND
     if (int rc = check_hip(hipGetLastError(), "kv_append launch")) return rc;
     return ok();

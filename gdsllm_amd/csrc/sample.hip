@@ -33,6 +33,7 @@ struct SampleArgs {
     int64_t* tokens;
     int64_t ld;
     int vocab;
+    int shift;  // masses in whole units of 2^-shift: the sum of vocab of them fits 63 bits
 };
 
 // 2^y for y <= 0 in 64 bits: the nearest whole number goes to the exponent, the
@@ -224,349 +225,6 @@ struct Place {
     double mass, w;      // mass before the bin; weight of the bin's tokens
 };
 
-// ---------------------------------------------------------------- fp16 logits
-
-// The counters: the values of magnitude h lie in word h, positive ones in its
-// low half, negative ones in its high half.  A unit is one binade of one sign,
-// 1024 words; in falling order of their values: unit 0 is +inf, 1 .. 31 the
-// positive binades, 32 .. 62 the negative ones.
-constexpr int kUnits = 63;
-constexpr int kMagnitudes = 32768;
-constexpr int kListed16 = 2048;  // indices that are sorted by counting
-
-struct Lds16 {
-    uint32_t hist[kMagnitudes];
-    double mass[64], wave_mass[kWaves];
-    Place place;
-    int count[64], wave_count[kWaves];
-    int top, outside, answer, listed, hit, last;
-};
-
-// Element k (in falling order) of unit u, as fp16 bits.
-__device__ __forceinline__ uint32_t unit_bits(int u, int k) {
-    const uint32_t base = u == 0 ? 0x7C00u : u < 32 ? static_cast<uint32_t>(31 - u) << 10 : 0x8000u | static_cast<uint32_t>(u - 32) << 10;
-    return base | ((u < 32 ? (u == 0 ? 0 : 1023) : 0) ^ (u == 0 ? 0 : k));
-}
-
-// One row of fp16 logits by one workgroup.  R > 0: a thread keeps its R granules
-// of the row in registers from the count to the search for the token's index; 0:
-// they are read twice.
-template <int R>
-__global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a, int* overflow_rows) {
-    extern __shared__ __attribute__((aligned(16))) char raw[];
-    Lds16& s = *reinterpret_cast<Lds16*>(raw);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-    const RowReader<uint16_t, 8> rd(static_cast<const uint16_t*>(a.logits) + row * a.ld, a.vocab);
-    const RowParams P(a, row);
-    constexpr uint32_t none = 0xFFFFu;  // a NaN
-    const int grans = rd.granules();
-
-    uint4 keep[R > 0 ? R : 1];
-#pragma unroll
-    for (int i = 0; i < R; ++i) keep[i] = rd.load_packed(tid + i * kThreads, none);
-    for (int i = tid; i < kMagnitudes / 4; i += kThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) {
-        s.top = 0;
-        s.outside = 0;
-        s.listed = 0;
-        s.answer = -1;
-    }
-    __syncthreads();
-
-    // -0 becomes +0 by adding +0: equal logits stand together
-    auto plain = [](uint32_t two) {
-        const half2_t zero = {static_cast<half_t>(0.f), static_cast<half_t>(0.f)};
-        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, two) + zero);
-    };
-    half2_t most = {static_cast<half_t>(-INFINITY), static_cast<half_t>(-INFINITY)};
-    auto count = [&](const uint4& w) {
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t x = plain(ws[j]);
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(half2_t, x));
-            if (!P.greedy) {
-                atomicAdd(&s.hist[x & 0x7FFFu], (x & 0x8000u) ? 0x10000u : 1u);
-                atomicAdd(&s.hist[(x >> 16) & 0x7FFFu], (x >> 31) ? 0x10000u : 1u);
-            }
-        }
-    };
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (tid + i * kThreads < grans) count(keep[i]);
-    } else {
-        for (int g0 = tid; g0 < grans; g0 += 4 * kThreads) {
-            uint4 w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = rd.load_packed(g0 + i * kThreads, none);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (g0 + i * kThreads < grans) count(w[i]);
-        }
-    }
-    {
-        // the largest logit, as an order-keeping whole number (1024: -inf, so no token)
-        const uint32_t x = __builtin_bit_cast(uint32_t, most);
-        auto key = [](uint32_t h) { return static_cast<int>((h & 0x8000u) ? 0xFFFFu - h : 0x8000u | h); };
-        int k = max(key(x & 0xFFFFu), key(x >> 16));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) k = max(k, __shfl_xor(k, o));
-        if (lane == 0) atomicMax(&s.top, k);
-    }
-    __syncthreads();
-    const int key = s.top;
-    if (key <= 0xFFFF - 0xFC00) {
-        if (tid == 0) a.tokens[row] = -1;
-        return;
-    }
-    const uint32_t top_bits = key & 0x8000 ? key & 0x7FFFu : 0xFFFFu - key;
-    const float top = h2f(top_bits);
-    uint32_t bin = top_bits;
-    int which = 0;
-    if (!P.greedy) {
-        auto counter = [&](uint32_t h) { return static_cast<int>((s.hist[h & 0x7FFFu] >> ((h >> 11) & 16)) & 0xFFFFu); };
-        auto weight = [&](uint32_t h) { return h == top_bits ? 1.0 : P.weight(h2f(h), top); };
-        auto step_of = [](uint32_t h) {  // between neighbouring values of h's binade
-            const uint32_t low = max(h & 0x7C00u, 0x400u);
-            return static_cast<double>(h2f(low + 1) - h2f(low));
-        };
-        // Counts and masses of the units, a wave to the two units of an exponent.  The
-        // 1024 values of a binade are evenly spaced, so a weight is the one at the
-        // start of its 64 values (lanes 0-15: of the positive ones, 16-31: of the
-        // negative ones) times one of 64 that all of these share.
-        for (int e = wave; e < 32; e += kWaves) {
-            const uint32_t first = static_cast<uint32_t>(e) << 10;  // smallest magnitude
-            int n_pos = 0, n_neg = 0;
-            double w_pos = 0.0, w_neg = 0.0;
-            uint32_t c[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) c[j] = s.hist[first + 64 * j + lane];
-            if (e == 31) {  // infinities and NaN: +inf alone of them is a token
-                if (lane == 0) {
-                    n_pos = c[0] & 0xFFFFu;
-                    w_pos = n_pos;
-                    c[0] &= 0xFFFF0000u;
-                }
-                int outside = 0;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) outside += (c[j] & 0xFFFFu) + (c[j] >> 16);
-                outside = wave_sum(outside);
-                if (lane == 0 && outside) atomicAdd(&s.outside, outside);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    n_pos += c[j] & 0xFFFFu;
-                    n_neg += c[j] >> 16;
-                }
-                if (__any(n_pos + n_neg > 0)) {
-                    const double up = exp2_neg(-step_of(first) * P.c * (63 - lane)), down = lane_mirror(up);
-                    // largest of the 64 values
-                    const float base = lane < 16 ? h2f(first + 64 * lane + 63) : h2f(0x8000u | (first + 64 * (lane & 15)));
-                    const double start = top == INFINITY ? 0.0 : exp2_neg(fmin((static_cast<double>(base) - top) * P.c, 0.0));
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        // the largest logit's own 64 values, some of them above it, come below
-                        const uint32_t own = first + 64 * j;
-                        const uint32_t cp = own >> 6 == top_bits >> 6 ? 0 : c[j] & 0xFFFFu;
-                        const uint32_t cn = (0x8000u | own) >> 6 == top_bits >> 6 ? 0 : c[j] >> 16;
-                        w_pos = fma(lane_double(start, j), static_cast<double>(cp), w_pos);
-                        w_neg = fma(lane_double(start, 16 + j), static_cast<double>(cn), w_neg);
-                    }
-                    w_pos *= up;
-                    w_neg *= down;
-                    if (first >> 10 == (top_bits & 0x7FFFu) >> 10) {
-                        const uint32_t h = (top_bits & ~63u) + lane;
-                        const int own = counter(h);
-                        const double w = own ? weight(h) * own : 0.0;
-                        w_pos += (h & 0x8000u) ? 0.0 : w;
-                        w_neg += (h & 0x8000u) ? w : 0.0;
-                    }
-                }
-            }
-            n_pos = wave_sum(n_pos);
-            n_neg = wave_sum(n_neg);
-            w_pos = wave_scan(w_pos);
-            w_neg = wave_scan(w_neg);
-            if (lane == 63) {
-                s.count[31 - e] = n_pos;
-                s.mass[31 - e] = w_pos;
-                s.count[32 + e] = n_neg;  // [63]: always 0
-                s.mass[32 + e] = w_neg;
-            }
-        }
-        __syncthreads();
-        // inclusive sums over the units, a unit to a lane, in every wave
-        const int unit_n = s.count[lane];
-        const double unit_w = s.mass[lane];
-        const int upto_n = wave_scan(unit_n);
-        const double upto_w = wave_scan(unit_w);
-        const int total = last_lane(upto_n);
-        if (total + s.outside != grans * 8) {
-            // a counter overflowed (over 65535 equal logits): the row goes to the other kernel
-            if (tid == 0) overflow_rows[row] = 1;
-            return;
-        }
-        // The place where the order has had `n` tokens (Count), the first token at
-        // which the mass reaches (Reach) or passes (Pass) `m`, or the last token
-        // whose weight is at least `m` (Weight).  The unit by its sums, then a value
-        // of it to each thread.
-        enum Kind { Count, Reach, Pass, Weight };
-        auto find = [&](Kind kind, int n, double m) {
-            auto at_border = [&](int upto, double mass) {
-                return kind == Count ? upto >= n : kind == Pass ? mass > m : mass >= m;
-            };
-            const uint64_t some = __ballot(unit_n > 0);
-            int u;
-            if (kind == Weight) {
-                // the last unit whose largest value is heavy enough
-                const uint64_t heavy = __ballot(unit_n > 0 && weight(unit_bits(lane, 0)) >= m);
-                u = heavy ? 63 - __builtin_clzll(heavy) : __builtin_ctzll(some);
-            } else {
-                const uint64_t hit = __ballot(unit_n > 0 && at_border(upto_n, upto_w));
-                u = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-            }
-            const uint32_t h = unit_bits(u, tid);
-            const int c = u == 0 && tid > 0 ? 0 : counter(h);
-            double w = 0.0;
-            if (__any(c > 0)) w = c ? weight(h) : 0.0;
-            int cu = wave_scan(c);
-            double wu = wave_scan(w * c);
-            __syncthreads();  // the last place has been read
-            if (lane == 63) {
-                s.wave_count[wave] = cu;
-                s.wave_mass[wave] = wu;
-            }
-            if (tid == 0) {
-                s.hit = kind == Weight ? -1 : kThreads;
-                s.last = -1;
-            }
-            __syncthreads();
-            cu += __builtin_amdgcn_readlane(upto_n - unit_n, u);
-            wu += lane_double(upto_w - unit_w, u);
-#pragma unroll
-            for (int v = 0; v < kWaves - 1; ++v) {
-                cu += v < wave ? s.wave_count[v] : 0;
-                wu += v < wave ? s.wave_mass[v] : 0.0;
-            }
-            // lanes of a wave stand in order: one atomic a wave
-            const uint64_t has = __ballot(c > 0);
-            const uint64_t good = __ballot(c > 0 && (kind == Weight ? w >= m : at_border(cu, wu)));
-            if (lane == 0) {
-                if (has) atomicMax(&s.last, 64 * wave + 63 - __builtin_clzll(has));
-                if (good && kind == Weight) atomicMax(&s.hit, 64 * wave + 63 - __builtin_clzll(good));
-                if (good && kind != Weight) atomicMin(&s.hit, 64 * wave + __builtin_ctzll(good));
-            }
-            __syncthreads();
-            const int hit = s.hit;
-            const bool none_hits = hit < 0 || hit == kThreads;
-            if (kind == Weight && none_hits) {  // the place before this unit
-                if (tid == 0) s.place = {0, 0, __builtin_amdgcn_readlane(upto_n - unit_n, u), 0.0, 0.0};
-            } else if (tid == (none_hits ? s.last : hit)) {
-                Place p{h, 0, cu - c, wu - w * c, w};
-                if (kind == Count) p.in_bin = n - p.count;
-                else if (kind == Weight) p.in_bin = c;
-                else if (c == 1 || none_hits) p.in_bin = kind == Pass ? c - 1 : c;  // none: rounding hid it, the last token
-                else {
-                    const double q = (m - p.mass) / p.w;
-                    p.in_bin = kind == Pass ? static_cast<int>(fmin(fmax(floor(q), 0.0), c - 1.0))
-                                            : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(c)));
-                }
-                s.place = p;
-            }
-            __syncthreads();
-            return s.place;
-        };
-        Place at{top_bits, 0, 0, 0.0, 1.0};
-        int n = total, cut = total;
-        double mass = lane_double(upto_w, 63);
-#pragma nounroll
-        for (int stage = 0; stage < 6; ++stage) {
-            Kind kind = Count;
-            int number = 0;
-            double amount = 0.0;
-            if (stage == 0) {  // the first top_k and their mass
-                if (P.top_k <= 0 || P.top_k >= n) continue;
-                number = n = cut = P.top_k;
-            } else if (stage == 1) {  // of those, top_p of their mass
-                if (P.top_p >= 1.0) continue;
-                kind = Reach;
-                amount = P.top_p * mass;
-            } else if (stage == 2) {  // of those, what min_p keeps
-                if (P.min_p <= 0.0) continue;
-                kind = Weight;
-                amount = P.min_p;
-            } else if (stage == 3) {  // the mass of the kept
-                if (cut == n) continue;
-                number = cut;
-            } else if (stage == 4) {  // the draw
-                kind = Pass;
-                amount = P.u * mass;
-            } else {  // rounding put it behind the last kept token
-                if (at.count + at.in_bin < cut) continue;
-                number = cut;
-            }
-            const Place p = find(kind, number, amount);
-            if (stage == 1 || stage == 2) {
-                cut = min(cut, max(p.count + p.in_bin, 1));
-            } else if (stage < 4) {
-                mass = p.mass + p.in_bin * p.w;
-            } else {
-                at = p;
-                at.in_bin -= stage == 5 ? 1 : 0;
-            }
-        }
-        bin = at.bin;
-        which = at.in_bin;
-        __syncthreads();  // the counters have been read: the list takes their place
-    }
-
-    // the index of token number `which` of `bin`: its tokens' indices in any order
-    // into LDS (over the counters), the one that has `which` before it
-    int* list = reinterpret_cast<int*>(s.hist);
-    const uint32_t pair = bin | (bin << 16);
-    auto look = [&](int gr, const uint4& w) {
-        const uint32_t ws[4] = {plain(w.x) ^ pair, plain(w.y) ^ pair, plain(w.z) ^ pair, plain(w.w) ^ pair};
-        uint32_t zero = 0;  // a half that is zero borrows from its top bit
-#pragma unroll
-        for (int j = 0; j < 4; ++j) zero |= (ws[j] - 0x00010001u) & ~ws[j];
-        if (!(zero & 0x80008000u)) return;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (((ws[j / 2] >> (16 * (j & 1))) & 0xFFFFu) == 0) {
-                const int n = atomicAdd(&s.listed, 1);
-                if (n < kListed16) list[n] = rd.index(gr) + j;
-            }
-    };
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (tid + i * kThreads < grans) look(tid + i * kThreads, keep[i]);
-    } else {
-        for (int g0 = tid; g0 < grans; g0 += 4 * kThreads) {
-            uint4 w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = rd.load_packed(g0 + i * kThreads, none);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (g0 + i * kThreads < grans) look(g0 + i * kThreads, w[i]);
-        }
-    }
-    __syncthreads();
-    const int n = s.listed;
-    if (n > kListed16) {
-        const int i = nth_index(rd, which, none, [&](uint32_t x) { return (x == 0x8000u ? 0u : x) == bin; }, s.wave_count, &s.answer);
-        if (tid == 0) a.tokens[row] = i;
-        return;
-    }
-    for (int i = tid; i < n; i += kThreads) {
-        const int mine = list[i];
-        int before = 0;
-        for (int k = 0; k < n; ++k) before += list[k] < mine ? 1 : 0;
-        if (before == which) a.tokens[row] = mine;
-    }
-}
-
 // ---------------------------------------------------------------- 32-bit keys
 
 constexpr int kLevel1 = 4096;  // rank >> 20
@@ -587,11 +245,8 @@ struct Lds32 {
 // the upper 12 bits of their rank once; a place is then looked for in its bin
 // alone, whose ranks are listed in LDS where they fit.
 template <class E>
-__global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* only_rows, int shift) {
-    extern __shared__ __attribute__((aligned(16))) char raw[];
-    Lds32& s = *reinterpret_cast<Lds32*>(raw);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-    if (only_rows && only_rows[row] == 0) return;
+__device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), shift = a.shift;
     const RowReader<E, 4> rd(static_cast<const E*>(a.logits) + row * a.ld, a.vocab);
     const RowParams P(a, row);
     constexpr uint32_t none = sizeof(E) == 2 ? 0xFFFFu : 0xFFFFFFFFu;  // a NaN
@@ -808,9 +463,353 @@ __global__ __launch_bounds__(kThreads) void sample_any(SampleArgs a, const int* 
     if (tid == 0) a.tokens[row] = i;
 }
 
-__global__ void clear_rows(int* rows, int n) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) rows[i] = 0;
+__global__ __launch_bounds__(kThreads) void sample_f32(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    sample_ranks<uint32_t>(a, blockIdx.x, *reinterpret_cast<Lds32*>(raw));
+}
+
+// ---------------------------------------------------------------- fp16 logits
+
+// The counters: the values of magnitude h lie in word h, positive ones in its
+// low half, negative ones in its high half.  A unit is one binade of one sign,
+// 1024 words; in falling order of their values: unit 0 is +inf, 1 .. 31 the
+// positive binades, 32 .. 62 the negative ones.
+constexpr int kUnits = 63;
+constexpr int kMagnitudes = 32768;
+constexpr int kListed16 = 2048;  // indices that are sorted by counting
+
+struct Lds16 {
+    uint32_t hist[kMagnitudes];
+    double mass[64], wave_mass[kWaves];
+    Place place;
+    int count[64], wave_count[kWaves];
+    int top, outside, answer, listed, hit, last;
+};
+
+// Element k (in falling order) of unit u, as fp16 bits.
+__device__ __forceinline__ uint32_t unit_bits(int u, int k) {
+    const uint32_t base = u == 0 ? 0x7C00u : u < 32 ? static_cast<uint32_t>(31 - u) << 10 : 0x8000u | static_cast<uint32_t>(u - 32) << 10;
+    return base | ((u < 32 ? (u == 0 ? 0 : 1023) : 0) ^ (u == 0 ? 0 : k));
+}
+
+// One row of fp16 logits by one workgroup.  R > 0: a thread keeps its R granules
+// of the row in registers from the count to the search for the token's index; 0:
+// they are read twice.
+template <int R>
+__global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    Lds16& s = *reinterpret_cast<Lds16*>(raw);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
+    const RowReader<uint16_t, 8> rd(static_cast<const uint16_t*>(a.logits) + row * a.ld, a.vocab);
+    const RowParams P(a, row);
+    constexpr uint32_t none = 0xFFFFu;  // a NaN
+    const int grans = rd.granules();
+
+    uint4 keep[R > 0 ? R : 1];
+#pragma unroll
+    for (int i = 0; i < R; ++i) keep[i] = rd.load_packed(tid + i * kThreads, none);
+    for (int i = tid; i < kMagnitudes / 4; i += kThreads) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) {
+        s.top = 0;
+        s.outside = 0;
+        s.listed = 0;
+        s.answer = -1;
+    }
+    __syncthreads();
+
+    // -0 becomes +0 by adding +0: equal logits stand together
+    auto plain = [](uint32_t two) {
+        const half2_t zero = {static_cast<half_t>(0.f), static_cast<half_t>(0.f)};
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, two) + zero);
+    };
+    half2_t most = {static_cast<half_t>(-INFINITY), static_cast<half_t>(-INFINITY)};
+    auto count = [&](const uint4& w) {
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t x = plain(ws[j]);
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(half2_t, x));
+            if (!P.greedy) {
+                atomicAdd(&s.hist[x & 0x7FFFu], (x & 0x8000u) ? 0x10000u : 1u);
+                atomicAdd(&s.hist[(x >> 16) & 0x7FFFu], (x >> 31) ? 0x10000u : 1u);
+            }
+        }
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (tid + i * kThreads < grans) count(keep[i]);
+    } else {
+        for (int g0 = tid; g0 < grans; g0 += 4 * kThreads) {
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = rd.load_packed(g0 + i * kThreads, none);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (g0 + i * kThreads < grans) count(w[i]);
+        }
+    }
+    {
+        // the largest logit, as an order-keeping whole number (1024: -inf, so no token)
+        const uint32_t x = __builtin_bit_cast(uint32_t, most);
+        auto key = [](uint32_t h) { return static_cast<int>((h & 0x8000u) ? 0xFFFFu - h : 0x8000u | h); };
+        int k = max(key(x & 0xFFFFu), key(x >> 16));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) k = max(k, __shfl_xor(k, o));
+        if (lane == 0) atomicMax(&s.top, k);
+    }
+    __syncthreads();
+    const int key = s.top;
+    if (key <= 0xFFFF - 0xFC00) {
+        if (tid == 0) a.tokens[row] = -1;
+        return;
+    }
+    const uint32_t top_bits = key & 0x8000 ? key & 0x7FFFu : 0xFFFFu - key;
+    const float top = h2f(top_bits);
+    uint32_t bin = top_bits;
+    int which = 0;
+    if (!P.greedy) {
+        auto counter = [&](uint32_t h) { return static_cast<int>((s.hist[h & 0x7FFFu] >> ((h >> 11) & 16)) & 0xFFFFu); };
+        auto weight = [&](uint32_t h) { return h == top_bits ? 1.0 : P.weight(h2f(h), top); };
+        auto step_of = [](uint32_t h) {  // between neighbouring values of h's binade
+            const uint32_t low = max(h & 0x7C00u, 0x400u);
+            return static_cast<double>(h2f(low + 1) - h2f(low));
+        };
+        // Counts and masses of the units, a wave to the two units of an exponent.  The
+        // 1024 values of a binade are evenly spaced, so a weight is the one at the
+        // start of its 64 values (lanes 0-15: of the positive ones, 16-31: of the
+        // negative ones) times one of 64 that all of these share.
+        for (int e = wave; e < 32; e += kWaves) {
+            const uint32_t first = static_cast<uint32_t>(e) << 10;  // smallest magnitude
+            int n_pos = 0, n_neg = 0;
+            double w_pos = 0.0, w_neg = 0.0;
+            uint32_t c[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) c[j] = s.hist[first + 64 * j + lane];
+            if (e == 31) {  // infinities and NaN: +inf alone of them is a token
+                if (lane == 0) {
+                    n_pos = c[0] & 0xFFFFu;
+                    w_pos = n_pos;
+                    c[0] &= 0xFFFF0000u;
+                }
+                int outside = 0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) outside += (c[j] & 0xFFFFu) + (c[j] >> 16);
+                outside = wave_sum(outside);
+                if (lane == 0 && outside) atomicAdd(&s.outside, outside);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    n_pos += c[j] & 0xFFFFu;
+                    n_neg += c[j] >> 16;
+                }
+                if (__any(n_pos + n_neg > 0)) {
+                    const double up = exp2_neg(-step_of(first) * P.c * (63 - lane)), down = lane_mirror(up);
+                    // largest of the 64 values
+                    const float base = lane < 16 ? h2f(first + 64 * lane + 63) : h2f(0x8000u | (first + 64 * (lane & 15)));
+                    const double start = top == INFINITY ? 0.0 : exp2_neg(fmin((static_cast<double>(base) - top) * P.c, 0.0));
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        // the largest logit's own 64 values, some of them above it, come below
+                        const uint32_t own = first + 64 * j;
+                        const uint32_t cp = own >> 6 == top_bits >> 6 ? 0 : c[j] & 0xFFFFu;
+                        const uint32_t cn = (0x8000u | own) >> 6 == top_bits >> 6 ? 0 : c[j] >> 16;
+                        w_pos = fma(lane_double(start, j), static_cast<double>(cp), w_pos);
+                        w_neg = fma(lane_double(start, 16 + j), static_cast<double>(cn), w_neg);
+                    }
+                    w_pos *= up;
+                    w_neg *= down;
+                    if (first >> 10 == (top_bits & 0x7FFFu) >> 10) {
+                        const uint32_t h = (top_bits & ~63u) + lane;
+                        const int own = counter(h);
+                        const double w = own ? weight(h) * own : 0.0;
+                        w_pos += (h & 0x8000u) ? 0.0 : w;
+                        w_neg += (h & 0x8000u) ? w : 0.0;
+                    }
+                }
+            }
+            n_pos = wave_sum(n_pos);
+            n_neg = wave_sum(n_neg);
+            w_pos = wave_scan(w_pos);
+            w_neg = wave_scan(w_neg);
+            if (lane == 63) {
+                s.count[31 - e] = n_pos;
+                s.mass[31 - e] = w_pos;
+                s.count[32 + e] = n_neg;  // [63]: always 0
+                s.mass[32 + e] = w_neg;
+            }
+        }
+        __syncthreads();
+        // inclusive sums over the units, a unit to a lane, in every wave
+        const int unit_n = s.count[lane];
+        const double unit_w = s.mass[lane];
+        const int upto_n = wave_scan(unit_n);
+        const double upto_w = wave_scan(unit_w);
+        const int total = last_lane(upto_n);
+        if (R == 0 && total + s.outside != grans * 8) {
+            // a counter overflowed (over 65535 equal logits): by ranks, 32-bit counters
+            __syncthreads();
+            sample_ranks<uint16_t>(a, row, *reinterpret_cast<Lds32*>(raw));
+            return;
+        }
+        // The place where the order has had `n` tokens (Count), the first token at
+        // which the mass reaches (Reach) or passes (Pass) `m`, or the last token
+        // whose weight is at least `m` (Weight).  The unit by its sums, then a value
+        // of it to each thread.
+        enum Kind { Count, Reach, Pass, Weight };
+        auto find = [&](Kind kind, int n, double m) {
+            auto at_border = [&](int upto, double mass) {
+                return kind == Count ? upto >= n : kind == Pass ? mass > m : mass >= m;
+            };
+            const uint64_t some = __ballot(unit_n > 0);
+            int u;
+            if (kind == Weight) {
+                // the last unit whose largest value is heavy enough
+                const uint64_t heavy = __ballot(unit_n > 0 && weight(unit_bits(lane, 0)) >= m);
+                u = heavy ? 63 - __builtin_clzll(heavy) : __builtin_ctzll(some);
+            } else {
+                const uint64_t hit = __ballot(unit_n > 0 && at_border(upto_n, upto_w));
+                u = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+            }
+            const uint32_t h = unit_bits(u, tid);
+            const int c = u == 0 && tid > 0 ? 0 : counter(h);
+            double w = 0.0;
+            if (__any(c > 0)) w = c ? weight(h) : 0.0;
+            int cu = wave_scan(c);
+            double wu = wave_scan(w * c);
+            __syncthreads();  // the last place has been read
+            if (lane == 63) {
+                s.wave_count[wave] = cu;
+                s.wave_mass[wave] = wu;
+            }
+            if (tid == 0) {
+                s.hit = kind == Weight ? -1 : kThreads;
+                s.last = -1;
+            }
+            __syncthreads();
+            cu += __builtin_amdgcn_readlane(upto_n - unit_n, u);
+            wu += lane_double(upto_w - unit_w, u);
+#pragma unroll
+            for (int v = 0; v < kWaves - 1; ++v) {
+                cu += v < wave ? s.wave_count[v] : 0;
+                wu += v < wave ? s.wave_mass[v] : 0.0;
+            }
+            // lanes of a wave stand in order: one atomic a wave
+            const uint64_t has = __ballot(c > 0);
+            const uint64_t good = __ballot(c > 0 && (kind == Weight ? w >= m : at_border(cu, wu)));
+            if (lane == 0) {
+                if (has) atomicMax(&s.last, 64 * wave + 63 - __builtin_clzll(has));
+                if (good && kind == Weight) atomicMax(&s.hit, 64 * wave + 63 - __builtin_clzll(good));
+                if (good && kind != Weight) atomicMin(&s.hit, 64 * wave + __builtin_ctzll(good));
+            }
+            __syncthreads();
+            const int hit = s.hit;
+            const bool none_hits = hit < 0 || hit == kThreads;
+            if (kind == Weight && none_hits) {  // the place before this unit
+                if (tid == 0) s.place = {0, 0, __builtin_amdgcn_readlane(upto_n - unit_n, u), 0.0, 0.0};
+            } else if (tid == (none_hits ? s.last : hit)) {
+                Place p{h, 0, cu - c, wu - w * c, w};
+                if (kind == Count) p.in_bin = n - p.count;
+                else if (kind == Weight) p.in_bin = c;
+                else if (c == 1 || none_hits) p.in_bin = kind == Pass ? c - 1 : c;  // none: rounding hid it, the last token
+                else {
+                    const double q = (m - p.mass) / p.w;
+                    p.in_bin = kind == Pass ? static_cast<int>(fmin(fmax(floor(q), 0.0), c - 1.0))
+                                            : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(c)));
+                }
+                s.place = p;
+            }
+            __syncthreads();
+            return s.place;
+        };
+        Place at{top_bits, 0, 0, 0.0, 1.0};
+        int n = total, cut = total;
+        double mass = lane_double(upto_w, 63);
+#pragma nounroll
+        for (int stage = 0; stage < 6; ++stage) {
+            Kind kind = Count;
+            int number = 0;
+            double amount = 0.0;
+            if (stage == 0) {  // the first top_k and their mass
+                if (P.top_k <= 0 || P.top_k >= n) continue;
+                number = n = cut = P.top_k;
+            } else if (stage == 1) {  // of those, top_p of their mass
+                if (P.top_p >= 1.0) continue;
+                kind = Reach;
+                amount = P.top_p * mass;
+            } else if (stage == 2) {  // of those, what min_p keeps
+                if (P.min_p <= 0.0) continue;
+                kind = Weight;
+                amount = P.min_p;
+            } else if (stage == 3) {  // the mass of the kept
+                if (cut == n) continue;
+                number = cut;
+            } else if (stage == 4) {  // the draw
+                kind = Pass;
+                amount = P.u * mass;
+            } else {  // rounding put it behind the last kept token
+                if (at.count + at.in_bin < cut) continue;
+                number = cut;
+            }
+            const Place p = find(kind, number, amount);
+            if (stage == 1 || stage == 2) {
+                cut = min(cut, max(p.count + p.in_bin, 1));
+            } else if (stage < 4) {
+                mass = p.mass + p.in_bin * p.w;
+            } else {
+                at = p;
+                at.in_bin -= stage == 5 ? 1 : 0;
+            }
+        }
+        bin = at.bin;
+        which = at.in_bin;
+        __syncthreads();  // the counters have been read: the list takes their place
+    }
+
+    // the index of token number `which` of `bin`: its tokens' indices in any order
+    // into LDS (over the counters), the one that has `which` before it
+    int* list = reinterpret_cast<int*>(s.hist);
+    const uint32_t pair = bin | (bin << 16);
+    auto look = [&](int gr, const uint4& w) {
+        const uint32_t ws[4] = {plain(w.x) ^ pair, plain(w.y) ^ pair, plain(w.z) ^ pair, plain(w.w) ^ pair};
+        uint32_t zero = 0;  // a half that is zero borrows from its top bit
+#pragma unroll
+        for (int j = 0; j < 4; ++j) zero |= (ws[j] - 0x00010001u) & ~ws[j];
+        if (!(zero & 0x80008000u)) return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (((ws[j / 2] >> (16 * (j & 1))) & 0xFFFFu) == 0) {
+                const int n = atomicAdd(&s.listed, 1);
+                if (n < kListed16) list[n] = rd.index(gr) + j;
+            }
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (tid + i * kThreads < grans) look(tid + i * kThreads, keep[i]);
+    } else {
+        for (int g0 = tid; g0 < grans; g0 += 4 * kThreads) {
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = rd.load_packed(g0 + i * kThreads, none);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (g0 + i * kThreads < grans) look(g0 + i * kThreads, w[i]);
+        }
+    }
+    __syncthreads();
+    const int n = s.listed;
+    if (n > kListed16) {
+        const int i = nth_index(rd, which, none, [&](uint32_t x) { return (x == 0x8000u ? 0u : x) == bin; }, s.wave_count, &s.answer);
+        if (tid == 0) a.tokens[row] = i;
+        return;
+    }
+    for (int i = tid; i < n; i += kThreads) {
+        const int mine = list[i];
+        int before = 0;
+        for (int k = 0; k < n; ++k) before += list[k] < mine ? 1 : 0;
+        if (before == which) a.tokens[row] = mine;
+    }
 }
 
 }  // namespace
@@ -818,14 +817,9 @@ __global__ void clear_rows(int* rows, int n) {
 
 using namespace gdsllm;
 
-extern "C" size_t gdsllm_sample_tokens_workspace_size(int64_t rows, int64_t vocab) {
-    return rows > 0 && vocab > 65535 ? static_cast<size_t>(rows) * sizeof(int32_t) : 0;
-}
-
 extern "C" int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, int64_t vocab, int64_t ld,
                                     const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
-                                    const float* min_p, int64_t* tokens, void* workspace, size_t workspace_bytes,
-                                    void* stream) {
+                                    const float* min_p, int64_t* tokens, void* stream) {
     const std::string n = "sample_tokens";
     auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
     if (bits != 16 && bits != 32) return bad("logits must be fp16 or fp32 (bits 16 or 32)");
@@ -837,39 +831,20 @@ extern "C" int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, 
     if (!u) return bad("one uniform number a row expected");
     if (reinterpret_cast<uintptr_t>(logits) % (bits / 8) || reinterpret_cast<uintptr_t>(tokens) % 8 ||
         (reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) |
-         reinterpret_cast<uintptr_t>(top_p) | reinterpret_cast<uintptr_t>(min_p) |
-         reinterpret_cast<uintptr_t>(workspace)) % 4)
+         reinterpret_cast<uintptr_t>(top_p) | reinterpret_cast<uintptr_t>(min_p)) % 4)
         return bad("misaligned pointer");
-    const SampleArgs a{logits, u, temperature, top_p, min_p, top_k, tokens, ld, static_cast<int>(vocab)};
-    const dim3 grid(static_cast<unsigned>(rows)), block(kThreads);
-    const hipStream_t s = as_stream(stream);
     int lg = 0;
     while ((int64_t(1) << lg) < vocab) ++lg;
-    const int shift = 62 - lg;
-    if (bits == 16) {
-        const size_t need = gdsllm_sample_tokens_workspace_size(rows, vocab);
-        if (need > 0 && (!workspace || workspace_bytes < need))
-            return bad("workspace of " + std::to_string(need) + " bytes needed, got " + std::to_string(workspace_bytes));
-        int* over = need > 0 ? static_cast<int*>(workspace) : nullptr;
-        if (over)
-            hipLaunchKernelGGL(clear_rows, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, over,
-                               static_cast<int>(rows));
-        auto launch = [&](auto kernel) {
-            if (int rc = prepare_lds(reinterpret_cast<const void*>(kernel), sizeof(Lds16))) return rc;
-            hipLaunchKernelGGL(kernel, grid, block, sizeof(Lds16), s, a, over);
-            return static_cast<int>(GDSLLM_OK);
-        };
-        const int64_t grans = vocab / 8 + 2;  // at most, wherever the rows begin
-        if (int rc = grans <= 4 * kThreads ? launch(&sample_f16<4>) : launch(&sample_f16<0>)) return rc;
-        // over 65535 tokens a 16-bit counter can overflow; such rows are left to this
-        if (over) {
-            if (int rc = prepare_lds(reinterpret_cast<const void*>(&sample_any<uint16_t>), sizeof(Lds32))) return rc;
-            hipLaunchKernelGGL(sample_any<uint16_t>, grid, block, sizeof(Lds32), s, a, static_cast<const int*>(over), shift);
-        }
-    } else {
-        if (int rc = prepare_lds(reinterpret_cast<const void*>(&sample_any<uint32_t>), sizeof(Lds32))) return rc;
-        hipLaunchKernelGGL(sample_any<uint32_t>, grid, block, sizeof(Lds32), s, a, static_cast<const int*>(nullptr), shift);
-    }
-    if (int rc = check_hip(hipGetLastError(), "sample_tokens launch")) return rc;
-    return ok();
+    const SampleArgs a{logits, u, temperature, top_p, min_p, top_k, tokens, ld, static_cast<int>(vocab), 62 - lg};
+    auto launch = [&](auto kernel, size_t lds) {
+        if (int rc = prepare_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), lds, as_stream(stream), a);
+        return check_hip(hipGetLastError(), "sample_tokens launch");
+    };
+    static_assert(sizeof(Lds32) <= sizeof(Lds16), "a row that overflows its counters reuses their space");
+    const int64_t granules = vocab / 8 + 2;  // at most, wherever the rows begin
+    const int rc = bits == 32                 ? launch(&sample_f32, sizeof(Lds32))
+                   : granules <= 4 * kThreads ? launch(&sample_f16<4>, sizeof(Lds16))
+                                              : launch(&sample_f16<0>, sizeof(Lds16));
+    return rc ? rc : ok();
 }

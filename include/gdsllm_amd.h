@@ -516,10 +516,9 @@ int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ld
  * top_k, top_p and min_p hold one value a row; null: 1, all, 1, 0.
  * Weights and sums in 64 bits.  Replaces _sample (engine.py:47-96), which
  * sorts the logits and draws on the host side of a sync.                     */
-size_t gdsllm_sample_tokens_workspace_size(int64_t rows, int64_t vocab);
 int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-                         int64_t* tokens, void* workspace, size_t workspace_bytes, void* stream);
+                         int64_t* tokens, void* stream);
 
 /* ------------------------------------------------------ measurement helpers --
  * Not on the matvec path and with no counterpart in the reference: reference

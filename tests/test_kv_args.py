@@ -114,8 +114,8 @@ def test_assign_refusals():
 
 
 def test_sample_refusals():
-    def call(l=8, bits=16, rows=1, v=10, ld=10, u=8, t=None, k=None, p=None, m=None, out=8, ws=None, wb=0):
-        return capi().gdsllm_sample_tokens(l, bits, rows, v, ld, u, t, k, p, m, out, ws, wb, None)
+    def call(l=8, bits=16, rows=1, v=10, ld=10, u=8, t=None, k=None, p=None, m=None, out=8):
+        return capi().gdsllm_sample_tokens(l, bits, rows, v, ld, u, t, k, p, m, out, None)
 
     assert call(rows=0) == 0
     assert call(bits=8) == BAD and "fp16 or fp32" in _err()
