@@ -20,6 +20,7 @@
 #include <climits>
 
 #include "kv_cache.h"
+#include "wave.h"
 
 namespace gdsllm {
 namespace {
@@ -27,6 +28,7 @@ namespace {
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;              // log2 of how far a score may pass the reference
 constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
 constexpr int kMaxPages = kSegment / 16;   // segments begin on a block of 64 tokens
 constexpr int kBlock = 64;                 // tokens of a unit of work
@@ -278,15 +280,17 @@ struct RowTile {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
                 mx = over_groups(mx, [](float u, float v) { return fmaxf(u, v); });
-                const float m_new = fmaxf(m, mx);
-                const float ref = m_new == -INFINITY ? 0.f : m_new;
-                if (__any(m_new > m)) {
-                    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+                // the reference follows the maximum only when that has left it 2^8 behind:
+                // weights up to 2^8 are as good in fp16 and the sums in fp32
+                if (__any(mx > m + kSlack)) {
+                    const float m_new = fmaxf(m, mx);
+                    const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                     l *= alpha;
 #pragma unroll
                     for (int j = 0; j < DB; ++j) acc[j] *= alpha;
                     m = m_new;
                 }
+                const float ref = m == -INFINITY ? 0.f : m;
                 half8_t pf[NT / 2];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -369,8 +373,8 @@ struct RowTile {
     }
 };
 
-// 128 rows over blocks [block0, block1) of a sequence, 32 rows to each of four
-// waves, for prompts.  BN tokens at a time are converted to fp16 once, into LDS
+// 32 rows to each of NW waves over blocks [block0, block1) of a sequence, for
+// prompts.  BN tokens at a time are converted to fp16 once, into LDS
 // (two buffers, one barrier a tile), while the tile before is worked on; matrix
 // tiles are 32x32x16:
 //  * S^T = K Q^T: K [token][channel] from LDS, Q in registers; lane l receives,
@@ -381,13 +385,13 @@ struct RowTile {
 // The four-token pieces of V^T come from 4x4 byte transposes of the codes.  Rows
 // of both tiles are 16 bytes longer than their data: reads and writes touch
 // every bank once.
-template <bool E4M3, int D>
+template <bool E4M3, int D, int NW>
 struct PromptTile {
-    static constexpr int kRows = 128, kThreads = 256, kD = D, kPerCu = D == 256 ? 1 : 2;
+    static constexpr int kRows = 32 * NW, kThreads = 64 * NW, kD = D, kPerCu = D == 256 ? 1 : 2;
     static constexpr int BN = D == 256 ? 32 : 64;
     static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
-    static constexpr int KC = BN * D / 16 / 256;                  // 16-code chunks of K a thread converts
-    static constexpr int VQ = BN / 4, VC = VQ * (D / 8), VN = (VC + 255) / 256;  // token quads; (quad, 8 channels) pieces
+    static constexpr int KC = (BN * D / 16 + kThreads - 1) / kThreads;             // 16-code chunks of K a thread converts
+    static constexpr int VQ = BN / 4, VC = VQ * (D / 8), VN = (VC + kThreads - 1) / kThreads;  // token quads; (quad, 8 channels) pieces
     struct Page {
         float c, e, inv;
         int id;
@@ -402,13 +406,13 @@ struct PromptTile {
         uint64_t v[VN][4];
     };
 
-    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows<128>& R, int tile, int head, int block0,
+    __device__ static void run(const AttendArgs& a, Lds& s, int b, const Rows<kRows>& R, int tile, int head, int block0,
                                int block1, int slot, int early) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31,
                   h = lane >> 5;
         const int bl = a.c.block_log2;
-        const int k0 = block0 * kBlock, k1 = min(block1 * kBlock, R.keys(a, tile * 128, 128));
-        const int w0 = tile * 128 + wave * 32;  // this wave's rows
+        const int k0 = block0 * kBlock, k1 = min(block1 * kBlock, R.keys(a, tile * kRows, kRows));
+        const int w0 = tile * kRows + wave * 32;  // this wave's rows
         const int r = w0 + col;
         const bool valid = r < R.rows;
         const int t_row = R.start + (valid ? r / a.group : 0), h_row = head * a.group + (valid ? r % a.group : 0);
@@ -451,15 +455,15 @@ struct PromptTile {
             auto load = [&](Codes& w, int base) {
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
-                    const int c = tid + 256 * i, token = base + c / (D / 16);
+                    const int c = tid + kThreads * i, token = base + c / (D / 16);
                     const int64_t row = ((static_cast<int64_t>(s.page[(token >> bl) - p0].id) * a.c.kv_heads + head) << bl) +
                                         (token & ((1 << bl) - 1));
                     w.k[i] = *reinterpret_cast<const u32x4_t*>(a.c.k + row * D + 16 * (c % (D / 16)));
                 }
 #pragma unroll
                 for (int i = 0; i < VN; ++i) {
-                    const int c = tid + 256 * i, token = base + 4 * (c % VQ);
-                    if (VC % 256 == 0 || c < VC) {
+                    const int c = tid + kThreads * i, token = base + 4 * (c % VQ);
+                    if (VC % kThreads == 0 || c < VC) {
                         const int64_t row = ((static_cast<int64_t>(s.page[(token >> bl) - p0].id) * a.c.kv_heads + head) << bl) +
                                             (token & ((1 << bl) - 1));
                         const uint8_t* p = a.c.v + row * D + 8 * (c / VQ);
@@ -471,7 +475,7 @@ struct PromptTile {
             auto store = [&](Codes& w, int base, int buf) {
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
-                    const int c = tid + 256 * i;
+                    const int c = tid + kThreads * i;
                     uint32_t f[8];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) codes_to_f16<E4M3>(w.k[i][j], f[2 * j], f[2 * j + 1]);
@@ -482,8 +486,8 @@ struct PromptTile {
                 const bool tail = base + BN > k1 || some_lost;
 #pragma unroll
                 for (int i = 0; i < VN; ++i) {
-                    const int c = tid + 256 * i, quad = c % VQ;
-                    if (VC % 256 == 0 || c < VC) {
+                    const int c = tid + kThreads * i, quad = c % VQ;
+                    if (VC % kThreads == 0 || c < VC) {
                         if (tail) {  // what lies behind the last token, or in a lost block, may be no number
                             const int token = base + 4 * quad;
                             const bool none = s.page[(token >> bl) - p0].inv == 0.f;
@@ -555,15 +559,15 @@ struct PromptTile {
                         swap32(p, q);
                         mx = fmaxf(p, q);
                     }
-                    const float m_new = fmaxf(m, mx);
-                    const float ref = m_new == -INFINITY ? 0.f : m_new;
-                    if (__any(m_new > m)) {
-                        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+                    if (__any(mx > m + kSlack)) {  // as in RowTile
+                        const float m_new = fmaxf(m, mx);
+                        const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                         l *= alpha;
 #pragma unroll
                         for (int j = 0; j < DT; ++j) acc[j] *= alpha;
                         m = m_new;
                     }
+                    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         const float er = pg[u].e - ref;
@@ -604,7 +608,7 @@ struct PromptTile {
                     *reinterpret_cast<uint2*>(o + 32 * j + 2 * i + 4 * h) = w;
                 }
         } else {
-            const int64_t row = static_cast<int64_t>(slot) * 128 + wave * 32 + col;
+            const int64_t row = static_cast<int64_t>(slot) * kRows + wave * 32 + col;
 #pragma unroll
             for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -651,12 +655,7 @@ __global__ __launch_bounds__(256, T::kPerCu) void attend_shared(AttendArgs a) {
         int carry = 0;
         for (int b0 = 0; b0 < a.requests; b0 += 256) {
             const int b = b0 + tid, w = b < a.requests ? Rows<T::kRows>(a, b).work(a) : 0;
-            int upto = w;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int u = __shfl_up(upto, o);
-                if (lane >= o) upto += u;
-            }
+            int upto = wave_scan(w);
             __syncthreads();
             if (lane == 63) s_part[wave] = upto;
             __syncthreads();
@@ -726,8 +725,13 @@ __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
         const int i = tid / TPR + k * NG;
         early[k] = i < parts ? sums(i) : float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const float2 mine = tid < parts ? a.part_ml[at(tid)] : make_float2(-INFINITY, 0.f);
-    float m = mine.x;
+    float my_m = -INFINITY, my_l = 0.f;
+    if (tid < parts) {
+        const float2 x = a.part_ml[at(tid)];
+        my_m = x.x;
+        my_l = x.y;
+    }
+    float m = my_m;
     for (int i = tid + THREADS; i < parts; i += THREADS) m = fmaxf(m, a.part_ml[at(i)].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -742,9 +746,13 @@ __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
         if (i0 > 0) __syncthreads();
         float w = 0.f;
         if (i0 + tid < parts) {
-            const float2 x = i0 == 0 ? mine : a.part_ml[at(i0 + tid)];
-            w = __builtin_amdgcn_exp2f(x.x - ref);
-            l = fmaf(x.y, w, l);
+            if (i0 > 0) {
+                const float2 x = a.part_ml[at(i0 + tid)];
+                my_m = x.x;
+                my_l = x.y;
+            }
+            w = __builtin_amdgcn_exp2f(my_m - ref);
+            l = fmaf(my_l, w, l);
         }
         s_f[tid] = w;
         lds_barrier();
@@ -767,7 +775,7 @@ __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < NWV; ++i) l += s_l[i];
-#pragma unroll
+#pragma unroll 8
     for (int i = 1; i < NG; ++i) acc += s_o[tid + i * TPR];
     const float inv = inverse(l);
     uint16_t* out = a.o + (R.start + row / a.group) * a.ldo + (head * a.group + row % a.group) * D + 4 * tid;
@@ -822,12 +830,16 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
                     max_len <= kWholeTokens || sequences >= 8 * resident);
     }
     if (many) {
-        p.many.rows = 128;
-        if (p.few.on) p.many.min_rows = kFewRows + 1;
         const int64_t resident = (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus);
+        // eight waves to a tile (each converts half as much) where that still leaves
+        // two workgroups to a compute unit, one after the other: 4096 tokens of 32
+        // heads 173 us against 183; 4 chunks of 300 tokens 166 against 162
+        const bool wide = head_dim <= 128 && requests * kv_heads * ((rows + 255) / 256) >= resident;
+        p.many.rows = wide ? 256 : 128;
+        if (p.few.on) p.many.min_rows = kFewRows + 1;
         const int64_t sequences = requests * kv_heads * ((rows + 127) / 128);
         finish_part(&p.many, requests, kv_heads, head_dim, rows, max_len, resident,
-                    max_len <= kWholeTokens || 2 * sequences >= resident);
+                    wide || max_len <= kWholeTokens || 2 * sequences >= resident);
     }
     return p;
 }
@@ -871,7 +883,10 @@ int launch_attend(AttendArgs a, const Plan& p, int64_t line, int64_t max_rows, c
     if (int rc = launch_part<RowTile<E4M3, D, 8>, RowTile<E4M3, D, 4>>(a, p.few, line, p.many.on ? kFewRows : max_rows, workspace, s))
         return rc;
     a.zero_tail = p.few.on ? 0 : zero_tail;
-    return launch_part<PromptTile<E4M3, D>, PromptTile<E4M3, D>>(a, p.many, line, max_rows, workspace + p.few.bytes, s);
+    char* ws = workspace + p.few.bytes;
+    if constexpr (D <= 128)
+        if (p.many.rows == 256) return launch_part<PromptTile<E4M3, D, 8>, PromptTile<E4M3, D, 4>>(a, p.many, line, max_rows, ws, s);
+    return launch_part<PromptTile<E4M3, D, 4>, PromptTile<E4M3, D, 4>>(a, p.many, line, max_rows, ws, s);
 }
 
 bool attend_sizes(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {

@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "kv_cache.h"
+#include "wave.h"
 
 namespace gdsllm {
 
@@ -61,74 +62,74 @@ struct AssignArgs {
     int n, width, ring_size, block_log2, max_tokens;
 };
 
-// Inclusive sums over the workgroup of one int64 per thread.
-template <int THREADS>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = __shfl_up(static_cast<long long>(v), o);
-        if (lane >= o) v += u;
-    }
-    __syncthreads();  // part may still be read from the last scan
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) v += part[w];
-    return v;
-}
-
-// Every workgroup takes the sums over all requests for itself (two scans over
-// at most 8192 of them: cheaper than a second launch or a grid barrier) and
-// then writes its share of the tables and of the token rows.
+// Every workgroup takes the sums over all requests for itself (at most 8192 of
+// them: cheaper than a second launch or a grid barrier) and then writes its share
+// of the tables and of the token rows.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
     extern __shared__ int32_t lds[];
     int32_t* ends = lds;              // tokens up to and with request r, at most max_tokens + 1
     int32_t* first = lds + a.n;       // blocks taken before request r; -1 where it is not served
     int32_t* given = lds + 2 * a.n;   // blocks given back before request r
-    __shared__ int64_t part[THREADS / 64];
+    constexpr int WAVES = THREADS / 64;
+    __shared__ uint64_t part[3][WAVES];
     __shared__ int taken, returned;
-    const int bs = 1 << a.block_log2, tid = threadIdx.x;
+    const int bs = 1 << a.block_log2, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row_tokens = static_cast<int64_t>(a.width) << a.block_log2;
-    if (tid == 0) taken = 0;
-    const int head = min(max(a.state[0], 0), a.ring_size - 1), count = min(max(a.state[1], 0), a.ring_size);
-
     auto len_of = [&](int r) { return max(a.lens[r], 0); };
     auto add_of = [&](int r) { return max(a.delta[r], 0); };
     auto drop_of = [&](int r) {
         return static_cast<int>(min(static_cast<int64_t>(len_of(r)), max(-static_cast<int64_t>(a.delta[r]), int64_t(0))));
     };
+    // entry `i` (at most ring_size) behind `head`
+    auto ring_at = [&](int head, int i) {
+        const int64_t at = static_cast<int64_t>(head) + i;
+        return at < a.ring_size ? at : at < 2 * static_cast<int64_t>(a.ring_size) ? at - a.ring_size : 0;
+    };
     auto blocks = [&](int64_t t) { return static_cast<int>((t + bs - 1) >> a.block_log2); };
+    // New blocks of request r, -1 where its row is too short.  Its tokens may still
+    // lie behind max_tokens; then so do all later ones', and none of them is served.
+    auto need_of = [&](int r) {
+        const int add = add_of(r);
+        const int64_t after = static_cast<int64_t>(len_of(r)) + add;
+        return add == 0 ? 0 : after <= row_tokens ? blocks(after) - blocks(len_of(r)) : -1;
+    };
 
     const int per = (a.n + THREADS - 1) / THREADS, r0 = min(tid * per, a.n), r1 = min(r0 + per, a.n);
-    int64_t sum = 0;
-    for (int r = r0; r < r1; ++r) sum += add_of(r);
-    int64_t at = block_scan<THREADS>(sum, part) - sum;
-    const int64_t at0 = at;
-    auto need_of = [&](int r, int64_t end) {
-        const int64_t after = static_cast<int64_t>(len_of(r)) + add_of(r);
-        if (add_of(r) == 0) return 0;
-        return after <= row_tokens && end <= a.max_tokens ? blocks(after) - blocks(len_of(r)) : -1;
-    };
-    int64_t need = 0, back = 0;
+    const int head0 = a.state[0], count0 = a.state[1];
+    if (tid == 0) taken = 0;
+    uint64_t tokens = 0, need = 0, back = 0;
     for (int r = r0; r < r1; ++r) {
-        at += add_of(r);
-        need += max(need_of(r, at), 0);
+        tokens += add_of(r);
+        need += max(need_of(r), 0);
         back += blocks(len_of(r)) - blocks(len_of(r) - drop_of(r));
     }
-    int64_t upto = block_scan<THREADS>(need, part) - need;
-    const int64_t back_end = block_scan<THREADS>(back, part);
-    if (tid == THREADS - 1) returned = static_cast<int>(min(back_end, static_cast<int64_t>(a.ring_size)));
-    int64_t back_at = back_end - back;
-    at = at0;
+    uint64_t at = wave_scan(tokens), upto = wave_scan(need), back_at = wave_scan(back);
+    if (lane == 63) {
+        part[0][wave] = at;
+        part[1][wave] = upto;
+        part[2][wave] = back_at;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        at += part[0][w];
+        upto += part[1][w];
+        back_at += part[2][w];
+    }
+    if (tid == THREADS - 1) returned = static_cast<int>(min(back_at, static_cast<uint64_t>(a.ring_size)));
+    at -= tokens;
+    upto -= need;
+    back_at -= back;
+    const int head = min(max(head0, 0), a.ring_size - 1), count = min(max(count0, 0), a.ring_size);
     int most = 0;
     for (int r = r0; r < r1; ++r) {
         at += add_of(r);
-        const int n = need_of(r, at);
-        const bool served = n == 0 || (n > 0 && upto + n <= count);
-        ends[r] = static_cast<int32_t>(min(at, static_cast<int64_t>(a.max_tokens) + 1));
-        first[r] = served ? static_cast<int32_t>(min(upto, static_cast<int64_t>(a.ring_size))) : -1;
-        given[r] = static_cast<int32_t>(min(back_at, static_cast<int64_t>(a.ring_size)));
+        const int n = need_of(r);
+        const bool served = n == 0 ? add_of(r) == 0 || at <= static_cast<uint64_t>(a.max_tokens)
+                                   : n > 0 && at <= static_cast<uint64_t>(a.max_tokens) && upto + n <= static_cast<uint64_t>(count);
+        ends[r] = static_cast<int32_t>(min(at, static_cast<uint64_t>(a.max_tokens) + 1));
+        first[r] = served ? static_cast<int32_t>(min(upto, static_cast<uint64_t>(a.ring_size))) : -1;
+        given[r] = static_cast<int32_t>(min(back_at, static_cast<uint64_t>(a.ring_size)));
         upto += max(n, 0);
         if (served && n > 0) most = static_cast<int>(upto);
         back_at += blocks(len_of(r)) - blocks(len_of(r) - drop_of(r));
@@ -146,21 +147,39 @@ __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
         a.state_out[1] = count - taken + min(returned, room);
     }
 
-    // new and returned blocks: one request to a wave
-    const int waves = THREADS / 64, lane = tid & 63;
-    for (int r = static_cast<int>(blockIdx.x) * waves + (tid >> 6); r < a.n; r += static_cast<int>(gridDim.x) * waves) {
-        const int len = len_of(r), add = add_of(r), have = blocks(len);
-        int32_t* row = a.tables + r * a.ld_table;
-        if (add > 0) {
-            const int n = blocks(static_cast<int64_t>(len) + add) - have;
-            if (first[r] >= 0)
-                for (int j = lane; j < n; j += 64)
-                    row[have + j] = a.ring[(static_cast<int64_t>(head) + first[r] + j) % a.ring_size];
-        } else {
-            const int keep = blocks(len - drop_of(r));
-            for (int j = lane; j < have - keep; j += 64)
-                if (keep + j < a.width && given[r] + j < room)
-                    a.ring[(static_cast<int64_t>(head) + count + given[r] + j) % a.ring_size] = row[keep + j];
+    // New and returned blocks: a request to a lane, which copies them itself where
+    // they are few (a decoding step), else the whole wave does.
+    constexpr int kOwn = 4;
+    for (int base = (static_cast<int>(blockIdx.x) * WAVES + wave) * 64; base < a.n; base += static_cast<int>(gridDim.x) * WAVES * 64) {
+        const int r = base + lane;
+        int n = 0, from = 0, ring = 0;  // blocks, the first one's place in the row and in the ring
+        bool take = false;
+        if (r < a.n) {
+            const int len = len_of(r), add = add_of(r), have = blocks(len);
+            take = add > 0;
+            if (take) {
+                n = first[r] >= 0 ? blocks(static_cast<int64_t>(len) + add) - have : 0;
+                from = have;
+                ring = first[r];
+            } else {
+                from = blocks(len - drop_of(r));
+                n = max(min(min(have, a.width) - from, room - given[r]), 0);
+                ring = count + given[r];
+            }
+        }
+        auto copy = [&](int request, int block, int place, bool taken_here) {
+            int32_t* entry = a.tables + request * a.ld_table + block;
+            if (taken_here) *entry = a.ring[ring_at(head, place)];
+            else a.ring[ring_at(head, place)] = *entry;
+        };
+        if (n <= kOwn)
+            for (int j = 0; j < n; ++j) copy(r, from + j, ring + j, take);
+        for (uint64_t many = __ballot(n > kOwn); many; many &= many - 1) {
+            const int l = __builtin_ctzll(many);
+            const int count_l = __builtin_amdgcn_readlane(n, l), from_l = __builtin_amdgcn_readlane(from, l);
+            const int ring_l = __builtin_amdgcn_readlane(ring, l);
+            const bool take_l = __builtin_amdgcn_readlane(take ? 1 : 0, l);
+            for (int j = lane; j < count_l; j += 64) copy(base + l, from_l + j, ring_l + j, take_l);
         }
     }
     // token rows: the request of a row is the first whose end lies past it
@@ -179,7 +198,7 @@ __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
                 pos = len + t - (lo > 0 ? ends[lo - 1] : 0);
                 const int b = pos >> a.block_log2;
                 const int id = b < have ? a.tables[lo * a.ld_table + b]
-                                        : a.ring[(static_cast<int64_t>(head) + first[lo] + b - have) % a.ring_size];
+                                        : a.ring[ring_at(head, first[lo] + b - have)];
                 slot = (id << a.block_log2) + (pos & (bs - 1));
             }
         }
