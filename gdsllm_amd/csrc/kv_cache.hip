@@ -147,11 +147,13 @@ __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
         a.state_out[1] = count - taken + min(returned, room);
     }
 
-    // New and returned blocks: a request to a lane, which copies them itself where
-    // they are few (a decoding step), else the whole wave does.
+    // New and returned blocks: the requests spread over the waves, one to a lane,
+    // which copies its blocks itself where they are few (a decoding step), else the
+    // whole wave does (a prompt's, an ended request's).
     constexpr int kOwn = 4;
-    for (int base = (static_cast<int>(blockIdx.x) * WAVES + wave) * 64; base < a.n; base += static_cast<int>(gridDim.x) * WAVES * 64) {
-        const int r = base + lane;
+    const int waves = static_cast<int>(gridDim.x) * WAVES, share = min((a.n + waves - 1) / waves, 64);
+    for (int base = (static_cast<int>(blockIdx.x) * WAVES + wave) * share; base < a.n; base += waves * share) {
+        const int r = lane < share ? base + lane : a.n;
         int n = 0, from = 0, ring = 0;  // blocks, the first one's place in the row and in the ring
         bool take = false;
         if (r < a.n) {
