@@ -18,7 +18,8 @@ the same contract:
 The decode step's fused launches are exposed as the reference's own units:
 qkv_projections (the three dequant_linear calls of runtime/llama.py:212-214 in
 one launch) and mlp (runtime/llama.py:247-256: gate, up and F.silu(gate)*up in
-one launch, then down).
+one launch, then down).  cached_attention is the attention block between them
+(runtime/llama.py:200-246) over an 8-bit cache.
 """
 
 from __future__ import annotations
@@ -130,6 +131,34 @@ def qkv_projections(x: torch.Tensor, weights: Dict, scratch: Optional[torch.Tens
                                               [m["offset"] for m in metas])
         return tuple(o.unsqueeze(1) for o in outs)
     return tuple(dequant_linear(x, weights, n, scratch) for n in names)
+
+
+def packed_rows(x: torch.Tensor) -> torch.Tensor:
+    """Rows x [T, K] of a step in the shape the projections tell decode from
+    prefill by: [T, 1, K] for up to 8 rows (a batched GEMV, whichever requests they
+    belong to), else one chunk [1, T, K]."""
+    return x.unsqueeze(1) if x.shape[0] <= 8 else x.unsqueeze(0)
+
+
+def cached_attention(x: torch.Tensor, weights: Dict, cache, layer: int, cos: torch.Tensor, sin: torch.Tensor,
+                     scale: Optional[float] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention block of runtime/llama.py:200-246 over an 8-bit cache: q/k/v
+    projections, rotation and append, attention, o_proj.
+
+    x fp16 [T, hidden]: the step's rows, one request's after another's as
+    cache.begin_step laid them out (a KVCache8; T its max_tokens); cos, sin from
+    rope_table.  Returns [T, hidden].  Inference only: x must need no gradient.
+    """
+    if x.dim() != 2 or cache.slots is None or x.shape[0] != cache.slots.numel():
+        raise ValueError("cached_attention: x must be [T, hidden] with the T rows of cache.begin_step")
+    if not untransformed(x):
+        raise RuntimeError("cached_attention writes a cache: it runs on plain tensors without gradients")
+    T, D = x.shape[0], cache.head_dim
+    if T == 0:
+        return x
+    q, k, v = (p.reshape(T, -1, D) for p in qkv_projections(packed_rows(x), weights, scratch))
+    o = cache.attend(layer, cache.append(layer, k, v, q, cos, sin), scale)
+    return dequant_linear(packed_rows(o.reshape(T, -1)), weights, "self_attn.o_proj", scratch).reshape(T, -1)
 
 
 def _gguf_pair(g, u) -> bool:

@@ -12,6 +12,7 @@ changes, both on the fast side of the same contract:
     into a temporary plus F.linear; an int8 lm_head goes through
     gds_io_ext.int8_linear instead of an fp32 copy of the matrix.
 
+next_tokens draws the step's tokens from lm_head's logits on the device.
 DecodeSweep drives the projection work of a cached decode step (the
 reference's CachedScheduler.forward) as one HIP graph per token.
 """
@@ -25,7 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ext
-from .llama import dequant_linear
+from .llama import dequant_linear, packed_rows
 
 
 def _embed_tokens(token_ids: torch.Tensor, tensors: dict, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -51,6 +52,26 @@ def _lm_head_proj(h: torch.Tensor, tensors: dict, key: str = "lm_head.weight",
     return F.linear(h, w)
 
 
+def next_tokens(h: torch.Tensor, tensors: dict, u: torch.Tensor, key: str = "lm_head.weight",
+                temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+                top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """h [rows, H] -> one token a row, int64: lm_head, then the draw that _sample
+    (engine.py:47-96) makes, without its sync.
+
+    u: uniform numbers in [0, 1), fp32 [rows]; temperature (<= 0: the largest
+    logit's token), top_k, top_p, min_p: one setting a row on the device, or None.
+    A row of NaN gives -1.  The tokens stay on the device, ready for
+    _embed_tokens, so a whole step can be one captured graph.
+    """
+    if h.dim() != 2:
+        raise ValueError("next_tokens: h must be [rows, hidden]")
+    if h.shape[0] == 0:
+        return torch.empty(0, dtype=torch.int64, device=h.device)
+    logits = _lm_head_proj(packed_rows(h), tensors, key, scratch)
+    return ext().sample_tokens(logits.reshape(h.shape[0], -1), u, temperature, top_k, top_p, min_p)
+
+
 _LAYER_PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
                "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
 _UNSUPPORTED = 2  # GDSLLM_ERR_UNSUPPORTED: a valid request no fused kernel serves
@@ -72,8 +93,8 @@ class DecodeSweep:
     the final hidden state: 4 launches per layer + 1 (129 for LLaMA-7B, where
     the reference issues 7 per layer + a dequant and a GEMM for lm_head).
 
-    Attention, RoPE, the norms and the residual adds are not matvec work and
-    stay with the caller, which writes each layer's inputs (attn_in[l],
+    Attention and RoPE (KVCache8.append and attend on q[l], k[l], v[l]), the norms
+    and the residual adds are not matvec work and stay with the caller, which writes each layer's inputs (attn_in[l],
     attn_out[l], mlp_in[l]: fp16 [batch, hidden]; final_in: [batch, hidden])
     before run() and reads q[l], k[l], v[l], o[l], h[l], down[l] and logits.
 
