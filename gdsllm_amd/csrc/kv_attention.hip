@@ -390,8 +390,10 @@ struct PromptTile {
     static constexpr int kRows = 32 * NW, kThreads = 64 * NW, kD = D, kPerCu = D == 256 ? 1 : 2;
     static constexpr int BN = D == 256 ? 32 : 64;
     static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
-    static constexpr int KC = (BN * D / 16 + kThreads - 1) / kThreads;             // 16-code chunks of K a thread converts
-    static constexpr int VQ = BN / 4, VC = VQ * (D / 8), VN = (VC + kThreads - 1) / kThreads;  // token quads; (quad, 8 channels) pieces
+    // 16-code chunks of K, and the ones a thread converts (the last threads none where there are fewer)
+    static constexpr int KT = BN * D / 16, KC = (KT + kThreads - 1) / kThreads;
+    // (four tokens, 8 channels) pieces of V, and the ones a thread converts
+    static constexpr int VQ = BN / 4, VC = VQ * (D / 8), VN = (VC + kThreads - 1) / kThreads;
     struct Page {
         float c, e, inv;
         int id;
@@ -456,6 +458,7 @@ struct PromptTile {
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
                     const int c = tid + kThreads * i, token = base + c / (D / 16);
+                    if (KT % kThreads != 0 && c >= KT) continue;
                     const int64_t row = ((static_cast<int64_t>(s.page[(token >> bl) - p0].id) * a.c.kv_heads + head) << bl) +
                                         (token & ((1 << bl) - 1));
                     w.k[i] = *reinterpret_cast<const u32x4_t*>(a.c.k + row * D + 16 * (c % (D / 16)));
@@ -476,6 +479,7 @@ struct PromptTile {
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
                     const int c = tid + kThreads * i;
+                    if (KT % kThreads != 0 && c >= KT) continue;
                     uint32_t f[8];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) codes_to_f16<E4M3>(w.k[i][j], f[2 * j], f[2 * j + 1]);
@@ -700,89 +704,94 @@ __global__ __launch_bounds__(256, T::kPerCu) void attend_shared(AttendArgs a) {
     }
 }
 
-// Sequences that several workgroups had a part of: one workgroup to a row adds
-// their sums.  Part 0 lies in slot `first`, part i in slot 2 * (first / 2 + i).
-// Its threads first take the parts' maxima and turn them into factors, then D/4
-// threads of four channels in each of NG groups run over every NGth part, and the groups' sums meet in LDS in a fixed order.
+// Sequences that several workgroups had a part of: one workgroup to a row (to
+// every rows-th one where the caller's bound on the rows was too small) adds their
+// sums.  Part 0 lies in slot `first`, part i in slot 2 * (first / 2 + i).  Its
+// threads first take the parts' maxima and turn them into factors, then D/4
+// threads of four channels in each of NG groups run over every NGth part, and the
+// groups' sums meet in LDS in a fixed order.
 template <int RT, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void attend_join(AttendArgs a, int rows) {
     constexpr int TPR = D / 4, NG = THREADS / TPR, NWV = THREADS / 64, EARLY = 2;
     __shared__ float s_f[THREADS], s_m[NWV], s_l[NWV];
     __shared__ __attribute__((aligned(16))) float4_t s_o[THREADS];
     const int b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
-    const int r = blockIdx.x % rows, sequence = blockIdx.x / rows;
-    const int head = sequence % a.c.kv_heads, row = sequence / a.c.kv_heads * RT + r;
+    const int sequence = blockIdx.x / rows, head = sequence % a.c.kv_heads, row0 = sequence / a.c.kv_heads * RT;
     const int2 d = a.parts[static_cast<int64_t>(b) * a.tiles * a.c.kv_heads + sequence];
     const Rows<RT> R(a, b);
-    if (row >= R.rows || d.y == 0) return;  // no such row (d is not set), or whole
+    const int r0 = blockIdx.x % rows, count = min(RT, R.rows - row0);
+    if (r0 >= count || d.y == 0) return;  // no such row (d is not set), or whole
     const int parts = d.y;
-    auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * RT + r; };
-    auto sums = [&](int i) { return *reinterpret_cast<const float4_t*>(a.part_o + at(i) * D + 4 * (tid % TPR)); };
-    // the first parts' sums come in while the factors are made
-    float4_t early[EARLY];
+    for (int r = r0; r < count; r += rows) {
+        if (r > r0) __syncthreads();  // the row before has read its sums
+        auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * RT + r; };
+        auto sums = [&](int i) { return *reinterpret_cast<const float4_t*>(a.part_o + at(i) * D + 4 * (tid % TPR)); };
+        // the first parts' sums come in while the factors are made
+        float4_t early[EARLY];
 #pragma unroll
-    for (int k = 0; k < EARLY; ++k) {
-        const int i = tid / TPR + k * NG;
-        early[k] = i < parts ? sums(i) : float4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    float my_m = -INFINITY, my_l = 0.f;
-    if (tid < parts) {
-        const float2 x = a.part_ml[at(tid)];
-        my_m = x.x;
-        my_l = x.y;
-    }
-    float m = my_m;
-    for (int i = tid + THREADS; i < parts; i += THREADS) m = fmaxf(m, a.part_ml[at(i)].x);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if ((tid & 63) == 0) s_m[wave] = m;
-    lds_barrier();
-#pragma unroll
-    for (int i = 0; i < NWV; ++i) m = fmaxf(m, s_m[i]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < parts; i0 += THREADS) {
-        if (i0 > 0) __syncthreads();
-        float w = 0.f;
-        if (i0 + tid < parts) {
-            if (i0 > 0) {
-                const float2 x = a.part_ml[at(i0 + tid)];
-                my_m = x.x;
-                my_l = x.y;
-            }
-            w = __builtin_amdgcn_exp2f(my_m - ref);
-            l = fmaf(my_l, w, l);
+        for (int k = 0; k < EARLY; ++k) {
+            const int i = tid / TPR + k * NG;
+            early[k] = i < parts ? sums(i) : float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        s_f[tid] = w;
+        float my_m = -INFINITY, my_l = 0.f;
+        if (tid < parts) {
+            const float2 x = a.part_ml[at(tid)];
+            my_m = x.x;
+            my_l = x.y;
+        }
+        float m = my_m;
+        for (int i = tid + THREADS; i < parts; i += THREADS) m = fmaxf(m, a.part_ml[at(i)].x);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if ((tid & 63) == 0) s_m[wave] = m;
         lds_barrier();
-        int i = tid / TPR;
-        if (i0 == 0) {
 #pragma unroll
-            for (int k = 0; k < EARLY; ++k, i += NG)
-                if (i < parts) acc += early[k] * s_f[i];
+        for (int i = 0; i < NWV; ++i) m = fmaxf(m, s_m[i]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        float4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < parts; i0 += THREADS) {
+            if (i0 > 0) __syncthreads();
+            float w = 0.f;
+            if (i0 + tid < parts) {
+                if (i0 > 0) {
+                    const float2 x = a.part_ml[at(i0 + tid)];
+                    my_m = x.x;
+                    my_l = x.y;
+                }
+                w = __builtin_amdgcn_exp2f(my_m - ref);
+                l = fmaf(my_l, w, l);
+            }
+            s_f[tid] = w;
+            lds_barrier();
+            int i = tid / TPR;
+            if (i0 == 0) {
+#pragma unroll
+                for (int k = 0; k < EARLY; ++k, i += NG)
+                    if (i < parts) acc += early[k] * s_f[i];
+            }
+            const int n = min(THREADS, parts - i0);
+#pragma unroll 8
+            for (; i < n; i += NG) acc += sums(i0 + i) * s_f[i];
         }
-        const int n = min(THREADS, parts - i0);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+        if ((tid & 63) == 0) s_l[wave] = l;
+        s_o[tid] = acc;
+        __syncthreads();
+        if (tid >= TPR) continue;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < NWV; ++i) l += s_l[i];
 #pragma unroll 8
-        for (; i < n; i += NG) acc += sums(i0 + i) * s_f[i];
+        for (int i = 1; i < NG; ++i) acc += s_o[tid + i * TPR];
+        const float inv = inverse(l);
+        uint16_t* out = a.o + (R.start + (row0 + r) / a.group) * a.ldo + (head * a.group + (row0 + r) % a.group) * D + 4 * tid;
+        uint2 w;
+        w.x = pack_h2(static_cast<half_t>(acc[0] * inv), static_cast<half_t>(acc[1] * inv));
+        w.y = pack_h2(static_cast<half_t>(acc[2] * inv), static_cast<half_t>(acc[3] * inv));
+        *reinterpret_cast<uint2*>(out) = w;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    if ((tid & 63) == 0) s_l[wave] = l;
-    s_o[tid] = acc;
-    __syncthreads();
-    if (tid >= TPR) return;
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < NWV; ++i) l += s_l[i];
-#pragma unroll 8
-    for (int i = 1; i < NG; ++i) acc += s_o[tid + i * TPR];
-    const float inv = inverse(l);
-    uint16_t* out = a.o + (R.start + row / a.group) * a.ldo + (head * a.group + row % a.group) * D + 4 * tid;
-    uint2 w;
-    w.x = pack_h2(static_cast<half_t>(acc[0] * inv), static_cast<half_t>(acc[1] * inv));
-    w.y = pack_h2(static_cast<half_t>(acc[2] * inv), static_cast<half_t>(acc[3] * inv));
-    *reinterpret_cast<uint2*>(out) = w;
 }
 
 // One launch of a call: the requests with min_rows to max_rows rows, in tiles of
@@ -847,7 +856,7 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
 // Launches one part of a call: W where a workgroup has a whole sequence, S where
 // the work is shared out.
 template <class W, class S>
-int launch_part(AttendArgs a, const Part& p, int64_t line, int64_t max_rows, char* workspace, hipStream_t s) {
+int launch_part(AttendArgs a, const Part& p, int64_t blocks, int64_t max_rows, char* workspace, hipStream_t s) {
     if (!p.on) return GDSLLM_OK;
     a.min_rows = p.min_rows;
     a.max_rows = p.max_rows;
@@ -855,7 +864,7 @@ int launch_part(AttendArgs a, const Part& p, int64_t line, int64_t max_rows, cha
     a.part_o = reinterpret_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.sums * S::kD);
     a.parts = reinterpret_cast<int2*>(a.part_ml + p.sums);
-    a.groups = line < (int64_t(1) << 31) ? p.groups : 0;  // the line of blocks is counted in 32 bits
+    a.groups = p.sequences * blocks < (int64_t(1) << 30) ? p.groups : 0;  // the line of blocks is counted in 32 bits
     const unsigned per_request = static_cast<unsigned>(p.tiles) * a.c.kv_heads, requests = a.requests;
     if (a.groups == 0) {
         const size_t lds = sizeof(typename W::Lds);
@@ -877,16 +886,16 @@ int launch_part(AttendArgs a, const Part& p, int64_t line, int64_t max_rows, cha
 }
 
 template <bool E4M3, int D>
-int launch_attend(AttendArgs a, const Plan& p, int64_t line, int64_t max_rows, char* workspace, hipStream_t s) {
+int launch_attend(AttendArgs a, const Plan& p, int64_t blocks, int64_t max_rows, char* workspace, hipStream_t s) {
     const int zero_tail = a.zero_tail;
     a.zero_tail = p.few.on ? zero_tail : 0;
-    if (int rc = launch_part<RowTile<E4M3, D, 8>, RowTile<E4M3, D, 4>>(a, p.few, line, p.many.on ? kFewRows : max_rows, workspace, s))
+    if (int rc = launch_part<RowTile<E4M3, D, 8>, RowTile<E4M3, D, 4>>(a, p.few, blocks, p.many.on ? kFewRows : max_rows, workspace, s))
         return rc;
     a.zero_tail = p.few.on ? 0 : zero_tail;
     char* ws = workspace + p.few.bytes;
     if constexpr (D <= 128)
-        if (p.many.rows == 256) return launch_part<PromptTile<E4M3, D, 8>, PromptTile<E4M3, D, 4>>(a, p.many, line, max_rows, ws, s);
-    return launch_part<PromptTile<E4M3, D, 4>, PromptTile<E4M3, D, 4>>(a, p.many, line, max_rows, ws, s);
+        if (p.many.rows == 256) return launch_part<PromptTile<E4M3, D, 8>, PromptTile<E4M3, D, 4>>(a, p.many, blocks, max_rows, ws, s);
+    return launch_part<PromptTile<E4M3, D, 4>, PromptTile<E4M3, D, 4>>(a, p.many, blocks, max_rows, ws, s);
 }
 
 bool attend_sizes(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
@@ -957,16 +966,16 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.width = static_cast<int>(table_width);
     a.zero_tail = zero_tail;
     const int64_t max_rows = max_new * a.group;
-    if (max_rows / 16 * 16 * cache->kv_heads > (int64_t(1) << 30)) return bad("too many rows for one call");
-    const int64_t line = ((tokens * a.group + 15) / 16 + requests) * cache->kv_heads * (most / kBlock + 1);
+    if (tokens * q_heads > (int64_t(1) << 30)) return bad("tokens * q_heads must be at most 2^30");
+    const int64_t blocks = most / kBlock + 1;
     const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
     const hipStream_t s = as_stream(stream);
     char* ws = static_cast<char*>(workspace);
     int rc = GDSLLM_OK;
 #define GDSLLM_ATTEND(DIM)                                                          \
     if (D == DIM)                                                                   \
-        rc = e4m3 ? launch_attend<true, DIM>(a, p, line, max_rows, ws, s)           \
-                  : launch_attend<false, DIM>(a, p, line, max_rows, ws, s);
+        rc = e4m3 ? launch_attend<true, DIM>(a, p, blocks, max_rows, ws, s)           \
+                  : launch_attend<false, DIM>(a, p, blocks, max_rows, ws, s);
     GDSLLM_ATTEND(64)
     GDSLLM_ATTEND(128)
     GDSLLM_ATTEND(256)

@@ -184,3 +184,78 @@ def test_long_cache_past_32_bits(gpu):
     want, bound = sv.attention(q, vals[:1], vals[1:], s, torch.tensor([[0]]), torch.tensor([200]), torch.tensor([0, 1]),
                                dim ** -0.5)
     assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+def repeated(p, dev, lens, new, seed):
+    """The problem's blocks, in any order and again and again, as long sequences."""
+    width = max(sv.blocks(n, p.bs) for n in lens)
+    p.tables = torch.randint(0, p.codes.shape[1], (len(lens), width), generator=gen(seed)).int()
+    p.lens = torch.tensor(lens, dtype=torch.int32)
+    p.starts = torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32)
+    p.q = torch.randn(sum(new), *p.q.shape[1:], generator=gen(seed + 1)).half()
+    p.new, p.longest = max(new), max(lens)
+
+
+def check_heads(p, got, kv_heads):
+    """check() of some kv heads and their query heads."""
+    G, sel = p.q.shape[1] // p.codes.shape[2], torch.tensor(kv_heads)
+    heads = (sel[:, None] * G + torch.arange(G)).flatten()
+    s = p.scales[:, :, sel].double()
+    vals = p.codes[:, :, sel].double() * s[..., None, None]
+    want, bound = sv.attention(p.q[:, heads], vals[0], vals[1], s[1], p.tables, p.lens, p.starts, p.scale)
+    assert bool(((got[:, heads.to(got.device)].cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("max_new,max_len", [(1, 0), (0, 4000), (2, 3000), (17, 2500), (1, 16)])
+def test_bounds_smaller_than_the_requests(gpu, max_new, max_len):
+    """The host's bounds only say how the work is split: requests with more rows and tokens than they say, where
+    sequences are shared out and where not."""
+    p = Problem(gpu, "e4m3", 64, 4, 2, 32, [2500, 40, 0, 3000, 700], [7, 20, 0, 1, 33], 1200)
+    p.poison()
+    p.check(p.run(max_new=max_new, max_len=max_len))
+
+
+def test_more_requests_than_a_step_of_the_sums(gpu):
+    """More than 256 requests share one line of work."""
+    lens = [(37 * i) % 90 for i in range(299)] + [2600, 5]
+    p = Problem(gpu, "int8", 64, 2, 1, 64, lens, [min(1, n) for n in lens], 1300)
+    p.poison()
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,kv_heads,bs", [(64, 4, 2, 16), (128, 2, 2, 64), (256, 6, 2, 128)])
+def test_long_prompts_share_the_work(gpu, fmt, dim, heads, kv_heads, bs):
+    """Few sequences past 2048 tokens: every tile's keys lie in several workgroups' shares, rows that see none of
+    a share among them; requests of few rows beside them."""
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, [2300, 70, 2100, 180], [150, 2, 1, 180], 1400 + dim)
+    p.poison()
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_sequences_take_the_widest_tiles(gpu, fmt, dim):
+    """512 and more (request, kv head, 256 rows): the last rows of a tile ragged, a request with few rows."""
+    p = Problem(gpu, fmt, dim, 512, 128, 16, [130, 65, 7], [100, 65, 2], 1500 + dim)
+    p.poison()
+    check_heads(p, p.run(), [0, 77, 127])
+
+
+def test_whole_sequences_past_a_segment(gpu):
+    """Many sequences, so that each has a workgroup of its own, longer than the block table it holds at once."""
+    p = Problem(gpu, "int8", 256, 1024, 1024, 64, [100, 3], [1, 1], 1600)
+    repeated(p, gpu, [8300, 3], [1, 1], 1601)
+    check_heads(p, p.run(), [0, 500, 1023])
+    p = Problem(gpu, "e4m3", 64, 256, 256, 16, [60], [2], 1602)
+    repeated(p, gpu, [4200], [40], 1603)
+    check_heads(p, p.run(), [0, 255])
+
+
+def test_a_sequence_in_more_parts_than_threads_that_join(gpu):
+    """One long sequence among short ones, in about 470 parts; 256 threads add a row's."""
+    lens = [120000] + list(range(1, 32))
+    p = Problem(gpu, "e4m3", 64, 16, 1, 256, [1000] * 32, [1] * 32, 1700)
+    repeated(p, gpu, lens, [1] * 32, 1701)
+    p.q *= 0.5
+    check_heads(p, p.run(), [0])
