@@ -550,6 +550,7 @@ extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, in
     if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) % 4 ||
         (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
         return bad("misaligned pointer (cos and sin: 16 bytes)");
+    if (q && q == q_out) return bad("q_out must not be q");
     a.k = static_cast<const uint16_t*>(k);
     a.v = static_cast<const uint16_t*>(v);
     a.q = static_cast<const uint16_t*>(q);
@@ -578,7 +579,7 @@ extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, in
     const int64_t q_tokens = q ? std::min<int64_t>(tokens, 16 * static_cast<int64_t>(cu_count())) : 0;
     const bool apart = q_tokens > 256 && waves == 16;
     const int64_t q_groups = apart ? 0 : q_tokens;
-    if (units + q_groups > (int64_t(1) << 31) - 1) return bad("too many tokens and heads for one call");
+    if ((units + q_groups) * 64 * waves >= (int64_t(1) << 32)) return bad("too many tokens and heads for one call");
     const dim3 grid(static_cast<unsigned>(units + q_groups));
     const bool e4m3 = cache->format == GDSLLM_KV_E4M3;
     const hipStream_t s = as_stream(stream);

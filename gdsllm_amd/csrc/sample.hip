@@ -790,7 +790,7 @@ extern "C" int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, 
     const std::string n = "sample_tokens";
     auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
     if (bits != 16 && bits != 32) return bad("logits must be fp16 or fp32 (bits 16 or 32)");
-    if (rows < 0 || rows > (int64_t(1) << 24)) return bad("bad row count");
+    if (rows < 0 || rows >= (int64_t(1) << 32) / kThreads) return bad("rows must be in [0, 4194303]");
     if (vocab < 1 || vocab > kMaxVocab) return bad("vocab must be in [1, 1048576], got " + std::to_string(vocab));
     if (rows == 0) return ok();
     if (ld < vocab) return bad("ld < vocab");

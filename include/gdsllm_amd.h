@@ -464,8 +464,8 @@ int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests
 
 /* Writes keys and values k, v fp16 [tokens][kv_heads * head_dim] (rows ldk, ldv
  * apart) to their slots.  With rotary > 0 (a multiple of 16, at most head_dim)
- * keys, and q [tokens][q_heads * head_dim] into q_out (rows contiguous; q may be
- * null), are rotated first: channels i and i + rotary/2 of a head turn by the
+ * keys, and q [tokens][q_heads * head_dim] into q_out (rows contiguous, apart from
+ * q; q may be null), are rotated first: channels i and i + rotary/2 of a head turn by the
  * angle whose cosine and sine are cos, sin [max_pos][rotary/2] at positions[t];
  * the rotated values are rounded once, to fp16.
  * The tokens of one block stand in consecutive rows (as kv_assign numbers
@@ -475,7 +475,8 @@ int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests
  * power of two s >= 2^-32 with |x| <= top * s (top 448 or 127) for its new
  * finite values, or the scale it had, if o > 0 and that is larger; older codes
  * are rescaled to a scale that grew.  Codes are x / s to nearest even,
- * saturated; NaN stays NaN in e4m3 and is 0 in int8.  A row whose slot lies
+ * saturated; NaN stays NaN in e4m3 and is 0 in int8.  (A scale that it had is
+ * taken to be a power of two, as this call leaves them.)  A row whose slot lies
  * outside the cache (-1) or whose position outside [0, max_pos) is padding:
  * not written, zeros in q_out.  Of several rows with one slot the last counts. */
 int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
@@ -489,10 +490,15 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * that sees none is zero.  Query head h reads kv head h / (q_heads / kv_heads).
  * Products of fp16 and code values in fp32, softmax in fp32, weights rounded
  * to fp16 before the product with the values.  scale and the cache's scales must
- * be positive; blocks outside the cache have no weight.
+ * be positive; blocks outside the cache have no weight.  What the cache holds
+ * behind a request's tokens is not read as a number.  A NaN among its values (e4m3
+ * only) also reaches rows of its request that stand before it in the same call.
+ * tokens * q_heads <= 2^30.
  * max_new and max_len: bounds on a request's rows and tokens, known to the host
  * (0: tokens, and table_width * block_size).  They set how the work is split;
- * larger requests than they say are computed all the same, more slowly.
+ * larger requests than they say are computed all the same, more slowly.  The
+ * workspace's size is asked for with the same bounds (tokens or table_width *
+ * block_size where one is 0).
  * Rows behind the last request are left as they were, or set to zero with
  * zero_tail.  workspace_bytes >= gdsllm_kv_attention_workspace_size(...).    */
 size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
@@ -505,7 +511,7 @@ int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ld
 
 /* -------------------------------------------------------------- sampling --
  * One token for each row of logits [rows][vocab] (fp16 or fp32: bits 16 or 32;
- * rows ld apart; vocab <= 2^20) from the uniform number u[row] in [0, 1).
+ * rows ld apart; vocab <= 2^20, rows < 2^22) from the uniform number u[row] in [0, 1).
  * Tokens are taken in falling order of their logits, equal ones by rising index,
  * with weights exp((l - max) / temperature).  Kept: the first top_k (<= 0: all);
  * of those, the tokens before which less than top_p of their mass lies; of

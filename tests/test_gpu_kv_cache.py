@@ -268,3 +268,30 @@ def test_append_offsets_past_32_bits(gpu):
     for c, s in zip(codes, scale):
         assert torch.equal(c[[0, -1]].cpu().double(), ref_c) and torch.equal(s[[0, -1]].cpu().double(), ref_s)
         assert not bool(c[1:-1].any())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,rotary", [(64, 5, 64), (256, 2, 128)])
+@pytest.mark.parametrize("spans", ["prompts", "long"])
+def test_append_largest_blocks(gpu, fmt, dim, heads, rotary, spans):
+    """Blocks of 256 tokens, pages longer than their threads hold; a second call that grows the scales."""
+    bs = 256
+    blocks = sum(sv.blocks(b, bs) for _, b in SPANS[spans]) + 2
+    kc, vc = (Cache(fmt, blocks, heads, bs, dim, gpu, s) for s in (61, 62))
+    slots, pos = _requests(SPANS[spans], bs, blocks, gen(63))
+    q, k, v = (torch.randn(slots.numel(), h, dim, generator=gen(64 + i)).half() for i, h in enumerate((3 * heads, heads, heads)))
+    cos, sin = _rope(int(pos.max()) + 1, rotary // 2)
+    _append(kc, vc, k, v, slots, q, pos, cos, sin)
+    _append(kc, vc, k * 300, v * 5, slots, q, pos, cos, sin)
+
+
+@pytest.mark.parametrize("bs", [16, 128])
+def test_append_large_decode_batch(gpu, bs):
+    """More tokens than a workgroup to each would leave room for, every one in a block of its own."""
+    n, heads, dim = 700, 2, 128
+    kc, vc = (Cache("e4m3", n + 3, heads, bs, dim, gpu, s) for s in (71, 72))
+    slots = torch.randperm(n + 3, generator=gen(73))[:n].int() * bs + torch.randint(0, bs, (n,), generator=gen(74)).int()
+    slots[::41] = -1
+    q, k, v = (torch.randn(n, h, dim, generator=gen(75 + h)).half() for h in (8, heads, heads))
+    cos, sin = _rope(90, 64)
+    _append(kc, vc, k, v, slots, q, torch.randint(0, 90, (n,), generator=gen(78)).int(), cos, sin)

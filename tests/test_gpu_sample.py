@@ -122,3 +122,15 @@ def test_frequencies(gpu):
     share = torch.bincount(got.cpu(), minlength=vocab).double()
     want = torch.softmax(x.double(), 0) * n
     assert bool(((share - want).abs() <= 1.0 + 1e-3).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [32752, 32753, 40000, 128257, 200003, 2 ** 20])
+def test_large_vocabularies(gpu, dtype, vocab):
+    """Rows in registers and not, and fp32 rows of which a 4096th of the keys' range holds more than the list."""
+    x = torch.randn(4, vocab, generator=gen(vocab))
+    x[1] = 1.0 + 1e-4 * x[1]
+    x[2] *= 0.05
+    u = [0.5, 0.123, 0.999, 0.25]
+    _check(gpu, x.to(dtype), u)
+    _check(gpu, x.to(dtype), u, [0.8, 1.0, 0.3, 0.0], [0, 20000, 5, 0], [0.95, 0.9, 1.0, 1.0], [0.0, 0.0, 0.01, 0.5])

@@ -126,6 +126,23 @@ def test_sample_refusals():
     assert call(l=9) == BAD and call(l=10, bits=32) == BAD and call(out=12) == BAD and call(t=6) == BAD and "misaligned" in _err()
 
 
+def test_calls_too_large_for_one_launch():
+    """Grids count threads in 32 bits and rows in 31."""
+    lib = capi()
+    assert lib.gdsllm_sample_tokens(8, 16, 2 ** 22, 10, 10, 8, None, None, None, None, 8, None) == BAD and "rows" in _err()
+    wide = _cache(kv_heads=1024, num_blocks=4)
+    assert lib.gdsllm_kv_append(wide, 16, 2 ** 16, 16, 2 ** 16, 16, 2 ** 30, None, 0, None, 0, None, None, None, 0, 0, None) == BAD
+    assert "too many" in _err()
+    n = 2 ** 30
+    assert lib.gdsllm_kv_attention(_cache(), 16, 256, 16, 256, n, 4, 16, 1, 1, 16, 16, 1, 1.0, 1, 16, 0, None, 0, None) == BAD
+    assert "2^30" in _err()
+
+
+def test_q_out_apart_from_q():
+    rope = (16, 16, 16, 32, 9, None)
+    assert capi().gdsllm_kv_append(_cache(), 16, 128, 16, 128, 16, 1, 32, 128, 32, 2, *rope) == BAD and "q_out" in _err()
+
+
 def test_extension_refuses_host_tensors():
     """The torch entry points name the argument that is not where or what it has to be."""
     e = ext()
