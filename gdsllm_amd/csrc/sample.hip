@@ -450,7 +450,7 @@ struct Lds16 {
     double mass[64], wave_mass[kWaves];
     Place place;
     int count[64], wave_count[kWaves];
-    int top, outside, answer, listed, hit, last;
+    int top, outside, answer, listed;
 };
 
 // Element k (in falling order) of unit u, as fp16 bits.
@@ -639,58 +639,49 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
                 u = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
             }
             const uint32_t h = unit_bits(u, tid);
-            const int c = u == 0 && tid > 0 ? 0 : counter(h);
+            int c = u == 0 && tid > 0 ? 0 : counter(h);
             double w = 0.0;
             if (__any(c > 0)) w = c ? weight(h) : 0.0;
+            if (kind == Weight && w < m) c = 0;  // the heavy ones of this unit: their sums are the answer
             int cu = wave_scan(c);
             double wu = wave_scan(w * c);
-            __syncthreads();  // the last place has been read
             if (lane == 63) {
                 s.wave_count[wave] = cu;
                 s.wave_mass[wave] = wu;
             }
-            if (tid == 0) {
-                s.hit = kind == Weight ? -1 : kThreads;
-                s.last = -1;
-            }
             __syncthreads();
-            cu += __builtin_amdgcn_readlane(upto_n - unit_n, u);
-            wu += lane_double(upto_w - unit_w, u);
-#pragma unroll
-            for (int v = 0; v < kWaves - 1; ++v) {
-                cu += v < wave ? s.wave_count[v] : 0;
-                wu += v < wave ? s.wave_mass[v] : 0.0;
-            }
-            // lanes of a wave stand in order: one atomic a wave
-            const uint64_t has = __ballot(c > 0);
-            const uint64_t good = __ballot(c > 0 && (kind == Weight ? w >= m : at_border(cu, wu)));
-            if (lane == 0) {
-                if (has) atomicMax(&s.last, 64 * wave + 63 - __builtin_clzll(has));
-                if (good && kind == Weight) atomicMax(&s.hit, 64 * wave + 63 - __builtin_clzll(good));
-                if (good && kind != Weight) atomicMin(&s.hit, 64 * wave + __builtin_ctzll(good));
-            }
-            __syncthreads();
-            const int hit = s.hit;
-            const bool none_hits = hit < 0 || hit == kThreads;
-            if (kind == Weight && none_hits) {  // the place before this unit
-                if (tid == 0) s.place = {0, 0, __builtin_amdgcn_readlane(upto_n - unit_n, u), 0.0, 0.0};
-            } else if (tid == (none_hits ? s.last : hit)) {
-                Place p{h, 0, cu - c, wu - w * c, w};
-                if (kind == Count) p.in_bin = n - p.count;
-                else if (kind == Weight) p.in_bin = c;
-                else if (c == 1 || none_hits) p.in_bin = kind == Pass ? c - 1 : c;  // none: rounding hid it, the last token
-                else {
-                    const double q = (m - p.mass) / p.w;
-                    p.in_bin = kind == Pass ? static_cast<int>(fmin(fmax(floor(q), 0.0), c - 1.0))
-                                            : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(c)));
+            // the waves' sums, a wave to each of 16 lanes, in every wave
+            const int own_n = lane < kWaves ? s.wave_count[lane] : 0;
+            const double own_w = lane < kWaves ? s.wave_mass[lane] : 0.0;
+            const int waves_n = wave_scan(own_n) + __builtin_amdgcn_readlane(upto_n - unit_n, u);
+            const double waves_w = wave_scan(own_w) + lane_double(upto_w - unit_w, u);
+            // the one that holds the place (rounding may hide it: then the last with any)
+            const uint64_t has = __ballot(own_n > 0), good = __ballot(own_n > 0 && at_border(waves_n, waves_w));
+            const int holder = good ? __builtin_ctzll(good) : has ? 63 - __builtin_clzll(has) : 0;
+            if (kind == Weight) {
+                if (tid == 0) s.place = {0, 0, last_lane(waves_n), lane_double(waves_w, 63), 0.0};
+            } else if (wave == holder) {
+                cu += __builtin_amdgcn_readlane(waves_n - own_n, holder);
+                wu += lane_double(waves_w - own_w, holder);
+                const uint64_t in = __ballot(c > 0 && at_border(cu, wu));
+                const int l = in ? __builtin_ctzll(in) : 63 - __builtin_clzll(__ballot(c > 0));
+                if (lane == l) {
+                    Place p{h, 0, cu - c, wu - w * c, w};
+                    if (kind == Count) p.in_bin = n - p.count;
+                    else if (c == 1 || !in) p.in_bin = kind == Pass ? c - 1 : c;  // hidden: the last token
+                    else {
+                        const double q = (m - p.mass) / p.w;
+                        p.in_bin = kind == Pass ? static_cast<int>(fmin(fmax(floor(q), 0.0), c - 1.0))
+                                                : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(c)));
+                    }
+                    s.place = p;
                 }
-                s.place = p;
             }
             __syncthreads();
             return s.place;
         };
         Place at{top_bits, 0, 0, 0.0, 1.0};
-        int n = total, cut = total;
+        int cut = total, weighed = total;  // kept tokens; those whose mass `mass` is
         double mass = lane_double(upto_w, 63);
 #pragma nounroll
         for (int stage = 0; stage < 6; ++stage) {
@@ -698,8 +689,8 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
             int number = 0;
             double amount = 0.0;
             if (stage == 0) {  // the first top_k and their mass
-                if (P.top_k <= 0 || P.top_k >= n) continue;
-                number = n = cut = P.top_k;
+                if (P.top_k <= 0 || P.top_k >= cut) continue;
+                number = P.top_k;
             } else if (stage == 1) {  // of those, top_p of their mass
                 if (P.top_p >= 1.0) continue;
                 kind = Reach;
@@ -708,8 +699,8 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
                 if (P.min_p <= 0.0) continue;
                 kind = Weight;
                 amount = P.min_p;
-            } else if (stage == 3) {  // the mass of the kept
-                if (cut == n) continue;
+            } else if (stage == 3) {  // the mass of the kept, where no stage found it
+                if (cut == weighed) continue;
                 number = cut;
             } else if (stage == 4) {  // the draw
                 kind = Pass;
@@ -719,10 +710,13 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
                 number = cut;
             }
             const Place p = find(kind, number, amount);
-            if (stage == 1 || stage == 2) {
-                cut = min(cut, max(p.count + p.in_bin, 1));
-            } else if (stage < 4) {
-                mass = p.mass + p.in_bin * p.w;
+            if (stage < 4) {
+                const int upto = p.count + p.in_bin;
+                if (upto <= cut) {
+                    weighed = upto;
+                    mass = p.mass + p.in_bin * p.w;
+                }
+                cut = max(min(cut, upto), 1);
             } else {
                 at = p;
                 at.in_bin -= stage == 5 ? 1 : 0;
