@@ -83,6 +83,8 @@ struct RowParams {
     }
 };
 
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+
 // Lane l gets lane 63 - l's value.
 __device__ __forceinline__ double lane_mirror(double v) { return __shfl_xor(v, 63); }
 
@@ -543,12 +545,14 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
             return static_cast<double>(h2f(low + 1) - h2f(low));
         };
         // Counts and masses of the units, a wave to the two units of an exponent.  The
-        // 1024 values of a binade are evenly spaced, so a weight is the one at the
-        // start of its 64 values (lanes 0-15: of the positive ones, 16-31: of the
-        // negative ones) times one of 64 that all of these share.
+        // 1024 values of a binade are evenly spaced, so neighbouring blocks of 64
+        // differ by one factor: a lane adds its value of each block by Horner's rule,
+        // from the lightest block up, and what is left is the heaviest block's weight
+        // times one of 64 that all blocks share.  The largest logit's own block, above
+        // which some values lie, is weighed value by value.
         for (int e = wave; e < 32; e += kWaves) {
             const uint32_t first = static_cast<uint32_t>(e) << 10;  // smallest magnitude
-            int n_pos = 0, n_neg = 0;
+            uint32_t n_pos = 0, n_neg = 0;
             double w_pos = 0.0, w_neg = 0.0;
             uint32_t c[16];
 #pragma unroll
@@ -567,42 +571,52 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    n_pos += c[j] & 0xFFFFu;
-                    n_neg += c[j] >> 16;
+                    const ushort2_t two = __builtin_bit_cast(ushort2_t, c[j]);
+                    n_pos = __builtin_amdgcn_udot2(two, ushort2_t{1, 0}, n_pos, false);
+                    n_neg = __builtin_amdgcn_udot2(two, ushort2_t{0, 1}, n_neg, false);
                 }
                 if (__any(n_pos + n_neg > 0)) {
-                    const double up = exp2_neg(-step_of(first) * P.c * (63 - lane)), down = lane_mirror(up);
-                    // largest of the 64 values
-                    const float base = lane < 16 ? h2f(first + 64 * lane + 63) : h2f(0x8000u | (first + 64 * (lane & 15)));
-                    const double start = top == INFINITY ? 0.0 : exp2_neg(fmin((static_cast<double>(base) - top) * P.c, 0.0));
+                    // blocks behind the heaviest of each sign; the largest logit's own is not among them
+                    const int own = e == static_cast<int>((top_bits & 0x7FFFu) >> 10) ? static_cast<int>(top_bits >> 6 & 15) : -1;
+                    const bool own_pos = own >= 0 && !(top_bits & 0x8000u), own_neg = own >= 0 && !own_pos;
+                    const int jp = own_pos ? own - 1 : 15, jn = own_neg ? own + 1 : 0;
+                    const double d = step_of(first) * P.c, up = exp2_neg(-d * (63 - lane)), down = lane_mirror(up);
+                    const float heaviest = h2f(lane == 1 ? first + 64 * max(jp, 0) + 63 : 0x8000u | (first + 64 * min(jn, 15)));
+                    const double y = lane == 0 ? -64.0 * d : fmin((static_cast<double>(heaviest) - top) * P.c, 0.0);
+                    const double f = exp2_neg(lane > 0 && top == INFINITY ? -INFINITY : y);
+                    const double r = lane_double(f, 0);
+                    if (own < 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        // the largest logit's own 64 values, some of them above it, come below
-                        const uint32_t own = first + 64 * j;
-                        const uint32_t cp = own >> 6 == top_bits >> 6 ? 0 : c[j] & 0xFFFFu;
-                        const uint32_t cn = (0x8000u | own) >> 6 == top_bits >> 6 ? 0 : c[j] >> 16;
-                        w_pos = fma(lane_double(start, j), static_cast<double>(cp), w_pos);
-                        w_neg = fma(lane_double(start, 16 + j), static_cast<double>(cn), w_neg);
+                        for (int j = 0; j < 16; ++j) {
+                            w_pos = fma(w_pos, r, static_cast<double>(c[j] & 0xFFFFu));
+                            w_neg = fma(w_neg, r, static_cast<double>(c[15 - j] >> 16));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int k = 15 - j;
+                            w_pos = j <= jp ? fma(w_pos, r, static_cast<double>(c[j] & 0xFFFFu)) : w_pos;
+                            w_neg = k >= jn ? fma(w_neg, r, static_cast<double>(c[k] >> 16)) : w_neg;
+                        }
                     }
-                    w_pos *= up;
-                    w_neg *= down;
-                    if (first >> 10 == (top_bits & 0x7FFFu) >> 10) {
+                    w_pos *= up * lane_double(f, 1);
+                    w_neg *= down * lane_double(f, 2);
+                    if (own >= 0) {
                         const uint32_t h = (top_bits & ~63u) + lane;
-                        const int own = counter(h);
-                        const double w = own ? weight(h) * own : 0.0;
-                        w_pos += (h & 0x8000u) ? 0.0 : w;
-                        w_neg += (h & 0x8000u) ? w : 0.0;
+                        const int n = counter(h);
+                        const double w = n ? weight(h) * n : 0.0;
+                        w_pos += own_pos ? w : 0.0;
+                        w_neg += own_pos ? 0.0 : w;
                     }
                 }
             }
-            n_pos = wave_sum(n_pos);
-            n_neg = wave_sum(n_neg);
+            const int all_pos = wave_sum(static_cast<int>(n_pos)), all_neg = wave_sum(static_cast<int>(n_neg));
             w_pos = wave_scan(w_pos);
             w_neg = wave_scan(w_neg);
             if (lane == 63) {
-                s.count[31 - e] = n_pos;
+                s.count[31 - e] = all_pos;
                 s.mass[31 - e] = w_pos;
-                s.count[32 + e] = n_neg;  // [63]: always 0
+                s.count[32 + e] = all_neg;  // [63]: always 0
                 s.mass[32 + e] = w_neg;
             }
         }
