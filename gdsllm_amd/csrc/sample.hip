@@ -470,7 +470,6 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
     Lds16& s = *reinterpret_cast<Lds16*>(raw);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
     const RowReader<uint16_t, 8> rd(static_cast<const uint16_t*>(a.logits) + row * a.ld, a.vocab);
-    const RowParams P(a, row);
     constexpr uint32_t none = 0xFFFFu;  // a NaN
     const int grans = rd.granules();
 
@@ -484,6 +483,7 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
         s.listed = 0;
         s.answer = -1;
     }
+    const RowParams P(a, row);
     __syncthreads();
 
     // -0 becomes +0 by adding +0: equal logits stand together
@@ -522,9 +522,7 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
         // the largest logit, as an order-keeping whole number (1024: -inf, so no token)
         const uint32_t x = __builtin_bit_cast(uint32_t, most);
         auto key = [](uint32_t h) { return static_cast<int>((h & 0x8000u) ? 0xFFFFu - h : 0x8000u | h); };
-        int k = max(key(x & 0xFFFFu), key(x >> 16));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) k = max(k, __shfl_xor(k, o));
+        const int k = wave_max(max(key(x & 0xFFFFu), key(x >> 16)));
         if (lane == 0) atomicMax(&s.top, k);
     }
     __syncthreads();

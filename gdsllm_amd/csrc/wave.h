@@ -39,5 +39,15 @@ __device__ __forceinline__ double lane_double(double v, int l) {
     return __builtin_bit_cast(double, (hi << 32) | lo);
 }
 __device__ __forceinline__ int wave_sum(int v) { return last_lane(wave_scan(v)); }
+// The largest of the wave's values, none of them negative, in every lane.
+__device__ __forceinline__ int wave_max(int v) {
+    v = max(v, dpp_shift<0x111, 0xF>(v));
+    v = max(v, dpp_shift<0x112, 0xF>(v));
+    v = max(v, dpp_shift<0x114, 0xF>(v));
+    v = max(v, dpp_shift<0x118, 0xF>(v));
+    v = max(v, dpp_shift<0x142, 0xA>(v));
+    v = max(v, dpp_shift<0x143, 0xC>(v));
+    return last_lane(v);
+}
 
 }  // namespace gdsllm
