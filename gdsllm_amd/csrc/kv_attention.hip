@@ -4,17 +4,31 @@
 // query head h of kv head h / G:
 //   x_j = scale * k_scale * (q . code_j),  j <= len_b - n_b + t
 //   o   = sum_j 2^(x_j log2 e) v_j / sum_j 2^(x_j log2 e)
-// in one pass over the tokens with a running maximum.  Codes enter the matrix
+// in one pass over the tokens with a running reference m.  Codes enter the matrix
 // cores as the fp16 values they are, so the products q . code and P . code are
 // exact and summed in fp32; the scales stay outside: a block's key scale
 // multiplies its scores, and its value scale is carried in the exponent.  With
-// e = log2(v_scale) and the running maximum m taken over y_j = x_j log2 e + e,
+// e = log2(v_scale) and m within 2^8 of the largest y_j = x_j log2 e + e so far,
 //   acc += 2^(y_j - m) * code_j,   l += 2^(y_j - m) / v_scale,   o = acc / l,
-// so the fp16 weights 2^(y_j - m) <= 1 lose nothing to a block whose values are
-// large or small, whatever the other blocks' scales are.
+// so the fp16 weights 2^(y_j - m) <= 2^8 (half a step of fp16 each: the one
+// rounding before the last) lose nothing to a block whose values are large or
+// small, whatever the other blocks' scales are.
 //
 // The G query heads of a kv head and the query rows share its keys: they are
-// the 16 columns of one matrix tile (row r = token r / G, head r % G).
+// the columns of a matrix tile (row r = token r / G, head r % G), 16 of them for
+// requests of up to 32 rows (RowTile), 128 or 256 for prompts (PromptTile).
+//  * Decode reads each code once and is bound by that: 32 requests of 8192 tokens
+//    over 8 heads 273 MB in 59 us, 4.6 TB/s, 53 us of it attend_shared (a large
+//    copy reaches 4.75); one of 131072 tokens over 2 heads of 256 134 MB in 37 us,
+//    30 of them attend_shared.  A short sequence (777 tokens, 32 heads, 9.6 us) is
+//    one chain of memory latencies: a launch, its length and table, its scales,
+//    then three tiles of codes to a wave.
+//  * Prompts are bound by vector work beside the matrix cores (softmax and the
+//    codes' conversion, about half the cycles; the matrix cores a third): 4096
+//    tokens of 32 heads 174 us, 790 TFLOP/s of a large product's 1028; 4 chunks of
+//    300 tokens with up to 5000 held 162 us, 510 TFLOP/s: 448 tiles of unequal
+//    length are 1.75 to a compute unit.  Even shares of their keys cost more than they
+//    give (156 us, and 92 to join 57000 rows); 16 such chunks reach 680.
 
 #include <algorithm>
 #include <climits>
@@ -809,9 +823,15 @@ struct Plan {
 };
 
 constexpr int kCus = 256;  // compute units of the device: the workspace's size goes by it
-// Requests with more rows than this take 128-row tiles, the others 16-row ones.
+// Requests of up to kFewRows rows take 16-row tiles, the others 128-row ones, and
+// all take 16-row ones, in one launch, where none has more than twice as many (32
+// requests of up to 4096 tokens over 8 heads: 8 to 32 rows each 21 us in 16-row
+// tiles, 44 with those past 16 in 128-row ones; 16 to 64 rows 37 us in 16-row tiles,
+// 49 split at 32; 40 to 128 rows 54 split at 64, 39 in 128-row ones).
 constexpr int kFewRows = 32;
-constexpr int64_t kWholeTokens = 2048;
+// A sequence of up to this many tokens is one workgroup's (4 requests over 8 heads,
+// up to 1024 tokens: 4.3 us whole, 5.7 shared out; up to 2048: 6.8 against 5.8).
+constexpr int64_t kWholeTokens = 1024;
 
 void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int64_t max_len,
                  int64_t resident, bool whole) {
@@ -825,18 +845,19 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
 }
 
 // One workgroup to a sequence where none is long or there are many of them, else
-// as many workgroups as the device holds at once, with even shares.
+// as many workgroups as the device holds at once, with even shares.  (256 requests
+// of up to 4000 tokens over 8 heads: 73 us whole, 79 shared out.)
 Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
     Plan p;
     const int64_t rows = max_new * (q_heads / kv_heads);
-    const bool many = rows > kFewRows;
+    const bool many = rows > 2 * kFewRows;
     if (!many || requests > 1) {
         p.few.rows = 16;
         if (many) p.few.max_rows = kFewRows;
         const int64_t most = many ? kFewRows : rows, resident = per_cu(head_dim) * static_cast<int64_t>(kCus);
         const int64_t sequences = requests * kv_heads * ((most + 15) / 16);
         finish_part(&p.few, requests, kv_heads, head_dim, most, max_len, resident,
-                    max_len <= kWholeTokens || sequences >= 8 * resident);
+                    max_len <= kWholeTokens || sequences >= (max_len <= 4 * kWholeTokens ? 2 : 8) * resident);
     }
     if (many) {
         const int64_t resident = (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus);
@@ -848,7 +869,7 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
         if (p.few.on) p.many.min_rows = kFewRows + 1;
         const int64_t sequences = requests * kv_heads * ((rows + 127) / 128);
         finish_part(&p.many, requests, kv_heads, head_dim, rows, max_len, resident,
-                    wide || max_len <= kWholeTokens || 2 * sequences >= resident);
+                    wide || max_len <= (4 * sequences >= resident ? 2 : 1) * kWholeTokens || 2 * sequences >= resident);
     }
     return p;
 }
