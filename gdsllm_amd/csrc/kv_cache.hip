@@ -64,7 +64,9 @@ struct AssignArgs {
 
 // Every workgroup takes the sums over all requests for itself (at most 8192 of
 // them: cheaper than a second launch or a grid barrier) and then writes its share
-// of the tables and of the token rows.
+// of the tables and of the token rows.  All of it is latency (a launch takes 1.65 us):
+// lengths, one scan of tokens, new and returned blocks, a ring entry, a store.  64
+// decoding requests 4.9 us, 2048 mixed ones with 66000 token rows 7.6 us.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
     extern __shared__ int32_t lds[];
@@ -149,7 +151,8 @@ __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
 
     // New and returned blocks: the requests spread over the waves, one to a lane,
     // which copies its blocks itself where they are few (a decoding step), else the
-    // whole wave does (a prompt's, an ended request's).
+    // whole wave does (a prompt's, an ended request's).  A request to a wave took 6.7
+    // us instead of 4.9 for 64 of them, 64 of 2048 to a wave 10.7 instead of 7.6.
     constexpr int kOwn = 4;
     const int waves = static_cast<int>(gridDim.x) * WAVES, share = min((a.n + waves - 1) / waves, 64);
     for (int base = (static_cast<int>(blockIdx.x) * WAVES + wave) * share; base < a.n; base += waves * share) {
@@ -382,7 +385,11 @@ __device__ void append_run(const Run& r, int tid, float* red) {
 // head in `rows_per_group` (at most 62) token rows.  A page's tokens stand in
 // consecutive rows; the workgroup takes every page whose first row lies in its
 // rows, to that page's last row wherever it is, so one workgroup alone writes a
-// page.  Pages with few new rows go to one wave each, others to all four.
+// page.  Pages with few new rows go to one wave each, others to all of them.
+// Bound by the bytes of k, v, q and the codes for prompts (2 x 1000 tokens of 32 heads
+// 66 MB in 21 us, 3.1 TB/s; 8192 tokens with 32 query heads of 256 296 MB in 88 us,
+// 3.4), by latency for a decode step (32 tokens 4.5 us: slot, row and scale, a maximum,
+// a store).
 template <bool E4M3, int D, int WAVES>
 __device__ void append_pages(const AppendArgs& a, int unit) {
     __shared__ float red[WAVES];
