@@ -581,10 +581,11 @@ extern "C" int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, in
     a.rows_per_group = static_cast<int>(std::min<int64_t>(std::max<int64_t>(share, 1), std::min<int64_t>(cache->block_size, 62)));
     a.groups = static_cast<int>((tokens + a.rows_per_group - 1) / a.rows_per_group);
     const int64_t units = (static_cast<int64_t>(a.groups) * cache->kv_heads * 2 + 7) / 8 * 8;
-    // q rides along, but not in workgroups of 1024 threads, which turn a token at a
-    // time too slowly (8192 tokens of 32 heads of 256: 93 us against 54)
+    // q rides along, but not that of long prompts in workgroups of 1024 threads, which
+    // turn a token at a time (32 heads of 256: 400 tokens 14 us riding along, 18 in a
+    // launch of its own; 1600 tokens 24 and 27; 3200 tokens 41 and 35)
     const int64_t q_tokens = q ? std::min<int64_t>(tokens, 16 * static_cast<int64_t>(cu_count())) : 0;
-    const bool apart = q_tokens > 256 && waves == 16;
+    const bool apart = q_tokens > 2048 && waves == 16;
     const int64_t q_groups = apart ? 0 : q_tokens;
     if ((units + q_groups) * 64 * waves >= (int64_t(1) << 32)) return bad("too many tokens and heads for one call");
     const dim3 grid(static_cast<unsigned>(units + q_groups));
