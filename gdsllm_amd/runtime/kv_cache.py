@@ -26,7 +26,7 @@ HEAD_DIMS = (64, 128, 256)
 
 class KVCache8:
     """The 8-bit KV cache of `layers` layers and up to `requests` requests of at
-    most max_len tokens each.
+    most max_len tokens each (rounded up to whole blocks).
 
     num_blocks: blocks of block_size tokens in the pool all requests share
     (None: as many as hold every request at max_len); a request that needs a
@@ -48,7 +48,7 @@ class KVCache8:
         num_blocks = requests * width if num_blocks is None else num_blocks
         if not 1 <= num_blocks <= (2 ** 31 - 1) // block_size:
             raise ValueError("KVCache8: num_blocks must be positive and num_blocks * block_size below 2^31")
-        self.layers, self.requests, self.max_len = layers, requests, max_len
+        self.layers, self.requests, self.max_len = layers, requests, width * block_size
         self.kv_heads, self.head_dim, self.block_size, self.num_blocks = kv_heads, head_dim, block_size, num_blocks
         shape = (num_blocks, kv_heads, block_size, head_dim)
         # blocks are read only behind tokens that were written: no codes need a value
@@ -111,6 +111,9 @@ class KVCache8:
         head_dim] turned the same way."""
         if self.slots is None:
             raise RuntimeError("KVCache8.append: begin_step comes first")
+        if cos is not None and cos.shape[0] < self.max_len:
+            # a token past the table would not be written, and read later all the same
+            raise ValueError(f"KVCache8.append: cos and sin must reach position {self.max_len - 1}")
         return ext().kv_append(k, v, self.slots, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
                                q, self.positions if cos is not None else None, cos, sin)
 

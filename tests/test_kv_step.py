@@ -136,6 +136,17 @@ def test_order_and_arguments(ops):
     assert llama.cached_attention(torch.zeros(0, 64).half(), {}, c, 0, None, None).shape == (0, 64)
 
 
+def test_the_rotation_reaches_every_position(ops):
+    """max_len counts whole blocks, and a table that ends before it is refused."""
+    c = cache(max_len=50)
+    assert c.max_len == 64 and c.block_tables.shape == (3, 4)
+    c.begin_step(i32(1, 0, 0), 1)
+    x = torch.zeros(1, 2, 64).half()
+    with pytest.raises(ValueError, match="position 63"):
+        c.append(0, x, x, x, *kv_cache.rope_table(50, 64, device="cpu"))
+    c.append(0, x, x, x, *kv_cache.rope_table(64, 64, device="cpu"))
+
+
 def test_rope_table():
     cos, sin = kv_cache.rope_table(100001, 64, theta=500000.0, device="cpu")
     for p, i in ((0, 0), (1, 0), (100000, 0), (100000, 31), (777, 5)):
