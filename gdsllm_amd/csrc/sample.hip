@@ -246,6 +246,7 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
         s.sum = 0;
     }
     for (int i = tid; i < kLevel1; i += kThreads) s.count1[i] = 0, s.mass1[i] = 0;
+    for (int i = tid; i < kLevel2; i += kThreads) s.count2[i] = 0, s.mass2[i] = 0;
     __syncthreads();
     uint32_t first = 0xFFFFFFFFu;
     int counted = 0;
@@ -298,12 +299,11 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
                 each([&](uint32_t r) {
                     if (static_cast<int>(r >> 20) == bin) s.list[atomicAdd(&s.length, 1)] = r;
                 });
+            __syncthreads();
         };
-        // Counts the tokens whose rank above bit low + 10 is `prefix` by the ten bits from `low` on.
+        // Counts the tokens whose rank above bit low + 10 is `prefix` by the ten bits from
+        // `low` on.  The counters are clear: a search clears what it has read.
         auto fill = [&](int low, uint32_t prefix, int bin) {
-            __syncthreads();
-            for (int i = tid; i < kLevel2; i += kThreads) s.count2[i] = 0, s.mass2[i] = 0;
-            __syncthreads();
             auto one = [&](uint32_t r) {
                 if ((r >> (low + 10)) == prefix) add((r >> low) & (kLevel2 - 1), r, s.count2, s.mass2);
             };
@@ -312,19 +312,10 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
             else each(one);
             __syncthreads();
         };
-        // The bin of this level in which the place lies, and what lies before it
-        // (added to n0, m0).
-        auto search = [&](const uint32_t* count, const uint64_t* mass, int bins, bool by_count, int n, uint64_t m,
-                          bool past, int& n0, uint64_t& m0) {
-            const int per = bins / kThreads;
-            int c = 0;
-            uint64_t w = 0;
-            for (int i = 0; i < per; ++i) {
-                c += count[tid * per + i];
-                w += mass[tid * per + i];
-            }
-            int cu = wave_scan(c);
-            uint64_t wu = wave_scan(w);
+        // What lies before this thread's c tokens of mass w, over all threads.
+        auto before = [&](int c, uint64_t w, int& ca, uint64_t& wa) {
+            const int cu = wave_scan(c);
+            const uint64_t wu = wave_scan(w);
             if (lane == 63) {
                 s.part_count[wave] = cu;
                 s.part_mass[wave] = wu;
@@ -334,21 +325,28 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
                 s.answer = -1;
             }
             __syncthreads();
-            for (int v = 0; v < wave; ++v) {
-                cu += s.part_count[v];
-                wu += s.part_mass[v];
-            }
-            int ca = n0 + cu - c;
-            uint64_t wa = m0 + wu - w;
+            const int own_c = lane < kWaves ? s.part_count[lane] : 0;
+            const uint64_t own_w = lane < kWaves ? s.part_mass[lane] : 0;
+            const int base_c = wave_scan(own_c) - own_c;
+            const uint64_t base_w = wave_scan(own_w) - own_w;
+            ca = cu - c + __builtin_amdgcn_readlane(base_c, wave);
+            wa = wu - w + __builtin_bit_cast(uint64_t, lane_double(__builtin_bit_cast(double, base_w), wave));
+        };
+        // The bin in which the place lies, of `per` bins to a thread from bin tid * per on,
+        // and what lies before it: n0, m0, of which ca and wa lie before this thread's.
+        auto pick = [&](const int* count, const uint64_t* mass, int per, bool by_count, int n, uint64_t m, bool past, int ca,
+                        uint64_t wa, int& n0, uint64_t& m0) {
             int last = -1, last_c = 0;  // the place if no bin reaches it: the last that has tokens
             uint64_t last_w = 0;
-            for (int i = 0; i < per; ++i) {
-                const int bc = count[tid * per + i];
-                const uint64_t bw = mass[tid * per + i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i == per) break;
+                const int bc = count[i];
+                const uint64_t bw = mass[i];
                 if (bc > 0) {
-                    const bool before = by_count ? ca < n : past ? wa <= m : (wa < m || ca == 0);
+                    const bool first = by_count ? ca < n : past ? wa <= m : (wa < m || ca == 0);
                     const bool reached = by_count ? ca + bc >= n : past ? wa + bw > m : wa + bw >= m;
-                    if (before && reached && atomicCAS(&s.found, -1, tid * per + i) == -1) {
+                    if (first && reached && atomicCAS(&s.found, -1, tid * per + i) == -1) {
                         s.before_count = ca;
                         s.before_mass = wa;
                     }
@@ -359,7 +357,7 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
                 ca += bc;
                 wa += bw;
             }
-            if (last >= 0) atomicMax(&s.answer, last);
+            if (last >= 0 && __ballot(last >= 0) >> lane == 1) atomicMax(&s.answer, last);
             __syncthreads();
             int f = s.found;
             if (f < 0) {
@@ -375,17 +373,50 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
             __syncthreads();
             return static_cast<uint32_t>(f);
         };
+        auto search2 = [&](bool by_count, int n, uint64_t m, bool past, int& n0, uint64_t& m0, int* tokens) {
+            const int c = s.count2[tid];
+            const uint64_t w = s.mass2[tid];
+            int ca;
+            uint64_t wa;
+            before(c, w, ca, wa);
+            const uint32_t f = pick(&c, &w, 1, by_count, n, m, past, ca + n0, wa + m0, n0, m0);
+            if (tokens) *tokens = s.count2[f];
+            __syncthreads();
+            s.count2[tid] = 0;
+            s.mass2[tid] = 0;
+            __syncthreads();
+            return f;
+        };
+        // this thread's bins of level 1, which stay
+        constexpr int kPer = kLevel1 / kThreads;
+        int c1[kPer], before1;
+        uint64_t w1[kPer], before1_w;
+        {
+            int c = 0;
+            uint64_t w = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                c += c1[i] = s.count1[kPer * tid + i];
+                w += w1[i] = s.mass1[kPer * tid + i];
+            }
+            before(c, w, before1, before1_w);
+        }
+        __syncthreads();
         auto find = [&](bool by_count, int n, double mass, bool past) {
             const uint64_t m = static_cast<uint64_t>(fmax(mass, 0.0) * unit + (past ? 0.0 : 0.5));
-            int n0 = 0;
+            int n0 = 0, bc = 0;
             uint64_t m0 = 0;
-            const uint32_t high = search(s.count1, s.mass1, kLevel1, by_count, n, m, past, n0, m0);
+            if (tid == 0) {
+                s.found = -1;
+                s.answer = -1;
+            }
+            __syncthreads();
+            const uint32_t high = pick(c1, w1, kPer, by_count, n, m, past, before1, before1_w, n0, m0);
             list(high);
             fill(10, high, high);
-            const uint32_t bin = (high << 10) | search(s.count2, s.mass2, kLevel2, by_count, n, m, past, n0, m0);
+            const uint32_t bin = (high << 10) | search2(by_count, n, m, past, n0, m0, nullptr);
             fill(0, bin, high);
-            const uint32_t low = search(s.count2, s.mass2, kLevel2, by_count, n, m, past, n0, m0);
-            const int bc = s.count2[low];
+            const uint32_t low = search2(by_count, n, m, past, n0, m0, &bc);
             Place p;
             p.bin = (bin << 10) | low;
             p.w = P.weight(value32(p.bin), top);
@@ -397,7 +428,7 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
                                  : static_cast<int>(fmin(fmax(ceil(q), 1.0), static_cast<double>(bc)));
             return p;
         };
-        int n = total, cut = total;
+        int cut = total, weighed = total;  // kept tokens; those whose mass `mass` is
         double mass = static_cast<double>(s.sum) * back;
 #pragma nounroll
         for (int stage = 0; stage < 5; ++stage) {
@@ -405,15 +436,15 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
             int number = 0;
             double amount = 0.0;
             if (stage == 0) {  // the first top_k and their mass
-                if (P.top_k <= 0 || P.top_k >= n) continue;
-                number = n = cut = P.top_k;
+                if (P.top_k <= 0 || P.top_k >= cut) continue;
+                number = P.top_k;
             } else if (stage == 1) {  // of those, top_p of their mass
                 if (P.top_p >= 1.0) continue;
                 by_count = false;
                 amount = P.top_p * mass;
-            } else if (stage == 2) {  // of those, what min_p keeps; the mass of the kept
+            } else if (stage == 2) {  // of those, what min_p keeps; the mass of the kept, where it is not known
                 cut = max(min(cut, s.kept), 1);
-                if (cut == n) continue;
+                if (cut == weighed) continue;
                 number = cut;
             } else if (stage == 3) {  // the draw
                 by_count = false;
@@ -424,10 +455,13 @@ __device__ void sample_ranks(const SampleArgs& a, int row, Lds32& s) {
                 number = cut;
             }
             const Place p = find(by_count, number, amount, past);
-            if (stage == 1) {
-                cut = min(cut, max(p.count + p.in_bin, 1));
-            } else if (stage < 3) {
-                mass = p.mass + p.in_bin * p.w;
+            if (stage < 3) {
+                const int upto = p.count + p.in_bin;
+                if (upto <= cut) {
+                    weighed = upto;
+                    mass = p.mass + p.in_bin * p.w;
+                }
+                cut = max(min(cut, upto), 1);
             } else {
                 at = p;
                 at.in_bin -= stage == 4 ? 1 : 0;
