@@ -288,3 +288,32 @@ def test_two_graphs_on_two_streams(gpu):
         for p, o, a in zip(ps, outs, args):
             p.check(o)
             assert torch.equal(o, ext().kv_attention(*a, p.scale))
+
+
+def test_one_key_head_for_many_query_heads(gpu):
+    """128 query heads over one key head: a single new token fills a tile of 128 rows."""
+    p = Problem(gpu, "e4m3", 64, 128, 1, 32, [2500, 100, 0, 3], [1, 1, 0, 1], 1900)
+    p.poison()
+    p.check(p.run())
+
+
+def test_no_rows(gpu):
+    p = Problem(gpu, "int8", 64, 4, 2, 16, [5, 40], [0, 0], 2000)
+    assert p.run(max_new=0).shape == (0, 4, 64)
+    p = Problem(gpu, "int8", 64, 4, 2, 16, [5, 40], [0, 0], 2000, extra_rows=3)
+    assert bool((p.run(max_new=0) == 0).all())
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_sizes(gpu, seed):
+    """Any sizes together: requests idle, decoding and with prompts, bounds given, loose or not at all."""
+    g = gen(3000 + seed)
+    pick = lambda *v: v[int(torch.randint(len(v), (1,), generator=g))]  # noqa: E731
+    kv, group = pick(1, 2, 3), pick(1, 2, 5, 8)
+    n, longest = pick(1, 2, 5, 9), pick(40, 300, 1100, 2600)
+    lens = [int(v) for v in torch.randint(0, longest + 1, (n,), generator=g)]
+    new = [min(pick(0, 1, 1, 2, 9, 70), m) for m in lens]
+    p = Problem(gpu, pick("e4m3", "int8"), pick(64, 128, 256), kv * group, kv, pick(16, 32, 64, 128, 256), lens, new, seed,
+                extra_rows=pick(0, 2))
+    p.poison()
+    p.check(p.run(max_new=pick(0, p.new, p.new + 3), max_len=pick(0, p.longest, 4 * p.longest)))

@@ -295,3 +295,15 @@ def test_append_large_decode_batch(gpu, bs):
     q, k, v = (torch.randn(n, h, dim, generator=gen(75 + h)).half() for h in (8, heads, heads))
     cos, sin = _rope(90, 64)
     _append(kc, vc, k, v, slots, q, torch.randint(0, 90, (n,), generator=gen(78)).int(), cos, sin)
+
+
+def test_append_turns_keys_without_queries(gpu):
+    """A rotation without q, and on a stream of the caller's."""
+    kc, vc = (Cache("e4m3", 9, 2, 16, 128, gpu, s) for s in (81, 82))
+    slots, pos = _requests([(0, 40), (7, 60)], 16, 9, gen(83))
+    k, v = (torch.randn(slots.numel(), 2, 128, generator=gen(84 + i)).half() for i in range(2))
+    cos, sin = _rope(64, 48)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        assert _append(kc, vc, k, v, slots, None, pos, cos, sin) is None
