@@ -825,12 +825,12 @@ struct Plan {
 constexpr int kCus = 256;  // compute units of the device: the workspace's size goes by it
 // Requests of up to kFewRows rows take 16-row tiles, the others 128-row ones, and
 // all take 16-row ones, in one launch, where none has more than twice as many (32
-// requests of up to 4096 tokens over 8 heads: 8 to 32 rows each 21 us in 16-row
-// tiles, 44 with those past 16 in 128-row ones; 16 to 64 rows 37 us in 16-row tiles,
-// 49 split at 32; 40 to 128 rows 54 split at 64, 39 in 128-row ones).
+// requests of up to 4096 tokens over 8 heads: 8 to 32 rows each 64 us in 16-row
+// tiles, 132 with those past 16 in 128-row ones; 16 to 64 rows 111 us in 16-row
+// tiles, 146 split at 32; 40 to 128 rows 162 split at 64, 119 in 128-row ones).
 constexpr int kFewRows = 32;
 // A sequence of up to this many tokens is one workgroup's (4 requests over 8 heads,
-// up to 1024 tokens: 4.3 us whole, 5.7 shared out; up to 2048: 6.8 against 5.8).
+// up to 1024 tokens: 12.8 us whole, 17.2 shared out; up to 2048: 20.3 against 17.3).
 constexpr int64_t kWholeTokens = 1024;
 
 void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int64_t max_len,
@@ -846,7 +846,8 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
 
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.  (256 requests
-// of up to 4000 tokens over 8 heads: 73 us whole, 79 shared out.)
+// of up to 4000 tokens over 8 heads: 218 us whole, 236 shared out; a prompt of 500 tokens
+// behind 1500, 128 tiles: 64 whole, 75 shared out; one of 64 in 32 tiles: 59 and 36.)
 Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
     Plan p;
     const int64_t rows = max_new * (q_heads / kv_heads);
