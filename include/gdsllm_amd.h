@@ -469,10 +469,10 @@ int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests
  * angle whose cosine and sine are cos, sin [max_pos][rotary/2] at positions[t];
  * the rotated values are rounded once, to fp16.
  * The tokens of one block stand in consecutive rows (as kv_assign numbers
- * them); a block occurs in one such run only.  With o the lowest offset that
- * the call writes in a block, what the block held before o stays and what it
- * held from o on is replaced.  The (block, head)'s scale becomes the smallest
- * power of two s >= 2^-32 with |x| <= top * s (top 448 or 127) for its new
+ * them, no padding between them); a block occurs in one such run only.  With o
+ * the lowest offset that the call writes in a block, what the block held before o
+ * stays and what it held from o on is replaced.  The (block, head)'s scale
+ * becomes the smallest power of two s >= 2^-32 with |x| <= top * s (top 448 or 127) for its new
  * finite values, or the scale it had, if o > 0 and that is larger; older codes
  * are rescaled to a scale that grew.  Codes are x / s to nearest even,
  * saturated; NaN stays NaN in e4m3 and is 0 in int8.  (A scale that it had is

@@ -307,3 +307,14 @@ def test_append_turns_keys_without_queries(gpu):
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         assert _append(kc, vc, k, v, slots, None, pos, cos, sin) is None
+
+
+def test_append_long_prompt_in_large_blocks(gpu):
+    """Past 2048 tokens the queries of large blocks are turned by a launch of their own."""
+    bs, dim = 256, 64
+    kc, vc = (Cache("int8", 12, 1, bs, dim, gpu, s) for s in (91, 92))
+    slots, pos = _requests([(0, 2100), (5, 80)], bs, 12, gen(93))
+    slots, pos = (torch.cat([t[:2100], torch.tensor([-1, -1], dtype=torch.int32), t[2100:]]) for t in (slots, pos))
+    q, k, v = (torch.randn(slots.numel(), h, dim, generator=gen(94 + h)).half() for h in (3, 1, 1))
+    cos, sin = _rope(2100, 16)
+    _append(kc, vc, k, v, slots, q, pos, cos, sin)
