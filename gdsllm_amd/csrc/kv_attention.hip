@@ -590,12 +590,16 @@ struct PromptTile {
                     for (int u = 0; u < U; ++u) {
                         const float er = pg[u].e - ref;
                         half8_t pf;
+                        // the sum takes the weights before they are rounded: a block of small
+                        // values has weights that fp16 does not hold, 1 / v_scale times which are
+                        // its share of the softmax
+                        float p[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            pf[i] = static_cast<half_t>(__builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u & 1) + i], pg[u].c, er)));
-                        const uint4 pw = __builtin_bit_cast(uint4, pf);
-                        constexpr uint32_t ones = 0x3C003C00u;
-                        l = fmaf(dot2(pw.x, ones, dot2(pw.y, ones, dot2(pw.z, ones, dot2(pw.w, ones, 0.f)))), pg[u].inv, l);
+                        for (int i = 0; i < 8; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u & 1) + i], pg[u].c, er));
+                            pf[i] = static_cast<half_t>(p[i]);
+                        }
+                        l = fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), pg[u].inv, l);
 #pragma unroll
                         for (int j = 0; j < DT; ++j) {
                             const half8_t vf = *reinterpret_cast<const half8_t*>(&s.v[buf][32 * j + col][16 * u + 8 * h]);

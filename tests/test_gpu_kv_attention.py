@@ -317,3 +317,32 @@ def test_drawn_sizes(gpu, seed):
                 extra_rows=pick(0, 2))
     p.poison()
     p.check(p.run(max_new=pick(0, p.new, p.new + 3), max_len=pick(0, p.longest, 4 * p.longest)))
+
+
+PROMPT_TILES = [("whole", 128, 2, 1, 64, [300], [100]), ("whole", 256, 4, 2, 16, [200, 90], [60, 90]),
+                ("shared", 64, 2, 1, 32, [2300], [80]), ("shared", 128, 3, 1, 128, [2100, 40], [40, 1]),
+                ("wide", 64, 512, 128, 16, [300, 140], [70, 110]), ("wide", 128, 512, 128, 64, [300, 140], [70, 110])]
+
+
+@pytest.mark.parametrize("values", ["apart", "zeros"])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("tiles,dim,heads,kv_heads,bs,lens,new", PROMPT_TILES,
+                         ids=[f"{t[0]}_{t[1]}" for t in PROMPT_TILES])
+def test_prompts_with_value_scales_far_apart(gpu, values, fmt, tiles, dim, heads, kv_heads, bs, lens, new):
+    """Prompts' tiles, one workgroup to a sequence and shared out, of 128 and 256 rows: a block whose values are
+    small or zero has its whole share of the softmax's sum.  "apart": value scales 2^20 and 2^40 apart; "zeros": all
+    blocks behind each request's first hold zeros at the scale kv_append gives them."""
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, lens, new, 2100 + dim, spread=0.0)
+    if values == "apart":
+        e = torch.arange(p.scales.shape[1]) % 3
+        p.scales[1] *= torch.exp2(torch.tensor([0.0, -40.0, -20.0]))[e][:, None]
+    else:
+        small = p.tables[:, 1:].flatten()
+        small = small[small >= 0].long()
+        p.codes[1].view(torch.uint8)[small] = 0
+        p.scales[1, small] = sv.MIN_SCALE
+    p.poison()
+    if tiles == "wide":
+        check_heads(p, p.run(), [0, 127])
+    else:
+        p.check(p.run())
