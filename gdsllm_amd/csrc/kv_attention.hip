@@ -837,6 +837,13 @@ constexpr int kFewRows = 32;
 // up to 1024 tokens: 12.8 us whole, 17.2 shared out; up to 2048: 20.3 against 17.3).
 constexpr int64_t kWholeTokens = 1024;
 
+// Bytes of `groups` workgroups' sums, two parts each of `rows` rows, and of the
+// sequences' entries.
+size_t part_bytes(int64_t groups, int64_t rows, int64_t sequences, int64_t head_dim) {
+    const size_t sums = static_cast<size_t>(groups) * 2 * rows * (head_dim + 2) * sizeof(float);
+    return groups ? (sums + sequences * sizeof(int2) + 15) / 16 * 16 : 0;
+}
+
 void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int64_t max_len,
                  int64_t resident, bool whole) {
     p->on = true;
@@ -844,9 +851,12 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
     p->sequences = requests * kv_heads * p->tiles;
     p->groups = whole ? 0 : static_cast<int>(std::min<int64_t>(resident, p->sequences * ((max_len + 255) / 256)));
     p->sums = static_cast<size_t>(p->groups) * 2 * p->rows;
-    p->bytes = p->groups ? p->sums * (head_dim + 2) * sizeof(float) + p->sequences * sizeof(int2) : 0;
-    p->bytes = (p->bytes + 15) / 16 * 16;
+    p->bytes = part_bytes(p->groups, p->rows, p->sequences, head_dim);
 }
+
+// Workgroups that the device holds at once, of 16-row and of 128-row tiles.
+int64_t resident_few(int64_t head_dim) { return per_cu(head_dim) * static_cast<int64_t>(kCus); }
+int64_t resident_many(int64_t head_dim) { return (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus); }
 
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.  (256 requests
@@ -859,13 +869,13 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
     if (!many || requests > 1) {
         p.few.rows = 16;
         if (many) p.few.max_rows = kFewRows;
-        const int64_t most = many ? kFewRows : rows, resident = per_cu(head_dim) * static_cast<int64_t>(kCus);
+        const int64_t most = many ? kFewRows : rows, resident = resident_few(head_dim);
         const int64_t sequences = requests * kv_heads * ((most + 15) / 16);
         finish_part(&p.few, requests, kv_heads, head_dim, most, max_len, resident,
                     max_len <= kWholeTokens || sequences >= (max_len <= 4 * kWholeTokens ? 2 : 8) * resident);
     }
     if (many) {
-        const int64_t resident = (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus);
+        const int64_t resident = resident_many(head_dim);
         // eight waves to a tile (each converts half as much) where that still leaves
         // two workgroups to a compute unit, one after the other: 4096 tokens of 32
         // heads 173 us against 183; 4 chunks of 300 tokens 166 against 162
@@ -877,6 +887,23 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
                     wide || max_len <= (4 * sequences >= resident ? 2 : 1) * kWholeTokens || 2 * sequences >= resident);
     }
     return p;
+}
+
+// At least the bytes of plan_attend for every smaller number of requests, max_new
+// and max_len too, which need not be less: a prompt of 4096 tokens of 32 heads is
+// whole and needs none, 64 tokens behind as many share their work.  Work is
+// shared out past kWholeTokens alone, by up to 64 rows of fewer than 8 * resident
+// sequences and by 128-row tiles of fewer than resident / 2.
+size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
+    if (max_len <= kWholeTokens) return 0;
+    const int64_t rows = max_new * (q_heads / kv_heads), units = (max_len + 255) / 256;
+    auto part = [&](int64_t tile, int64_t most, int64_t limit, int64_t resident) {
+        const int64_t sequences = std::min(requests * kv_heads * std::max<int64_t>(1, (most + tile - 1) / tile), limit);
+        return part_bytes(std::min(resident, sequences * units), tile, sequences, head_dim);
+    };
+    size_t bytes = part(16, std::min<int64_t>(rows, 2 * kFewRows), 8 * resident_few(head_dim), resident_few(head_dim));
+    if (rows > 2 * kFewRows) bytes += part(128, rows, resident_many(head_dim) / 2, resident_many(head_dim));
+    return bytes;
 }
 
 // Launches one part of a call: W where a workgroup has a whole sequence, S where
@@ -938,7 +965,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return plan_attend(requests, q_heads, kv_heads, head_dim, max_new, max_len).bytes();
+    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len);
 }
 
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,

@@ -498,7 +498,8 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * (0: tokens, and table_width * block_size).  They set how the work is split;
  * larger requests than they say are computed all the same, more slowly.  The
  * workspace's size is asked for with the same bounds (tokens or table_width *
- * block_size where one is 0).
+ * block_size where one is 0) or larger ones: it serves every call with as many
+ * requests, rows and tokens or fewer.
  * Rows behind the last request are left as they were, or set to zero with
  * zero_tail.  workspace_bytes >= gdsllm_kv_attention_workspace_size(...).    */
 size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,

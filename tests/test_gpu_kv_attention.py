@@ -1,9 +1,12 @@
 """Attention over the 8-bit cache against the plain 64-bit form
 (oracle/serve.py attention, which derives the bound its results are held to)."""
 
+import ctypes
+
 import pytest
 import torch
 
+from gdsllm_amd import KvCache8, capi
 from gdsllm_amd.runtime import ext
 from helpers import gen
 from oracle import serve as sv
@@ -346,3 +349,26 @@ def test_prompts_with_value_scales_far_apart(gpu, values, fmt, tiles, dim, heads
         check_heads(p, p.run(), [0, 127])
     else:
         p.check(p.run())
+
+
+@pytest.mark.parametrize("lens,new", [([3000], [64]), ([3000, 40], [1, 1]), ([2500, 700, 0], [70, 3, 0]), ([90], [1])])
+def test_workspace_of_the_largest_step(gpu, lens, new):
+    """C callers size their workspace once: a call with the same bounds and fewer tokens, or with bounds of its own,
+    finds it large enough and writes nothing behind it."""
+    p = Problem(gpu, "e4m3", 128, 4, 2, 64, lens, new, 2200 + sum(lens))
+    p.poison()
+    lib = capi()
+    size = lib.gdsllm_kv_attention_workspace_size(4, 4, 2, 128, 4096, 4096)
+    t = [x.to(gpu) for x in (p.q, p.codes[0], p.codes[1], p.scales[0], p.scales[1], p.tables, p.lens, p.starts)]
+    q, k, v, ks, vs, tables, lens_d, starts = t
+    cache = KvCache8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.shape[0], 2, 64, 128, 0)
+    for max_new, max_len in ((4096, 4096), (p.new, p.longest), (0, 0)):
+        ws, out = torch.full((size + 4096,), 0x5A, dtype=torch.uint8, device=gpu), torch.full_like(q, 9.0)
+        torch.cuda.synchronize()
+        rc = lib.gdsllm_kv_attention(ctypes.byref(cache), q.data_ptr(), 512, out.data_ptr(), 512, q.shape[0], 4,
+                                     tables.data_ptr(), tables.shape[1], tables.shape[1], lens_d.data_ptr(),
+                                     starts.data_ptr(), len(lens), p.scale, max_new, max_len, 1, ws.data_ptr(), size,
+                                     torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, lib.gdsllm_last_error().decode()
+        p.check(out)
+        assert bool((ws[size:] == 0x5A).all())

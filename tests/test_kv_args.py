@@ -157,3 +157,16 @@ def test_extension_refuses_host_tensors():
         e.kv_attention(row, cache, cache, f, f, i.view(2, 1), i, i, 1.0)
     with pytest.raises(RuntimeError, match="sample_tokens: logits must be"):
         e.sample_tokens(torch.zeros(2, 5), f)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 32, 128), (64, 8, 128), (32, 2, 256), (8, 1, 64), (128, 1, 64)])
+def test_attention_workspace_serves_smaller_calls(heads, kv_heads, dim):
+    """A workspace sized for the largest step is enough for every step with fewer requests, rows or tokens."""
+    size = capi().gdsllm_kv_attention_workspace_size
+    steps = [(r, new, length) for r in (1, 4, 64, 300) for new in (0, 1, 3, 33, 64, 70, 300, 4096)
+             for length in (16, 1024, 1025, 2048, 4096, 4097, 131072)]
+    sizes = {s: size(s[0], heads, kv_heads, dim, s[1], s[2]) for s in steps}
+    for big in steps:
+        for small in steps:
+            if all(a <= b for a, b in zip(small, big)):
+                assert sizes[small] <= sizes[big], (small, big)
