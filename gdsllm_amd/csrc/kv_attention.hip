@@ -8,11 +8,14 @@
 // cores as the fp16 values they are, so the products q . code and P . code are
 // exact and summed in fp32; the scales stay outside: a block's key scale
 // multiplies its scores, and its value scale is carried in the exponent.  With
-// e = log2(v_scale) and m within 2^8 of the largest y_j = x_j log2 e + e so far,
-//   acc += 2^(y_j - m) * code_j,   l += 2^(y_j - m) / v_scale,   o = acc / l,
-// so the fp16 weights 2^(y_j - m) <= 2^8 (half a step of fp16 each: the one
-// rounding before the last) lose nothing to a block whose values are large or
-// small, whatever the other blocks' scales are.
+// e = log2(v_scale) and m 7 to 15 below the largest y_j = x_j log2 e + e so far,
+//   acc += 2^(y_j - m) * code_j,   l += 2^(y_j - m) / v_scale,   o = acc / l.
+// The weights are rounded to fp16 for the product with the codes (the matrix cores
+// take no wider operand at this rate) and for it alone: l takes them in fp32,
+// since in a block of small values they may be less than fp16 holds.  That
+// rounding, the one before the last, is half an fp16 step of a weight, and 2^-25
+// at least: the largest is 2^7 to 2^15, so a key's share of the values is off by
+// 2^-11 of itself or 2^-32 of the largest share, whichever is more.
 //
 // The G query heads of a kv head and the query rows share its keys: they are
 // the columns of a matrix tile (row r = token r / G, head r % G), 16 of them for
@@ -42,7 +45,10 @@ namespace {
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;              // log2 of how far a score may pass the reference
+// log2 of a weight where the reference is set, and of the largest that leaves it
+// (fp16 holds 2^15): the lower the reference, the more of a long tail of small
+// weights fp16 holds (largest weights of 1 lost tails of 2^-25 a key altogether).
+constexpr float kSet = 7.f, kMost = 15.f;
 constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
 constexpr int kMaxPages = kSegment / 16;   // segments begin on a block of 64 tokens
 constexpr int kBlock = 64;                 // tokens of a unit of work
@@ -294,10 +300,9 @@ struct RowTile {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
                 mx = over_groups(mx, [](float u, float v) { return fmaxf(u, v); });
-                // the reference follows the maximum only when that has left it 2^8 behind:
-                // weights up to 2^8 are as good in fp16 and the sums in fp32
-                if (__any(mx > m + kSlack)) {
-                    const float m_new = fmaxf(m, mx);
+                // the reference follows the maximum only when a weight would pass 2^15
+                if (__any(mx > m + kMost)) {
+                    const float m_new = fmaxf(m, mx - kSet);
                     const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                     l *= alpha;
 #pragma unroll
@@ -577,8 +582,8 @@ struct PromptTile {
                         swap32(p, q);
                         mx = fmaxf(p, q);
                     }
-                    if (__any(mx > m + kSlack)) {  // as in RowTile
-                        const float m_new = fmaxf(m, mx);
+                    if (__any(mx > m + kMost)) {  // as in RowTile
+                        const float m_new = fmaxf(m, mx - kSet);
                         const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                         l *= alpha;
 #pragma unroll

@@ -2,6 +2,7 @@
 (oracle/serve.py attention, which derives the bound its results are held to)."""
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -372,3 +373,38 @@ def test_workspace_of_the_largest_step(gpu, lens, new):
         assert rc == 0, lib.gdsllm_last_error().decode()
         p.check(out)
         assert bool((ws[size:] == 0x5A).all())
+
+
+LONG_TAILS = [("decode", 64, 2, 1, 16, [1000], [1]), ("decode_shared", 128, 2, 2, 64, [3000, 500], [1, 1]),
+              ("prompt", 128, 2, 1, 64, [900], [80]), ("prompt_shared", 256, 2, 1, 32, [2200], [70]),
+              ("prompt_wide", 64, 512, 128, 16, [200, 100], [70, 70])]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim,heads,kv_heads,bs,lens,new", [t[1:] for t in LONG_TAILS], ids=[t[0] for t in LONG_TAILS])
+def test_many_small_weights(gpu, fmt, dim, heads, kv_heads, bs, lens, new):
+    """Keys 2^-25.1 of the largest weight, 31 of every 32, with all of the values: they count by their share.  The
+    largest weight is taken as 2^7 at least, so theirs are 2^-18.1 and off by half a step of fp16's least, 2^-25;
+    the scores' and sums' fp32 and the result add 2^-20 and half an fp16 step."""
+    p = Problem(gpu, fmt, dim, heads, kv_heads, bs, lens, new, 2300 + dim, spread=0.0)
+    codes = torch.zeros(p.codes.shape)
+    codes[0, :, :, 0::32 if bs >= 32 else bs, 0] = 64
+    codes[1] = 100 * (codes[0, ..., :1] == 0)
+    if bs < 32:  # every other block of 16
+        odd = p.tables[:, 1::2].flatten()
+        codes[0, odd[odd >= 0].long()], codes[1, odd[odd >= 0].long()] = 0, 100
+    p.codes = codes.to(sv.DTYPE[fmt])
+    p.scales[0], p.scales[1], p.scale = 1.0, 2.0 ** 8, 1.0
+    p.q.zero_()
+    p.q[..., 0] = 17.4 / 64
+    got = p.run().cpu().double()
+    sel = [0] if kv_heads == 128 else range(kv_heads)
+    G = heads // kv_heads
+    for h in sel:
+        vals = p.codes[:, :, h:h + 1].double() * p.scales[:, :, h:h + 1, None, None].double()
+        want, _ = sv.attention(p.q[:, h * G:(h + 1) * G], vals[0], vals[1], p.scales[1, :, h:h + 1].double(), p.tables, p.lens,
+                               p.starts, p.scale)
+        assert float(want.max()) > 0.01
+        err = (got[:, h * G:(h + 1) * G] - want).abs()
+        weight = 2.0 ** (7 - float(p.q[0, 0, 0]) * 64 * math.log2(math.e))
+        assert bool((err <= (2.0 ** -25 / weight + 2.0 ** -11 + 2.0 ** -20) * want + 2.0 ** -25).all()), float((err / want).max())
