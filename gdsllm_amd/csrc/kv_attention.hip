@@ -67,7 +67,7 @@ struct AttendArgs {
     int min_rows, max_rows;  // requests with other numbers of rows are left to another launch
     int tiles;               // row tiles of a request that the grids have
     int groups;              // workgroups that share the work evenly
-    int zero_tail;           // rows behind the last request are set to zero
+    int zero_other;          // rows of no request are set to zero
 };
 
 // A request's rows, in tiles of RT, and the keys they may see.
@@ -112,11 +112,15 @@ constexpr int per_cu(int64_t D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
 
 __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
 
-__device__ __forceinline__ void zero_rows_behind(const AttendArgs& a, int D) {
-    if (!a.zero_tail) return;
-    for (int64_t t = min(max(a.starts[a.requests], 0), a.tokens) + blockIdx.x; t < a.tokens; t += gridDim.x)
-        for (int i = threadIdx.x; i < a.q_heads * D / 8; i += blockDim.x)
-            *reinterpret_cast<uint4*>(a.o + t * a.ldo + 8 * i) = make_uint4(0, 0, 0, 0);
+// Rows of no request: before the first one's and behind the last one's.
+__device__ __forceinline__ void zero_other_rows(const AttendArgs& a, int D) {
+    if (!a.zero_other) return;
+    const int before = min(max(a.starts[0], 0), a.tokens), end = min(max(a.starts[a.requests], before), a.tokens);
+    for (int64_t i = blockIdx.x; i < before + a.tokens - end; i += gridDim.x) {
+        const int64_t t = i < before ? i : end + i - before;
+        for (int c = threadIdx.x; c < a.q_heads * D / 8; c += blockDim.x)
+            *reinterpret_cast<uint4*>(a.o + t * a.ldo + 8 * c) = make_uint4(0, 0, 0, 0);
+    }
 }
 
 // 16 rows over blocks [block0, block1) of a sequence, by NW waves.  Matrix tiles
@@ -659,7 +663,7 @@ __global__ __launch_bounds__(T::kThreads) void attend_whole(AttendArgs a) {
     const int head = blockIdx.x % a.c.kv_heads;
     for (int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / a.c.kv_heads; tile < R.tiles(); tile += a.tiles)
         T::run(a, s, b, R, tile, head, 0, R.blocks(), -1, early);
-    if (b == 0) zero_rows_behind(a, T::kD);
+    if (b == 0) zero_other_rows(a, T::kD);
 }
 
 // The work as one line of blocks: request after request, in each its row tiles,
@@ -676,7 +680,7 @@ __global__ __launch_bounds__(256, T::kPerCu) void attend_shared(AttendArgs a) {
     typename T::Lds& s = *reinterpret_cast<typename T::Lds*>(raw);
     __shared__ int s_part[4], s_request, s_begin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wg = blockIdx.x;
-    zero_rows_behind(a, T::kD);
+    zero_other_rows(a, T::kD);
     int total = 0, share = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int carry = 0;
@@ -945,11 +949,11 @@ int launch_part(AttendArgs a, const Part& p, int64_t blocks, int64_t max_rows, c
 
 template <bool E4M3, int D>
 int launch_attend(AttendArgs a, const Plan& p, int64_t blocks, int64_t max_rows, char* workspace, hipStream_t s) {
-    const int zero_tail = a.zero_tail;
-    a.zero_tail = p.few.on ? zero_tail : 0;
+    const int zero_other = a.zero_other;
+    a.zero_other = p.few.on ? zero_other : 0;
     if (int rc = launch_part<RowTile<E4M3, D, 8>, RowTile<E4M3, D, 4>>(a, p.few, blocks, p.many.on ? kFewRows : max_rows, workspace, s))
         return rc;
-    a.zero_tail = p.few.on ? 0 : zero_tail;
+    a.zero_other = p.few.on ? 0 : zero_other;
     char* ws = workspace + p.few.bytes;
     if constexpr (D <= 128)
         if (p.many.rows == 256) return launch_part<PromptTile<E4M3, D, 8>, PromptTile<E4M3, D, 4>>(a, p.many, blocks, max_rows, ws, s);
@@ -976,7 +980,7 @@ extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
                                    int64_t tokens, int64_t q_heads, const int32_t* block_tables, int64_t table_width,
                                    int64_t ld_table, const int32_t* lens, const int32_t* starts, int64_t requests,
-                                   float scale, int64_t max_new, int64_t max_len, int zero_tail, void* workspace,
+                                   float scale, int64_t max_new, int64_t max_len, int zero_other, void* workspace,
                                    size_t workspace_bytes, void* stream) {
     const std::string n = "kv_attention";
     auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
@@ -1022,7 +1026,7 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     a.q_heads = static_cast<int>(q_heads);
     a.group = static_cast<int>(q_heads / cache->kv_heads);
     a.width = static_cast<int>(table_width);
-    a.zero_tail = zero_tail;
+    a.zero_other = zero_other;
     const int64_t max_rows = max_new * a.group;
     if (tokens * q_heads > (int64_t(1) << 30)) return bad("tokens * q_heads must be at most 2^30");
     const int64_t blocks = most / kBlock + 1;

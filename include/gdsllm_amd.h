@@ -502,14 +502,14 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * workspace's size is asked for with the same bounds (tokens or table_width *
  * block_size where one is 0) or larger ones: it serves every call with as many
  * requests, rows and tokens or fewer.
- * Rows behind the last request are left as they were, or set to zero with
- * zero_tail.  workspace_bytes >= gdsllm_kv_attention_workspace_size(...).    */
+ * Rows of no request, before the first one's and behind the last one's, are left
+ * as they were, or set to zero with zero_other.  workspace_bytes >= gdsllm_kv_attention_workspace_size(...).    */
 size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                           int64_t max_new, int64_t max_len);
 int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
                         int64_t tokens, int64_t q_heads, const int32_t* block_tables, int64_t table_width,
                         int64_t ld_table, const int32_t* lens, const int32_t* starts, int64_t requests, float scale,
-                        int64_t max_new, int64_t max_len, int zero_tail, void* workspace, size_t workspace_bytes,
+                        int64_t max_new, int64_t max_len, int zero_other, void* workspace, size_t workspace_bytes,
                         void* stream);
 
 /* -------------------------------------------------------------- sampling --

@@ -408,3 +408,22 @@ def test_many_small_weights(gpu, fmt, dim, heads, kv_heads, bs, lens, new):
         err = (got[:, h * G:(h + 1) * G] - want).abs()
         weight = 2.0 ** (7 - float(p.q[0, 0, 0]) * 64 * math.log2(math.e))
         assert bool((err <= (2.0 ** -25 / weight + 2.0 ** -11 + 2.0 ** -20) * want + 2.0 ** -25).all()), float((err / want).max())
+
+
+@pytest.mark.parametrize("lens,new,max_len", [([100, 7], [2, 1], 0), ([2500, 30], [1, 1], 0), ([200], [90], 0)],
+                         ids=["whole", "shared", "prompt"])
+def test_rows_before_the_first_request(gpu, lens, new, max_len):
+    """Some of a batch's requests: the rows of none of them are zero in a new tensor and left alone in a given one."""
+    p = Problem(gpu, "e4m3", 64, 4, 2, 32, lens, new, 2400, extra_rows=5)
+    p.poison()
+    p.starts += 3
+    used = [torch.full(p.q.shape, 9.0, dtype=torch.float16, device=gpu) for _ in range(1024)]
+    del used  # what a new tensor holds is no zero by chance
+    got = p.run(max_len=max_len)
+    p.check(got)
+    rest = torch.ones(p.q.shape[0], dtype=torch.bool)
+    rest[3:3 + sum(new)] = False
+    assert bool((got[rest.to(gpu)] == 0).all())
+    out = torch.full_like(got, 7.0)
+    p.run(max_len=max_len, output=out)
+    assert bool((out[rest.to(gpu)] == 7).all()) and torch.equal(out[~rest.to(gpu)], got[~rest.to(gpu)])
