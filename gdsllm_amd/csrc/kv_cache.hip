@@ -512,7 +512,9 @@ extern "C" int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64
          reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(starts) |
          reinterpret_cast<uintptr_t>(lens_out) | reinterpret_cast<uintptr_t>(state_out)) % 4)
         return bad("misaligned pointer");
-    if (lens_out == lens || state_out == free_state) return bad("lens_out and state_out must not be the inputs");
+    for (const int32_t* in : {lens, delta, free_state})
+        if (lens_out == in || state_out == in) return bad("lens_out and state_out must not be the inputs");
+    if (lens_out == state_out) return bad("lens_out and state_out must not be one buffer");
     AssignArgs a{lens, delta, block_tables, free_ring, free_state, slots, positions, starts, lens_out, state_out,
                  ld_table, static_cast<int>(requests), static_cast<int>(table_width), static_cast<int>(ring_size),
                  __builtin_ctzll(static_cast<unsigned long long>(block_size)), static_cast<int>(max_tokens)};

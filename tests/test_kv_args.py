@@ -170,3 +170,11 @@ def test_attention_workspace_serves_smaller_calls(heads, kv_heads, dim):
         for small in steps:
             if all(a <= b for a, b in zip(small, big)):
                 assert sizes[small] <= sizes[big], (small, big)
+
+
+def test_assign_outputs_apart_from_every_input():
+    """Workgroups read all of lens, delta and free_state while the first writes lens_out and state_out."""
+    base = [16, 32, 1, 48, 1, 1, 64, 1, 80, 16, 1, 96, 112, 128]  # lens, delta, ..., free_state, ..., slots, positions, starts
+    for lens_out, state_out in ((16, 144), (32, 144), (80, 144), (144, 16), (144, 32), (144, 80), (144, 144)):
+        assert capi().gdsllm_kv_assign(*base, lens_out, state_out, None) == BAD
+        assert "must not be" in _err()
