@@ -26,12 +26,13 @@
 //    30 of them attend_shared.  A short sequence (777 tokens, 32 heads, 9.6 us) is
 //    one chain of memory latencies: a launch, its length and table, its scales,
 //    then three tiles of codes to a wave.
-//  * Prompts are bound by vector work beside the matrix cores (softmax and the
-//    codes' conversion, about half the cycles; the matrix cores a third): 4096
-//    tokens of 32 heads 174 us, 790 TFLOP/s of a large product's 1028; 4 chunks of
-//    300 tokens with up to 5000 held 162 us, 510 TFLOP/s: 448 tiles of unequal
-//    length are 1.75 to a compute unit.  Even shares of their keys cost more than they
-//    give (156 us, and 92 to join 57000 rows); 16 such chunks reach 680.
+//  * Prompts are bound by vector work beside the matrix cores (by counters, softmax
+//    and the codes' conversion take 40% of a SIMD's cycles, its matrix core 35%):
+//    4096 tokens of 32 heads 171 us, 800 TFLOP/s of a large product's 1060; 4 chunks
+//    of 300 tokens with up to 5000 held 160 us, 515 TFLOP/s: 448 tiles of unequal
+//    length are 1.75 to a compute unit.  Even shares of their keys take 257 us, 92 of
+//    them in attend_join, which gives each of 57000 rows, most of two parts,
+//    a workgroup of its own; 16 such chunks reach 674.
 
 #include <algorithm>
 #include <climits>
@@ -870,7 +871,7 @@ int64_t resident_many(int64_t head_dim) { return (head_dim == 256 ? 1 : 2) * sta
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.  (256 requests
 // of up to 4000 tokens over 8 heads: 218 us whole, 236 shared out; a prompt of 500 tokens
-// behind 1500, 128 tiles: 64 whole, 75 shared out; one of 64 in 32 tiles: 59 and 36.)
+// behind 1500, 128 tiles: 62 whole, 66 shared out; one of 64 in 32 tiles: 57 and 34.)
 Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
     Plan p;
     const int64_t rows = max_new * (q_heads / kv_heads);
@@ -887,7 +888,7 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
         const int64_t resident = resident_many(head_dim);
         // eight waves to a tile (each converts half as much) where that still leaves
         // two workgroups to a compute unit, one after the other: 4096 tokens of 32
-        // heads 173 us against 183; 4 chunks of 300 tokens 166 against 162
+        // heads 172 us against 188; 4 chunks of 300 tokens 167 against 161
         const bool wide = head_dim <= 128 && requests * kv_heads * ((rows + 255) / 256) >= resident;
         p.many.rows = wide ? 256 : 128;
         if (p.few.on) p.many.min_rows = kFewRows + 1;

@@ -66,7 +66,8 @@ struct AssignArgs {
 // them: cheaper than a second launch or a grid barrier) and then writes its share
 // of the tables and of the token rows.  All of it is latency (a launch takes 1.65 us):
 // lengths, one scan of tokens, new and returned blocks, a ring entry, a store.  64
-// decoding requests 4.9 us, 2048 mixed ones with 66000 token rows 7.6 us.
+// decoding requests 4.9 us in a graph (called one by one, the host takes 7),
+// 2048 mixed ones with 66000 token rows 7.6 us.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_assign(AssignArgs a) {
     extern __shared__ int32_t lds[];
@@ -237,8 +238,9 @@ __device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
 }
 
 // Cosines and sines of eight channels, and their product with eight pairs: in 64
-// bits, where the products are exact, so the one rounding that counts is the
-// last, to fp16.
+// bits, where the products are exact; then to fp32 and from there to fp16, as
+// torch's own cast from 64 bits goes (a value within 2^-25 of itself of the middle
+// between two fp16 values may go to the farther one).
 struct Turn {
     float4_t c[2], s[2];
     __device__ __forceinline__ void load(const float* cos, const float* sin) {
@@ -388,7 +390,7 @@ __device__ void append_run(const Run& r, int tid, float* red) {
 // page.  Pages with few new rows go to one wave each, others to all of them.
 // Bound by the bytes of k, v, q and the codes for prompts (2 x 1000 tokens of 32 heads
 // 66 MB in 21 us, 3.1 TB/s; 8192 tokens with 32 query heads of 256 296 MB in 88 us,
-// 3.4), by latency for a decode step (32 tokens 4.5 us: slot, row and scale, a maximum,
+// 3.4), by latency for a decode step (32 tokens 4.2 us: slot, row and scale, a maximum,
 // a store).
 template <bool E4M3, int D, int WAVES>
 __device__ void append_pages(const AppendArgs& a, int unit) {

@@ -12,18 +12,22 @@
 // and every cut is found on the counts and on count * w: a prefix of the order
 // is a prefix of the values and a number of tokens of one of them.  First the
 // binade by its sum, then a value of it to each thread.  fp32 logits take the same
-// cuts over three levels of a 32-bit key.  All masses are 64-bit sums in a fixed
-// order (or whole numbers), so a row's token depends on its inputs alone, and a draw
-// next to a border falls on the side where 64 bits put it.
+// cuts over three levels of a 32-bit key.  Masses of fp16 rows are 64-bit floating
+// sums in a fixed order.  Those of fp32 rows, and of fp16 rows with more than 65535
+// equal logits, are 64-bit whole numbers of units of 2^-(62 - L) of the largest
+// weight, L = ceil(log2 vocab), so that atomics may add them in any order: each
+// weight is off by half a unit at most (less than that: it counts as none), a sum by
+// vocab / 2 units, 2^-29 of the largest weight at 131072 tokens, 2^-23 at 2^20.
+// Either way a row's token depends on its inputs alone.
 //
-// A row is one workgroup's, and bound by its latencies: 32000 tokens 15.5 us, of them
+// A row is one workgroup's, and bound by its latencies: 32000 tokens 15.2 us, of them
 // 3.5 to load and count, 4 for the sums of the binades (64-bit arithmetic in all
 // waves), 2 for each cut and the draw (two barriers and a chain of 64-bit scans), 1 to
-// find the token's index; 64 rows of 128257 on 64 compute units 27.3 us, 13 of them
+// find the token's index; 64 rows of 128257 on 64 compute units 27 us, 13 of them
 // for the two reads of a row.  More registers for the row (8 granules a thread, or 16)
 // spill; places looked for by four waves of four values a thread took as long.  fp32
-// rows are bound by the 64-bit weight of every token: 32000 tokens 68 us with three
-// cuts, 43 with none, 12 of them for what a row's largest logit alone takes.
+// rows are bound by the 64-bit weight of every token: 32000 tokens 63 to 69 us with
+// three cuts, 40 with none, 13 of them for what a row's largest logit alone takes.
 
 #include <algorithm>
 
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(kThreads) void sample_f16(SampleArgs a) {
         }
     }
     {
-        // the largest logit, as an order-keeping whole number (1024: -inf, so no token)
+        // the largest logit, as an order-keeping whole number (1023: -inf, so no token)
         const uint32_t x = __builtin_bit_cast(uint32_t, most);
         auto key = [](uint32_t h) { return static_cast<int>((h & 0x8000u) ? 0xFFFFu - h : 0x8000u | h); };
         const int k = wave_max(max(key(x & 0xFFFFu), key(x >> 16)));

@@ -80,7 +80,9 @@ class KVCache8:
         (starts[r] .. starts[r + 1] - 1 are request r's).  max_new and max_len:
         bounds on a request's new tokens and length that the host knows (0: none),
         which attend() splits its work by.  Leaves lens, slots, positions and
-        starts for the layers; asynchronous, and fit for a captured graph.
+        starts for the layers; asynchronous, and fit for a captured graph: lens and
+        the blocks are then advanced by each replay, while slots, positions, starts
+        and last_rows() stay those of the begin_step that Python ran last.
         """
         slots, positions, starts, lens, state = ext().kv_assign(
             self.lens, delta, self.block_tables, self.free_ring, self.free_state, self.block_size, max_tokens)
@@ -99,7 +101,8 @@ class KVCache8:
 
     def last_rows(self) -> torch.Tensor:
         """int64 [requests]: the row of each request's last new token in this
-        step's packed tensors; -1 for a request without one."""
+        step's packed tensors; -1 for a request without one.  Of a captured step:
+        taken within the capture."""
         last = self.starts[1:]
         return torch.where(last > self.starts[:-1], last - 1, -1).long()
 

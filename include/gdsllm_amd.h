@@ -467,7 +467,8 @@ int gdsllm_kv_assign(const int32_t* lens, const int32_t* delta, int64_t requests
  * keys, and q [tokens][q_heads * head_dim] into q_out (rows contiguous, apart from
  * q; q may be null), are rotated first: channels i and i + rotary/2 of a head turn by the
  * angle whose cosine and sine are cos, sin [max_pos][rotary/2] at positions[t];
- * the rotated values are rounded once, to fp16.
+ * the rotated values are taken in 64 bits and rounded to fp32 and then to fp16,
+ * as a cast from 64 bits to fp16 goes in torch.
  * The tokens of one block stand in consecutive rows (as kv_assign numbers
  * them, no padding between them); a block occurs in one such run only.  With o
  * the lowest offset that the call writes in a block, what the block held before o
@@ -523,7 +524,11 @@ int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ld
  * u times the kept mass.  temperature <= 0 (or NaN): the first token.  NaN and
  * -inf are never drawn; a row without any other value gives -1.  temperature,
  * top_k, top_p and min_p hold one value a row; null: 1, all, 1, 0.
- * Weights and sums in 64 bits.  Replaces _sample (engine.py:47-96), which
+ * Weights in 64 bits.  Sums too: fp16 rows in floating point; fp32 rows, and fp16
+ * rows with more than 65535 equal logits, in whole units of
+ * 2^-(62 - ceil(log2 vocab)) of the largest weight, half a unit off for each token
+ * at most (all of them together 2^-29 of it at 131072 tokens, 2^-23 at 2^20), so a
+ * draw or a cut that near to a border may fall on its other side.  Replaces _sample (engine.py:47-96), which
  * sorts the logits and draws on the host side of a sync.                     */
 int gdsllm_sample_tokens(const void* logits, int bits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
