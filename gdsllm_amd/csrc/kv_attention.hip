@@ -8,13 +8,13 @@
 // cores as the fp16 values they are, so the products q . code and P . code are
 // exact and summed in fp32; the scales stay outside: a block's key scale
 // multiplies its scores, and its value scale is carried in the exponent.  With
-// e = log2(v_scale) and m 7 to 15 below the largest y_j = x_j log2 e + e so far,
+// e = log2(v_scale) and m 7 to 11 below the largest y_j = x_j log2 e + e so far,
 //   acc += 2^(y_j - m) * code_j,   l += 2^(y_j - m) / v_scale,   o = acc / l.
 // The weights are rounded to fp16 for the product with the codes (the matrix cores
 // take no wider operand at this rate) and for it alone: l takes them in fp32,
 // since in a block of small values they may be less than fp16 holds.  That
 // rounding, the one before the last, is half an fp16 step of a weight, and 2^-25
-// at least: the largest is 2^7 to 2^15, so a key's share of the values is off by
+// at least: the largest is 2^7 to 2^11, so a key's share of the values is off by
 // 2^-11 of itself or 2^-32 of the largest share, whichever is more.
 //
 // The G query heads of a kv head and the query rows share its keys: they are
@@ -46,10 +46,14 @@ namespace {
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-// log2 of a weight where the reference is set, and of the largest that leaves it
-// (fp16 holds 2^15): the lower the reference, the more of a long tail of small
-// weights fp16 holds (largest weights of 1 lost tails of 2^-25 a key altogether).
-constexpr float kSet = 7.f, kMost = 15.f;
+// log2 of a weight where the reference is set, and of the largest that leaves it:
+// the lower the reference, the more of a long tail of small weights fp16 holds
+// (largest weights of 1 lost tails of 2^-25 a key altogether).  What is left up to
+// fp16's 2^16 is for scores so large that fp32 rounds them: PromptTile's exponents
+// are off by up to 4 where y is below 2^27, and by 8 below 2^28, where scores are 16
+// apart and the reference moves with each.  (Compared as a difference, which fp32
+// holds where the sum of the reference and kMost would be rounded.)
+constexpr float kSet = 7.f, kMost = 11.f;
 constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
 constexpr int kMaxPages = kSegment / 16;   // segments begin on a block of 64 tokens
 constexpr int kBlock = 64;                 // tokens of a unit of work
@@ -305,8 +309,8 @@ struct RowTile {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
                 mx = over_groups(mx, [](float u, float v) { return fmaxf(u, v); });
-                // the reference follows the maximum only when a weight would pass 2^15
-                if (__any(mx > m + kMost)) {
+                // the reference follows the maximum only when a weight would pass 2^kMost
+                if (__any(mx - m > kMost)) {
                     const float m_new = fmaxf(m, mx - kSet);
                     const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                     l *= alpha;
@@ -587,7 +591,7 @@ struct PromptTile {
                         swap32(p, q);
                         mx = fmaxf(p, q);
                     }
-                    if (__any(mx > m + kMost)) {  // as in RowTile
+                    if (__any(mx - m > kMost)) {  // as in RowTile
                         const float m_new = fmaxf(m, mx - kSet);
                         const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
                         l *= alpha;

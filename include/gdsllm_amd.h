@@ -493,7 +493,8 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * block's value scale is rounded to fp16 before the product with the codes (off
  * by 2^-11 of itself or 2^-32 of the largest).  scale and the cache's scales must
  * be positive, a request's value scales within 2^80 of each other (kv_append's
- * are within 2^42); blocks outside the cache have no weight.  What the cache holds
+ * are within 2^42), scores (scale * q.k) below 2^27; blocks outside the cache have no
+ * weight.  What the cache holds
  * behind a request's tokens is not read as a number.  A NaN among its values (e4m3
  * only) also reaches rows of its request that stand before it in the same call.
  * tokens * q_heads <= 2^30.

@@ -427,3 +427,38 @@ def test_rows_before_the_first_request(gpu, lens, new, max_len):
     out = torch.full_like(got, 7.0)
     p.run(max_len=max_len, output=out)
     assert bool((out[rest.to(gpu)] == 7).all()) and torch.equal(out[~rest.to(gpu)], got[~rest.to(gpu)])
+
+
+@pytest.mark.parametrize("power", [20, 23, 24, 25, 26])
+@pytest.mark.parametrize("lens,new", [([700], [1]), ([3000], [1]), ([700], [150]), ([2100], [40])],
+                         ids=["decode", "decode_shared", "prompt", "prompt_shared"])
+def test_large_scores(gpu, power, lens, new):
+    """Scores of 2^power, where fp32 tells neighbours apart by up to 8, that rise a little from one block of 64 tokens to
+    the next and then by more than any weight's range: results are means of the values, so no larger than the largest,
+    and where one token is far ahead they are its values.  Half an fp16 step for the weight in the product with the
+    values (the sum has it unrounded), half a step for the result, 2^-20 for fp32 sums and quotients."""
+    heads, bs = 8, 64
+    p = Problem(gpu, "int8", 128, 2 * heads, heads, bs, lens, new, 2500, spread=0.0)
+    n, step = lens[0], torch.arange(heads)
+    codes = torch.zeros(p.codes.shape)
+    codes[0, ..., 0] = 100
+    for i, page in enumerate(p.tables[0].tolist()):
+        codes[0, page, :, :, 1] = i % 16
+    codes[1] = p.codes[1].float()
+    codes[0, p.tables[0, n // 2 // bs], :, n // 2 % bs, 2] = 127
+    p.codes = codes.to(torch.int8)
+    p.scales[0] = 16.0
+    p.scales[1] = torch.exp2(0.37 * step - 6)
+    p.scale = 1.0
+    p.q.zero_()
+    p.q[..., 0] = 2.0 ** power / 1600
+    p.q[..., 1] = (0.05 + 0.04 * torch.arange(2 * heads)).half()  # 1 to 16 in log2 from block to block
+    got = p.run().cpu().double()
+    top = 127 * p.scales[1, 0].double().repeat_interleave(2)[None, :, None]
+    assert bool((got.abs() <= top * (1 + 2.0 ** -9)).all())
+    p.q[..., 2] = 1000.0
+    got = p.run().cpu().double()
+    page, at = int(p.tables[0, n // 2 // bs]), n // 2 % bs
+    want = (p.codes[1, page, :, at].double() * p.scales[1, page].double()[:, None]).repeat_interleave(2, 0)
+    seen = torch.arange(new[0]) + n - new[0] >= n // 2
+    assert bool(((got[seen] - want).abs() <= (2.0 ** -10 + 2.0 ** -20) * want.abs() + 2.0 ** -25).all()) and bool(seen.any())
