@@ -28,7 +28,7 @@
 //    then three tiles of codes to a wave.
 //  * Prompts are bound by vector work beside the matrix cores (by counters, softmax
 //    and the codes' conversion take 40% of a SIMD's cycles, its matrix core 35%):
-//    4096 tokens of 32 heads 171 us, 800 TFLOP/s of a large product's 1060; 4 chunks
+//    4096 tokens of 32 heads 174 us, 790 TFLOP/s of a large product's 1060; 4 chunks
 //    of 300 tokens with up to 5000 held 160 us, 515 TFLOP/s: 448 tiles of unequal
 //    length are 1.75 to a compute unit.  Even shares of their keys take 257 us, 92 of
 //    them in attend_join, which gives each of 57000 rows, most of two parts,
