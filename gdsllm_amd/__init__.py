@@ -40,6 +40,15 @@ class KvCache8(ctypes.Structure):
     ]
 
 
+class KvCache4(ctypes.Structure):
+    """gdsllm_kv_cache4 (include/gdsllm_amd.h)."""
+
+    _fields_ = [
+        ("k", _c_vp), ("v", _c_vp), ("k_affine", _c_vp), ("v_affine", _c_vp), ("num_blocks", _c_i64),
+        ("kv_heads", _c_i64), ("block_size", _c_i64), ("head_dim", _c_i64), ("group_size", _c_i64),
+    ]
+
+
 # name -> (restype, argtypes); must match include/gdsllm_amd.h
 SIGNATURES = {
     "gdsllm_last_error": (ctypes.c_char_p, []),
@@ -93,6 +102,11 @@ SIGNATURES = {
     "gdsllm_kv_append": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
     "gdsllm_kv_attention_workspace_size": (ctypes.c_size_t, [_c_i64] * 6),
     "gdsllm_kv_attention": (ctypes.c_int, [ctypes.POINTER(KvCache8), _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_size_t, _c_vp]),
+    "gdsllm_rope": (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64] * 2 + [_c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, ctypes.c_int, _c_vp]),
+    "gdsllm_kv4_append": (ctypes.c_int, [ctypes.POINTER(KvCache4), _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, ctypes.c_int, _c_vp]),
+    "gdsllm_kv4_values": (ctypes.c_int, [ctypes.POINTER(KvCache4), _c_vp, _c_i64, _c_vp, _c_vp, _c_vp]),
+    "gdsllm_kv4_attention_workspace_size": (ctypes.c_size_t, [_c_i64] * 6),
+    "gdsllm_kv4_attention": (ctypes.c_int, [ctypes.POINTER(KvCache4), _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_size_t, _c_vp]),
     "gdsllm_sample_tokens": (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_i64, _c_i64] + [_c_vp] * 7),
     "gdsllm_read_stream": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, ctypes.c_uint32, _c_vp, _c_vp]),
     "gdsllm_empty_launch": (ctypes.c_int, [_c_i64, _c_vp]),

@@ -39,10 +39,11 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
-# Flags of single sources.  kv_attention.hip: accumulators of matrix instructions
-# in ordinary registers, which its running maximum rescales (in accumulation
+# Flags of single sources.  kv_attention.hip, kv4_attention.hip: accumulators of matrix instructions
+# in ordinary registers, which their running maximum rescales (in accumulation
 # registers every rescaling moves them there and back).
-SOURCE_FLAGS = {"kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+SOURCE_FLAGS = {"kv_attention.hip": _VGPR_FORM, "kv4_attention.hip": _VGPR_FORM}
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

@@ -1032,39 +1032,194 @@ py::object kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torc
     return has_q ? py::cast(out) : py::none();
 }
 
+// What an attention call over a paged cache brings besides the cache.
+struct AttentionRows {
+    torch::Tensor q, lens, starts, out;
+    int64_t requests, tokens, heads, most_new, most_len;
+    AttentionRows(const torch::Tensor& q_in, const torch::Tensor& tables, const torch::Tensor& lens_in,
+                  const torch::Tensor& starts_in, const c10::optional<torch::Tensor>& output, int dev, int64_t dim,
+                  int64_t block_size, int64_t max_new, int64_t max_len, const char* where) {
+        q = head_rows(q_in, dev, 0, dim, "q", where);
+        requests = lens_in.numel(), tokens = q.size(0), heads = q.size(1);
+        lens = flat(lens_in, torch::kInt32, dev, requests, "lens", where);
+        starts = flat(starts_in, torch::kInt32, dev, requests + 1, "starts", where);
+        check_tables(tables, dev, requests, where);
+        if (output.has_value()) {
+            out = *output;
+            check_on(out, torch::kFloat16, dev, "output", where);
+            if (!out.sizes().equals(q.sizes()) || out.stride(2) != 1 || (heads > 1 && out.stride(1) != dim) ||
+                (tokens > 1 && out.stride(0) < heads * dim))
+                throw std::runtime_error(std::string(where) + ": output must have q's shape with contiguous rows");
+        } else {
+            out = torch::empty(q.sizes(), q.options());
+        }
+        const int64_t held = tables.size(1) * block_size;
+        most_new = max_new > 0 ? std::min(max_new, tokens) : tokens;
+        most_len = max_len > 0 ? std::min(max_len, held) : held;
+    }
+    torch::Tensor workspace(size_t bytes) const {
+        torch::Tensor ws;
+        if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+        return ws;
+    }
+};
+
 torch::Tensor kv_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
                            torch::Tensor v_scale, torch::Tensor block_tables, torch::Tensor lens, torch::Tensor starts,
                            double scale, int64_t max_new, int64_t max_len, c10::optional<torch::Tensor> output) {
     const char* where = "kv_attention";
     const gdsllm_kv_cache8 c = kv_cache_of(k_cache, v_cache, k_scale, v_scale, where);
     const int dev = k_cache.get_device();
-    torch::Tensor qr = head_rows(q, dev, 0, c.head_dim, "q", where);
-    const int64_t n = lens.numel(), tokens = qr.size(0), heads = qr.size(1);
-    torch::Tensor l = flat(lens, torch::kInt32, dev, n, "lens", where);
-    torch::Tensor st = flat(starts, torch::kInt32, dev, n + 1, "starts", where);
-    check_tables(block_tables, dev, n, where);
-    torch::Tensor out;
-    if (output.has_value()) {
-        out = *output;
-        check_on(out, torch::kFloat16, dev, "output", where);
-        if (!out.sizes().equals(qr.sizes()) || out.stride(2) != 1 || (heads > 1 && out.stride(1) != c.head_dim) ||
-            (tokens > 1 && out.stride(0) < heads * c.head_dim))
-            throw std::runtime_error("kv_attention: output must have q's shape with contiguous rows");
-    } else {
+    const AttentionRows r(q, block_tables, lens, starts, output, dev, c.head_dim, c.block_size, max_new, max_len, where);
+    torch::Tensor ws = r.workspace(
+        gdsllm_kv_attention_workspace_size(r.requests, r.heads, c.kv_heads, c.head_dim, r.most_new, r.most_len));
+    check(gdsllm_kv_attention(&c, r.q.data_ptr(), row_stride(r.q), r.out.data_ptr(), row_stride(r.out), r.tokens, r.heads,
+                              block_tables.data_ptr<int32_t>(), block_tables.size(1), table_stride(block_tables),
+                              r.lens.data_ptr<int32_t>(), r.starts.data_ptr<int32_t>(), r.requests, static_cast<float>(scale),
+                              max_new, max_len, output.has_value() ? 0 : 1, ws.defined() ? ws.data_ptr() : nullptr,
+                              ws.defined() ? ws.numel() : 0, OnDevice(dev).stream()),
+          where);
+    return r.out;
+}
+
+// ---- 4-bit KV cache ----------------------------------------------------------------
+
+// cos and sin [positions, rotary / 2] fp32 and positions int32 [tokens].
+struct Rotation {
+    torch::Tensor positions, cos, sin;
+    int64_t rotary = 0, max_pos = 0;
+    Rotation() = default;
+    Rotation(const torch::Tensor& p, const torch::Tensor& c, const torch::Tensor& s, int device, int64_t tokens, const char* where) {
+        positions = flat(p, torch::kInt32, device, tokens, "positions", where);
+        check_on(c, torch::kFloat32, device, "cos", where);
+        if (c.dim() != 2) throw std::runtime_error(std::string(where) + ": cos must be [positions, rotary / 2]");
+        cos = c.contiguous();
+        sin = flat(s, torch::kFloat32, device, cos.numel(), "sin", where);
+        if (!s.sizes().equals(c.sizes())) throw std::runtime_error(std::string(where) + ": cos and sin differ in shape");
+        max_pos = cos.size(0);
+        rotary = 2 * cos.size(1);
+    }
+    const int32_t* positions_ptr() const { return positions.defined() ? positions.data_ptr<int32_t>() : nullptr; }
+    const float* cos_ptr() const { return cos.defined() ? cos.data_ptr<float>() : nullptr; }
+    const float* sin_ptr() const { return sin.defined() ? sin.data_ptr<float>() : nullptr; }
+};
+
+// Heads [tokens, heads, dim] fp16 to rotate: as they are where rows are
+// contiguous and apart, else a copy (an error where they are rotated in place).
+torch::Tensor rope_rows(const torch::Tensor& t, int device, int64_t tokens, int64_t dim, bool inplace, const char* what) {
+    check_on(t, torch::kFloat16, device, what, "rope");
+    if (t.dim() != 3 || t.size(0) != tokens || t.size(2) != dim)
+        throw std::runtime_error(std::string("rope: ") + what + " must be [" + std::to_string(tokens) + ", heads, " +
+                                 std::to_string(dim) + "]");
+    if (t.numel() == 0 || ((dim == 1 || t.stride(2) == 1) && (t.size(1) == 1 || t.stride(1) == dim) &&
+                           (tokens == 1 || t.stride(0) >= t.size(1) * dim)))
+        return t;
+    if (inplace) throw std::runtime_error(std::string("rope: ") + what + " must have contiguous rows to be rotated in place");
+    return t.contiguous();
+}
+
+py::tuple rope(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions, torch::Tensor cos, torch::Tensor sin,
+               bool neighbours, bool inplace) {
+    if (!q.is_cuda() || q.dim() != 3) throw std::runtime_error("rope: q must be a GPU tensor [tokens, heads, dim]");
+    const int dev = q.get_device();
+    const int64_t n = q.size(0), dim = q.size(2);
+    torch::Tensor qr = rope_rows(q, dev, n, dim, inplace, "q"), kr;
+    if (k.has_value()) kr = rope_rows(*k, dev, n, dim, inplace, "k");
+    const Rotation r(positions, cos, sin, dev, n, "rope");
+    const bool has_k = kr.defined() && kr.size(1) > 0;
+    torch::Tensor qo = inplace ? qr : torch::empty(qr.sizes(), qr.options()), ko;
+    if (kr.defined()) ko = inplace ? kr : torch::empty(kr.sizes(), kr.options());
+    if (qr.size(1) == 0) throw std::runtime_error("rope: q has no heads");
+    check(gdsllm_rope(qr.data_ptr(), row_stride(qr), qo.data_ptr(), row_stride(qo), qr.size(1), has_k ? kr.data_ptr() : nullptr,
+                      has_k ? row_stride(kr) : 0, has_k ? ko.data_ptr() : nullptr, has_k ? row_stride(ko) : 0,
+                      has_k ? kr.size(1) : 0, dim, n, r.positions_ptr(), r.cos_ptr(), r.sin_ptr(), r.rotary, r.max_pos,
+                      neighbours ? 1 : 0, OnDevice(dev).stream()),
+          "rope");
+    return py::make_tuple(qo, ko.defined() ? py::cast(ko) : py::none());
+}
+
+gdsllm_kv_cache4 kv4_cache_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ka,
+                              const torch::Tensor& va, const char* where) {
+    if (!k.is_cuda() || k.dim() != 4 || !k.is_contiguous() || k.scalar_type() != torch::kUInt8)
+        throw std::runtime_error(std::string(where) + ": k_cache must be a contiguous uint8 GPU tensor "
+                                 "[blocks, kv_heads, block_size, head_dim / 2]");
+    const int dev = k.get_device();
+    check_on(v, torch::kUInt8, dev, "v_cache", where);
+    if (!v.sizes().equals(k.sizes()) || !v.is_contiguous())
+        throw std::runtime_error(std::string(where) + ": v_cache must have k_cache's shape and be contiguous");
+    for (const auto* t : {&ka, &va}) {
+        check_on(*t, torch::kFloat16, dev, "the affine pairs", where);
+        if (t->dim() != 5 || t->size(0) != k.size(0) || t->size(1) != k.size(1) || t->size(2) < 1 || t->size(3) != k.size(2) ||
+            t->size(4) != 2 || !t->is_contiguous() || !t->sizes().equals(ka.sizes()) || 2 * k.size(3) % t->size(2))
+            throw std::runtime_error(std::string(where) +
+                                     ": affine pairs must be contiguous [blocks, kv_heads, groups, block_size, 2]");
+    }
+    return {k.data_ptr(), v.data_ptr(), ka.data_ptr(), va.data_ptr(), k.size(0), k.size(1), k.size(2), 2 * k.size(3),
+            2 * k.size(3) / ka.size(2)};
+}
+
+py::object kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
+                      torch::Tensor k_affine, torch::Tensor v_affine, c10::optional<torch::Tensor> q,
+                      c10::optional<torch::Tensor> positions, c10::optional<torch::Tensor> cos,
+                      c10::optional<torch::Tensor> sin, bool neighbours) {
+    const char* where = "kv4_append";
+    const gdsllm_kv_cache4 c = kv4_cache_of(k_cache, v_cache, k_affine, v_affine, where);
+    const int dev = k_cache.get_device();
+    torch::Tensor kr = head_rows(k, dev, c.kv_heads, c.head_dim, "k", where);
+    torch::Tensor vr = head_rows(v, dev, c.kv_heads, c.head_dim, "v", where);
+    const int64_t n = kr.size(0);
+    if (vr.size(0) != n) throw std::runtime_error("kv4_append: k and v differ in tokens");
+    torch::Tensor s = flat(slots, torch::kInt32, dev, n, "slots", where);
+    if (cos.has_value() != sin.has_value()) throw std::runtime_error("kv4_append: cos and sin come together");
+    if (q.has_value() && !cos.has_value()) throw std::runtime_error("kv4_append: q is given without cos and sin");
+    Rotation r;
+    if (cos.has_value()) {
+        if (!positions.has_value()) throw std::runtime_error("kv4_append: a rotation needs positions");
+        r = Rotation(*positions, *cos, *sin, dev, n, where);
+    }
+    torch::Tensor qr, out;
+    if (q.has_value()) {
+        qr = head_rows(*q, dev, 0, c.head_dim, "q", where);
+        if (qr.size(0) != n) throw std::runtime_error("kv4_append: q and k differ in tokens");
         out = torch::empty(qr.sizes(), qr.options());
     }
-    const size_t bytes = gdsllm_kv_attention_workspace_size(n, heads, c.kv_heads, c.head_dim,
-                                                            max_new > 0 ? std::min(max_new, tokens) : tokens,
-                                                            max_len > 0 ? std::min(max_len, block_tables.size(1) * c.block_size)
-                                                                        : block_tables.size(1) * c.block_size);
-    torch::Tensor ws;
-    if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, qr.options().dtype(torch::kUInt8));
-    check(gdsllm_kv_attention(&c, qr.data_ptr(), row_stride(qr), out.data_ptr(), row_stride(out), tokens, heads,
-                              block_tables.data_ptr<int32_t>(), block_tables.size(1), table_stride(block_tables),
-                              l.data_ptr<int32_t>(), st.data_ptr<int32_t>(), n, static_cast<float>(scale), max_new, max_len,
-                              output.has_value() ? 0 : 1, bytes > 0 ? ws.data_ptr() : nullptr, bytes, OnDevice(dev).stream()),
+    const bool has_q = qr.defined();
+    check(gdsllm_kv4_append(&c, kr.data_ptr(), row_stride(kr), vr.data_ptr(), row_stride(vr), s.data_ptr<int32_t>(), n,
+                            has_q ? qr.data_ptr() : nullptr, has_q ? row_stride(qr) : 0, has_q ? out.data_ptr() : nullptr,
+                            has_q ? qr.size(1) : 0, r.positions_ptr(), r.cos_ptr(), r.sin_ptr(), r.rotary, r.max_pos,
+                            neighbours ? 1 : 0, OnDevice(dev).stream()),
           where);
-    return out;
+    return has_q ? py::cast(out) : py::none();
+}
+
+py::tuple kv4_values(torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_affine,
+                     torch::Tensor v_affine) {
+    const char* where = "kv4_values";
+    const gdsllm_kv_cache4 c = kv4_cache_of(k_cache, v_cache, k_affine, v_affine, where);
+    const int dev = k_cache.get_device();
+    torch::Tensor s = flat(slots, torch::kInt32, dev, slots.numel(), "slots", where);
+    const std::vector<int64_t> shape = {s.numel(), c.kv_heads, c.head_dim};
+    torch::Tensor k = torch::empty(shape, k_affine.options()), v = torch::empty(shape, k_affine.options());
+    check(gdsllm_kv4_values(&c, s.data_ptr<int32_t>(), s.numel(), k.data_ptr(), v.data_ptr(), OnDevice(dev).stream()), where);
+    return py::make_tuple(k, v);
+}
+
+torch::Tensor kv4_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_affine,
+                            torch::Tensor v_affine, torch::Tensor block_tables, torch::Tensor lens, torch::Tensor starts,
+                            double scale, int64_t max_new, int64_t max_len, c10::optional<torch::Tensor> output) {
+    const char* where = "kv4_attention";
+    const gdsllm_kv_cache4 c = kv4_cache_of(k_cache, v_cache, k_affine, v_affine, where);
+    const int dev = k_cache.get_device();
+    const AttentionRows r(q, block_tables, lens, starts, output, dev, c.head_dim, c.block_size, max_new, max_len, where);
+    torch::Tensor ws = r.workspace(
+        gdsllm_kv4_attention_workspace_size(r.requests, r.heads, c.kv_heads, c.head_dim, r.most_new, r.most_len));
+    check(gdsllm_kv4_attention(&c, r.q.data_ptr(), row_stride(r.q), r.out.data_ptr(), row_stride(r.out), r.tokens, r.heads,
+                               block_tables.data_ptr<int32_t>(), block_tables.size(1), table_stride(block_tables),
+                               r.lens.data_ptr<int32_t>(), r.starts.data_ptr<int32_t>(), r.requests, static_cast<float>(scale),
+                               max_new, max_len, output.has_value() ? 0 : 1, ws.defined() ? ws.data_ptr() : nullptr,
+                               ws.defined() ? ws.numel() : 0, OnDevice(dev).stream()),
+          where);
+    return r.out;
 }
 
 torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u, c10::optional<torch::Tensor> temperature,
@@ -1197,6 +1352,22 @@ PYBIND11_MODULE(gds_io_ext, m) {
           py::arg("sin") = py::none());
     m.def("kv_attention", &kv_attention, "Causal attention of q [T, heads, dim] over the 8-bit cache.", py::arg("q"),
           py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_tables"),
+          py::arg("lens"), py::arg("starts"), py::arg("scale"), py::arg("max_new") = 0, py::arg("max_len") = 0,
+          py::arg("output") = py::none());
+    m.def("rope", &rope,
+          "q and k [T, heads, dim] rotated by their positions: (q, k); k may be None. neighbours: channels 2i and 2i + 1 "
+          "turn together, else i and i + rotary / 2.",
+          py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("cos"), py::arg("sin"), py::arg("neighbours") = false,
+          py::arg("inplace") = false);
+    m.def("kv4_append", &kv4_append,
+          "Rotate k (and q), write k and v to their slots of the 4-bit cache; returns the rotated q (None without q).",
+          py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_affine"),
+          py::arg("v_affine"), py::arg("q") = py::none(), py::arg("positions") = py::none(), py::arg("cos") = py::none(),
+          py::arg("sin") = py::none(), py::arg("neighbours") = false);
+    m.def("kv4_values", &kv4_values, "(k, v) fp16 [slots, kv_heads, head_dim] that the 4-bit cache holds; zeros outside it.",
+          py::arg("slots"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_affine"), py::arg("v_affine"));
+    m.def("kv4_attention", &kv4_attention, "Causal attention of q [T, heads, dim] over the 4-bit cache.", py::arg("q"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_affine"), py::arg("v_affine"), py::arg("block_tables"),
           py::arg("lens"), py::arg("starts"), py::arg("scale"), py::arg("max_new") = 0, py::arg("max_len") = 0,
           py::arg("output") = py::none());
     m.def("sample_tokens", &sample_tokens,

@@ -19,7 +19,7 @@ The decode step's fused launches are exposed as the reference's own units:
 qkv_projections (the three dequant_linear calls of runtime/llama.py:212-214 in
 one launch) and mlp (runtime/llama.py:247-256: gate, up and F.silu(gate)*up in
 one launch, then down).  cached_attention is the attention block between them
-(runtime/llama.py:200-246) over an 8-bit cache.
+(runtime/llama.py:200-246) over an 8- or 4-bit cache.
 """
 
 from __future__ import annotations
@@ -141,13 +141,15 @@ def packed_rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def cached_attention(x: torch.Tensor, weights: Dict, cache, layer: int, cos: torch.Tensor, sin: torch.Tensor,
-                     scale: Optional[float] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The attention block of runtime/llama.py:200-246 over an 8-bit cache: q/k/v
-    projections, rotation and append, attention, o_proj.
+                     scale: Optional[float] = None, scratch: Optional[torch.Tensor] = None,
+                     neighbours: bool = False) -> torch.Tensor:
+    """The attention block of runtime/llama.py:200-246 over an 8- or 4-bit cache:
+    q/k/v projections, rotation and append, attention, o_proj.
 
     x fp16 [T, hidden]: the step's rows, one request's after another's as
-    cache.begin_step laid them out (a KVCache8; T its max_tokens); cos, sin from
-    rope_table.  Returns [T, hidden].  Inference only: x must need no gradient.
+    cache.begin_step laid them out (a KVCache8 or KVCache4; T its max_tokens);
+    cos, sin from rope_table; neighbours: the checkpoint turns channels 2i and 2i +
+    1 together.  Returns [T, hidden].  Inference only: x must need no gradient.
     """
     if x.dim() != 2 or cache.slots is None or x.shape[0] != cache.slots.numel():
         raise ValueError("cached_attention: x must be [T, hidden] with the T rows of cache.begin_step")
@@ -157,7 +159,8 @@ def cached_attention(x: torch.Tensor, weights: Dict, cache, layer: int, cos: tor
     if T == 0:
         return x
     q, k, v = (p.reshape(T, -1, D) for p in qkv_projections(packed_rows(x), weights, scratch))
-    o = cache.attend(layer, cache.append(layer, k, v, q, cos, sin), scale)
+    pairs = {"neighbours": True} if neighbours else {}
+    o = cache.attend(layer, cache.append(layer, k, v, q, cos, sin, **pairs), scale)
     return dequant_linear(packed_rows(o.reshape(T, -1)), weights, "self_attn.o_proj", scratch).reshape(T, -1)
 
 

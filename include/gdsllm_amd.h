@@ -514,6 +514,77 @@ int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ld
                         int64_t max_new, int64_t max_len, int zero_other, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ------------------------------------------------------ 4-bit KV cache --
+ * The same step over a cache at the width of 4-bit weights.  No counterpart in
+ * the reference.
+ *
+ * One layer's cache: blocks as above, codes [num_blocks][kv_heads][block_size]
+ * [head_dim / 2] bytes (channel 2i in the low four bits of byte i, 2i + 1 in the
+ * high ones) and, for each token and group of group_size (32, 64 or 128, at most
+ * head_dim) channels, a pair of fp16 (scale, bias),
+ * [num_blocks][kv_heads][head_dim / group_size][block_size][2]:
+ * element = fp16(code * scale + bias), the affine format of the 4-bit weights.  */
+typedef struct gdsllm_kv_cache4 {
+    void* k;
+    void* v;
+    void* k_affine;
+    void* v_affine;
+    int64_t num_blocks;
+    int64_t kv_heads;
+    int64_t block_size;
+    int64_t head_dim;
+    int64_t group_size;
+} gdsllm_kv_cache4;
+
+/* q [tokens][q_heads * head_dim] and k [tokens][k_heads * head_dim] (fp16, rows
+ * ldq, ldk apart; k_heads 0: no k) turned by their tokens' positions into q_out
+ * and k_out: pair i of a head, channels i and i + rotary/2 (neighbours 0) or 2i and
+ * 2i + 1 (neighbours 1), by the angle whose cosine and sine are cos, sin
+ * [max_pos][rotary/2] at positions[t], in 64 bits, rounded to fp32 and then to
+ * fp16; the channels past `rotary` are copied.  A row whose position lies outside
+ * [0, max_pos) is zero.  head_dim in [2, 1024], rotary even.  q_out may be q with the same
+ * stride, k_out k (in place); otherwise the outputs overlap neither input.  Fast
+ * for head_dim % 8 == 0, rotary % 16 == 0 (neighbours: % 8) and everything on the
+ * 16-byte grid.  Replaces the rotation of runtime/llama.py:60-103.             */
+int gdsllm_rope(const void* q, int64_t ldq, void* q_out, int64_t ldqo, int64_t q_heads, const void* k, int64_t ldk,
+                void* k_out, int64_t ldko, int64_t k_heads, int64_t head_dim, int64_t tokens,
+                const int32_t* positions, const float* cos, const float* sin, int64_t rotary, int64_t max_pos,
+                int neighbours, void* stream);
+
+/* gdsllm_kv_append's arguments over the 4-bit cache, with both ways of pairing
+ * channels (neighbours as in gdsllm_rope).  Each token, head and group for itself:
+ * bias = the smallest of its finite values, scale = their range / 15 rounded to fp16
+ * (to the next smaller fp16 value where 15 * scale + bias would not round to a
+ * finite one), code = (x - bias) / scale to nearest even, in [0, 15]; +inf is 15,
+ * -inf and NaN are 0; no finite value: all zero.  Other tokens of a block stay
+ * as they are.  A row whose slot lies outside the cache (-1) or whose position
+ * outside [0, max_pos) is padding: not written, zeros in q_out.  Of several rows with one
+ * slot the last counts, where the tokens of a block stand in consecutive rows (as
+ * kv_assign numbers them, no padding between them).                          */
+int gdsllm_kv4_append(const gdsllm_kv_cache4* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                      const int32_t* slots, int64_t tokens, const void* q, int64_t ldq, void* q_out, int64_t q_heads,
+                      const int32_t* positions, const float* cos, const float* sin, int64_t rotary, int64_t max_pos,
+                      int neighbours, void* stream);
+
+/* The keys and values that the cache holds in `rows` slots, fp16 k and v
+ * [rows][kv_heads][head_dim]: a request handed to another cache or another server.
+ * A slot outside the cache gives zeros.  16-byte aligned k and v.             */
+int gdsllm_kv4_values(const gdsllm_kv_cache4* cache, const int32_t* slots, int64_t rows, void* k, void* v,
+                      void* stream);
+
+/* gdsllm_kv_attention over the 4-bit cache, with its arguments and workspace
+ * rules.  Products of fp16 q and elements in fp32, softmax in fp32, weights rounded
+ * to fp16 before the product with the values (off by 2^-11 of themselves or 2^-32
+ * of the largest).  scale must be positive; blocks outside the cache have no weight; what
+ * the cache holds behind a request's tokens is not read as a number.          */
+size_t gdsllm_kv4_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t max_new, int64_t max_len);
+int gdsllm_kv4_attention(const gdsllm_kv_cache4* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
+                         int64_t tokens, int64_t q_heads, const int32_t* block_tables, int64_t table_width,
+                         int64_t ld_table, const int32_t* lens, const int32_t* starts, int64_t requests, float scale,
+                         int64_t max_new, int64_t max_len, int zero_other, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* -------------------------------------------------------------- sampling --
  * One token for each row of logits [rows][vocab] (fp16 or fp32: bits 16 or 32;
  * rows ld apart; vocab <= 2^20, rows < 2^22) from the uniform number u[row] in [0, 1).
