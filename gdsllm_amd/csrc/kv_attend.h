@@ -116,22 +116,22 @@ __global__ __launch_bounds__(T::kThreads) void attend_whole(typename T::Args a) 
 // The work as one line of blocks: request after request, in each its row tiles,
 // kv heads and blocks of tokens, innermost last; `groups` workgroups take even
 // shares of it, so none waits for a long sequence.  Each sums the requests'
-// work for itself, 256 a step, and looks up where its share begins.  A sequence
+// work for itself, a request to a thread a step, and looks up where its share begins.  A sequence
 // that lies in several shares leaves a part in each: a workgroup has at most
 // two, the one its share begins with and the one it ends in.
 
 template <class T>
-__global__ __launch_bounds__(256, T::kPerCu) void attend_shared(typename T::Args a) {
-    static_assert(T::kThreads == 256, "the sums over requests go 256 a step");
+__global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void attend_shared(typename T::Args a) {
+    constexpr int N = T::kThreads, NW = N / 64;
     extern __shared__ __attribute__((aligned(16))) char raw[];
     typename T::Lds& s = *reinterpret_cast<typename T::Lds*>(raw);
-    __shared__ int s_part[4], s_request, s_begin;
+    __shared__ int s_part[NW], s_request, s_begin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wg = blockIdx.x;
     zero_other_rows(a, T::kD);
     int total = 0, share = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int carry = 0;
-        for (int b0 = 0; b0 < a.requests; b0 += 256) {
+        for (int b0 = 0; b0 < a.requests; b0 += N) {
             const int b = b0 + tid, w = b < a.requests ? Rows<T::kRows>(a, b).work(a) : 0;
             int upto = wave_scan(w);
             __syncthreads();
@@ -139,15 +139,16 @@ __global__ __launch_bounds__(256, T::kPerCu) void attend_shared(typename T::Args
             __syncthreads();
             for (int i = 0; i < wave; ++i) upto += s_part[i];
             const int begin = carry + upto - w;
-            carry += s_part[0] + s_part[1] + s_part[2] + s_part[3];
-            if (a.requests <= 256) {  // one step: the sum is all here
+#pragma unroll
+            for (int i = 0; i < NW; ++i) carry += s_part[i];
+            if (a.requests <= N) {  // one step: the sum is all here
                 total = carry;
                 share = max((total + a.groups - 1) / a.groups, 4);
             }
             const int at = wg * share;
             if (share > 0 && w > 0 && begin <= at && at < begin + w) s_request = b, s_begin = begin;
         }
-        if (a.requests <= 256) break;
+        if (a.requests <= N) break;
         total = carry;
         share = max((total + a.groups - 1) / a.groups, 4);
     }
@@ -316,15 +317,15 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
     p->bytes = part_bytes(p->groups, p->rows, p->sequences, head_dim);
 }
 
-// Workgroups that the device holds at once, of 16-row and of 128-row tiles.
+// Workgroups that the device holds at once, of 16-row tiles and of many rows': a
+// compute unit holds `many` of those.
 int64_t resident_few(int64_t head_dim) { return per_cu(head_dim) * static_cast<int64_t>(kCus); }
-int64_t resident_many(int64_t head_dim) { return (head_dim == 256 ? 1 : 2) * static_cast<int64_t>(kCus); }
 
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.  (256 requests
 // of up to 4000 tokens over 8 heads: 218 us whole, 236 shared out; a prompt of 500 tokens
 // behind 1500, 128 tiles: 62 whole, 66 shared out; one of 64 in 32 tiles: 57 and 34.)
-Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
+Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len, int many_per_cu) {
     Plan p;
     const int64_t rows = max_new * (q_heads / kv_heads);
     const bool many = rows > 2 * kFewRows;
@@ -337,10 +338,10 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
                     max_len <= kWholeTokens || sequences >= (max_len <= 4 * kWholeTokens ? 2 : 8) * resident);
     }
     if (many) {
-        const int64_t resident = resident_many(head_dim);
-        // eight waves to a tile (each converts half as much) where that still leaves
+        const int64_t resident = many_per_cu * static_cast<int64_t>(kCus);
+        // 256 rows to a tile (each wave converts half as much) where that still leaves
         // two workgroups to a compute unit, one after the other: 4096 tokens of 32
-        // heads 172 us against 188; 4 chunks of 300 tokens 167 against 161
+        // heads over the 8-bit cache 172 us against 188; 4 chunks of 300 tokens 167 against 161
         const bool wide = head_dim <= 128 && requests * kv_heads * ((rows + 255) / 256) >= resident;
         p.many.rows = wide ? 256 : 128;
         if (p.few.on) p.many.min_rows = kFewRows + 1;
@@ -356,7 +357,8 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
 // whole and needs none, 64 tokens behind as many share their work.  Work is
 // shared out past kWholeTokens alone, by up to 64 rows of fewer than 8 * resident
 // sequences and by 128-row tiles of fewer than resident / 2.
-size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len) {
+size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len,
+                       int many_per_cu) {
     if (max_len <= kWholeTokens) return 0;
     const int64_t rows = max_new * (q_heads / kv_heads), units = (max_len + 255) / 256;
     auto part = [&](int64_t tile, int64_t most, int64_t limit, int64_t resident) {
@@ -364,7 +366,7 @@ size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int6
         return part_bytes(std::min(resident, sequences * units), tile, sequences, head_dim);
     };
     size_t bytes = part(16, std::min<int64_t>(rows, 2 * kFewRows), 8 * resident_few(head_dim), resident_few(head_dim));
-    if (rows > 2 * kFewRows) bytes += part(128, rows, resident_many(head_dim) / 2, resident_many(head_dim));
+    if (rows > 2 * kFewRows) bytes += part(128, rows, many_per_cu * kCus / 2, many_per_cu * kCus);
     return bytes;
 }
 
@@ -389,7 +391,7 @@ int launch_part(typename S::Args a, const Part& p, int64_t blocks, int64_t max_r
     }
     const size_t lds = sizeof(typename S::Lds);
     if (int rc = prepare_lds(reinterpret_cast<const void*>(&attend_shared<S>), lds)) return rc;
-    hipLaunchKernelGGL(attend_shared<S>, dim3(a.groups), dim3(256), lds, s, a);
+    hipLaunchKernelGGL(attend_shared<S>, dim3(a.groups), dim3(S::kThreads), lds, s, a);
     const int rows = static_cast<int>(std::min<int64_t>(S::kRows, std::max<int64_t>(1, max_rows)));
     const dim3 join(per_request * rows, requests);
     // few sequences are long, in many parts each
@@ -417,7 +419,7 @@ template <class Args, class Desc>
 int attend_call(const std::string& n, const Desc* cache, const void* q, int64_t ldq, void* o, int64_t ldo, int64_t tokens,
                 int64_t q_heads, const int32_t* block_tables, int64_t table_width, int64_t ld_table, const int32_t* lens,
                 const int32_t* starts, int64_t requests, float scale, int64_t max_new, int64_t max_len, int zero_other,
-                void* workspace, size_t workspace_bytes, Args& a, AttendCall* call) {
+                void* workspace, size_t workspace_bytes, int many_per_cu, Args& a, AttendCall* call) {
     auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
     const int64_t D = cache->head_dim;
     if (tokens < 0 || tokens > (int64_t(1) << 30)) return bad("bad token count");
@@ -442,7 +444,7 @@ int attend_call(const std::string& n, const Desc* cache, const void* q, int64_t 
     if (max_len == 0 || max_len > most) max_len = most;
     if (!attend_sizes(requests, q_heads, cache->kv_heads, D, max_new, max_len)) return bad("sizes out of range");
     if (requests == 0) return bad("no requests for the tokens");
-    const Plan& p = call->plan = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len);
+    const Plan& p = call->plan = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len, many_per_cu);
     const size_t need = p.bytes();
     if (need > 0 && (!workspace || workspace_bytes < need))
         return bad("workspace of " + std::to_string(need) + " bytes needed, got " + std::to_string(workspace_bytes));

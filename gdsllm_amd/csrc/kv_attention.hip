@@ -41,6 +41,8 @@ namespace gdsllm {
 namespace {
 
 typedef AttendArgs<KvCache> Args8;
+// Workgroups of PromptTile that a compute unit holds at once.
+constexpr int prompts_per_cu(int64_t D) { return D == 256 ? 1 : 2; }
 
 // 16 rows over blocks [block0, block1) of a sequence, by NW waves.  Matrix tiles
 // are 16x16x32 and nothing passes through LDS but the block table and the waves'
@@ -331,7 +333,7 @@ struct RowTile {
 template <bool E4M3, int D, int NW>
 struct PromptTile {
     typedef Args8 Args;
-    static constexpr int kRows = 32 * NW, kThreads = 64 * NW, kD = D, kPerCu = D == 256 ? 1 : 2;
+    static constexpr int kRows = 32 * NW, kThreads = 64 * NW, kD = D, kPerCu = prompts_per_cu(D);
     static constexpr int BN = D == 256 ? 32 : 64;
     static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
     // 16-code chunks of K, and the ones a thread converts (the last threads none where there are fewer)
@@ -593,7 +595,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len);
+    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len, prompts_per_cu(head_dim));
 }
 
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
@@ -605,7 +607,8 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     AttendCall c;
     if (int rc = kv_cache_args(cache, "kv_attention", &a.c)) return rc;
     if (int rc = attend_call("kv_attention", cache, q, ldq, o, ldo, tokens, q_heads, block_tables, table_width, ld_table, lens,
-                             starts, requests, scale, max_new, max_len, zero_other, workspace, workspace_bytes, a, &c))
+                             starts, requests, scale, max_new, max_len, zero_other, workspace, workspace_bytes,
+                             prompts_per_cu(cache->head_dim), a, &c))
         return rc;
     if (c.empty) return ok();
     const int64_t D = cache->head_dim;
