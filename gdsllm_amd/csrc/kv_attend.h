@@ -44,6 +44,7 @@ struct AttendArgs {
     int min_rows, max_rows;  // requests with other numbers of rows are left to another launch
     int tiles;               // row tiles of a request that the grids have
     int groups;              // workgroups that share the work evenly
+    int begin;               // blocks that beginning a sequence counts as
     int zero_other;          // rows of no request are set to zero
 };
 
@@ -51,6 +52,7 @@ struct AttendArgs {
 template <int RT>
 struct Rows {
     int start, n, len, rows;
+    Rows() = default;
     template <class Args>
     __device__ __forceinline__ Rows(const Args& a, int b) {
         const int s0 = a.starts[b], s1 = a.starts[b + 1], held = a.lens[b];
@@ -70,7 +72,7 @@ struct Rows {
     // Blocks of kBlock tokens to each of its sequences (row tile and kv head).
     __device__ __forceinline__ int blocks() const { return max((len + kBlock - 1) / kBlock, 1); }
     template <class Args>
-    __device__ __forceinline__ int work(const Args& a) const { return min(tiles(), a.tiles) * a.c.kv_heads * blocks(); }
+    __device__ __forceinline__ int work(const Args& a) const { return min(tiles(), a.tiles) * a.c.kv_heads * (blocks() + a.begin); }
 };
 
 // f over the values of lanes l % 16 + {0, 16, 32, 48}: every lane gets the result.
@@ -118,7 +120,10 @@ __global__ __launch_bounds__(T::kThreads) void attend_whole(typename T::Args a) 
 // shares of it, so none waits for a long sequence.  Each sums the requests'
 // work for itself, a request to a thread a step, and looks up where its share begins.  A sequence
 // that lies in several shares leaves a part in each: a workgroup has at most
-// two, the one its share begins with and the one it ends in.
+// two, the one its share begins with and the one it ends in.  A sequence counts
+// `begin` blocks more than it has, in front of them: the time it takes to begin one
+// (4 us, four loads one after the other), so that no workgroup has several short
+// ones beside a full share.
 
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void attend_shared(typename T::Args a) {
@@ -126,13 +131,20 @@ __global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void at
     extern __shared__ __attribute__((aligned(16))) char raw[];
     typename T::Lds& s = *reinterpret_cast<typename T::Lds*>(raw);
     __shared__ int s_part[NW], s_request, s_begin;
+    __shared__ Rows<T::kRows> s_rows;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wg = blockIdx.x;
     zero_other_rows(a, T::kD);
     int total = 0, share = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int carry = 0;
         for (int b0 = 0; b0 < a.requests; b0 += N) {
-            const int b = b0 + tid, w = b < a.requests ? Rows<T::kRows>(a, b).work(a) : 0;
+            const int b = b0 + tid;
+            Rows<T::kRows> R;
+            int w = 0;
+            if (b < a.requests) {
+                R = Rows<T::kRows>(a, b);
+                w = R.work(a);
+            }
             int upto = wave_scan(w);
             __syncthreads();
             if (lane == 63) s_part[wave] = upto;
@@ -143,28 +155,34 @@ __global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void at
             for (int i = 0; i < NW; ++i) carry += s_part[i];
             if (a.requests <= N) {  // one step: the sum is all here
                 total = carry;
-                share = max((total + a.groups - 1) / a.groups, 4);
+                share = max((total + a.groups - 1) / a.groups, 4 + a.begin);
             }
             const int at = wg * share;
-            if (share > 0 && w > 0 && begin <= at && at < begin + w) s_request = b, s_begin = begin;
+            if (share > 0 && w > 0 && begin <= at && at < begin + w) s_request = b, s_begin = begin, s_rows = R;
         }
         if (a.requests <= N) break;
         total = carry;
-        share = max((total + a.groups - 1) / a.groups, 4);
+        share = max((total + a.groups - 1) / a.groups, 4 + a.begin);
     }
     __syncthreads();
-    int at = wg * share, b = s_request, begin = s_begin;
-    const int end = min(at + share, total);
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    share = uniform(share);
+    int at = wg * share, b = uniform(s_request), begin = uniform(s_begin);
+    const int end = min(at + share, uniform(total));
     if (at >= end) return;
     bool first = true;
+    Rows<T::kRows> R;
+    R.start = uniform(s_rows.start), R.n = uniform(s_rows.n), R.len = uniform(s_rows.len), R.rows = uniform(s_rows.rows);
     while (at < end) {
-        Rows<T::kRows> R(a, b);
         while (at >= begin + R.work(a)) {
             begin += R.work(a);
             R = Rows<T::kRows>(a, ++b);
         }
-        const int blocks = R.blocks(), sequence = (at - begin) / blocks, block0 = at - begin - sequence * blocks;
-        const int block1 = min(blocks, block0 + end - at);
+        const int blocks = R.blocks(), cost = blocks + a.begin, sequence = (at - begin) / cost;
+        const int from = at - begin - sequence * cost, to = min(cost, from + end - at);
+        const int block0 = max(from - a.begin, 0), block1 = to - a.begin;
+        at += to - from;
+        if (block1 <= 0) break;  // the share ends before the sequence's first block
         const int head = sequence % a.c.kv_heads, tile = sequence / a.c.kv_heads;
         const bool whole = block0 == 0 && block1 == blocks;
         const int slot = 2 * wg + (first ? 0 : 1);
@@ -174,7 +192,6 @@ __global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void at
         T::run(a, s, b, R, tile, head, block0, block1, whole ? -1 : slot, -2);
         if (block0 == 0)  // more rows than the caller said: whole, by whoever begins the tile below
             for (int t = tile + a.tiles; t < R.tiles(); t += a.tiles) T::run(a, s, b, R, t, head, 0, blocks, -1, -2);
-        at += block1 - block0;
         first = false;
     }
 }
@@ -187,7 +204,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerCu * T::kThreads / 256) void at
 // groups' sums meet in LDS in a fixed order.
 template <class Args, int RT, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void attend_join(Args a, int rows) {
-    constexpr int TPR = D / 4, NG = THREADS / TPR, NWV = THREADS / 64, EARLY = 2;
+    constexpr int TPR = D / 4, NG = THREADS / TPR, NWV = THREADS / 64, EARLY = THREADS > 256 ? 8 : 2;
     __shared__ float s_f[THREADS], s_m[NWV], s_l[NWV];
     __shared__ __attribute__((aligned(16))) float4_t s_o[THREADS];
     const int b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
@@ -381,7 +398,9 @@ int launch_part(typename S::Args a, const Part& p, int64_t blocks, int64_t max_r
     a.part_o = reinterpret_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.sums * S::kD);
     a.parts = reinterpret_cast<int2*>(a.part_ml + p.sums);
-    a.groups = p.sequences * blocks < (int64_t(1) << 30) ? p.groups : 0;  // the line of blocks is counted in 32 bits
+    a.groups = p.sequences * (blocks + S::kBegin) < (int64_t(1) << 30) ? p.groups : 0;  // the line of blocks is counted in 32 bits
+    // (of few long sequences each share begins with one anyway)
+    a.begin = 16 * p.sequences >= p.groups ? S::kBegin : 0;
     const unsigned per_request = static_cast<unsigned>(p.tiles) * a.c.kv_heads, requests = a.requests;
     if (a.groups == 0) {
         const size_t lds = sizeof(typename W::Lds);
