@@ -51,6 +51,10 @@ __device__ __forceinline__ uint4 load_nt16(const void* p) {
     const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
     return make_uint4(v.x, v.y, v.z, v.w);
 }
+// 16-byte streaming (non-temporal) global store.
+__device__ __forceinline__ void store_nt16(void* p, const uint4& v) {
+    __builtin_nontemporal_store(u32x4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_t*>(p));
+}
 
 __device__ __forceinline__ float h2f(uint32_t bits16) {
     return static_cast<float>(__builtin_bit_cast(half_t, static_cast<uint16_t>(bits16)));

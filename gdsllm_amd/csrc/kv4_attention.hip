@@ -340,7 +340,7 @@ struct RowTile4 {
 // every other tile, each tile one slot, and add their sums in the end: twice the
 // conversion to a row, half the rows to a workgroup.
 //
-// A prompt of 4096 tokens, 32 heads over 8 of 128 channels: 163 us (four waves that
+// A prompt of 4096 tokens, 32 heads of 128 channels: 163 us (four waves that
 // do all of it in turn, two workgroups to a compute unit: 178), 840 TFLOP/s.  A
 // slot takes 2000 cycles: its 32 matrix instructions 1024 of them, its vector work
 // as many as the slot, 230 instructions for 64 tokens of 32 rows at 5 to 8 cycles.

@@ -96,31 +96,60 @@ __device__ __forceinline__ float over_lanes(float v, int log2, F f) {
 }
 
 // The affine pair (scale, bias) of a group with smallest and largest finite value
-// lo and hi (lo > hi: it has none).
+// lo and hi (lo > hi: it has none).  The quotient by 15 is one product and its
+// remainder's correction: right to the last bit but one, and exact where it has few
+// bits, so that its rounding to fp32 is the quotient's (a difference of fp16
+// values is a whole number of 2^-24 below 2^41: a fifteenth of it that is no
+// middle of two fp32 values is 2^-29 of itself away from one).
 __device__ __forceinline__ uint32_t affine_of(float lo, float hi) {
     if (lo > hi) return 0;
     const double span = static_cast<double>(hi) - static_cast<double>(lo);
-    uint16_t s = f2h_bits(fp32_rounded(static_cast<float>(span / 15.0)));
-    // the largest element must be finite: 15 * s is exact in fp32, and so is the comparison's sum in 64 bits
-    if (15.0 * static_cast<double>(h2f(s)) + static_cast<double>(lo) >= 65520.0) --s;
+    double q = span * (1.0 / 15.0);
+    q = fma(fma(-q, 15.0, span), 1.0 / 15.0, q);
+    uint16_t s = f2h_bits(fp32_rounded(static_cast<float>(q)));
+    // the largest element must be finite: 15 * s is exact in fp32, and so is the sum in
+    // 64 bits (half a step of s is at most 2^-11 of the span: 64 in all)
+    if (hi > 65000.f && 15.0 * static_cast<double>(h2f(s)) + static_cast<double>(lo) >= 65520.0) --s;
     return s | (static_cast<uint32_t>(f2h_bits(lo + 0.f)) << 16);
 }
 
-// round((x - bias) / scale), ties to even, in [0, 15]: a candidate in fp32, put
-// right by its remainder, which is exact in 64 bits.  NaN is 0.
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float inv, float bias) {
-    if (!(fabsf(x) < INFINITY)) return x > 0.f ? 15u : 0u;
-    const double d = static_cast<double>(x) - static_cast<double>(bias), s = scale;
-    float n = __builtin_rintf(static_cast<float>(d) * inv);
-    const double r2 = 2.0 * fma(-static_cast<double>(n), s, d);
-    const bool odd = static_cast<int>(n) & 1;
-    if (r2 > s || (r2 == s && odd)) n += 1.f;
-    else if (r2 < -s || (r2 == -s && odd)) n -= 1.f;
-    return static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f));
+// A dword of codes round((x - bias) / scale), ties to even, in [0, 15], of eight
+// values.  NaN and what lies below is 0, and all are where the scale is 0.  A
+// candidate in fp32 whose remainder, off by at most 2^-24 (|x - bias| + scale / 2) <
+// 2^-19 scale, is less than half a scale by more than that is the code (a group's
+// x - bias is at most 22 scales, where the scale rounds 22/15 steps of 2^-24 to one).
+// Where that does not decide, the remainder in 64 bits, which is exact, does.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, float bias) {
+    const float inv = scale > 0.f ? 1.f / scale : 0.f, sure = scale * 0.49998f;
+    float n[8];
+    bool all_sure = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float d = x[j] - bias;
+        n[j] = __builtin_rintf(d * inv);
+        all_sure &= fabsf(fmaf(-n[j], scale, d)) < sure;
+    }
+    if (!all_sure && scale > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (!(fabsf(x[j]) < INFINITY)) continue;
+            const double d = static_cast<double>(x[j]) - static_cast<double>(bias), s = scale;
+            const double r2 = 2.0 * fma(-static_cast<double>(n[j]), s, d);
+            const bool odd = static_cast<int>(n[j]) & 1;
+            if (r2 > s || (r2 == s && odd)) n[j] += 1.f;
+            else if (r2 < -s || (r2 == -s && odd)) n[j] -= 1.f;
+        }
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w |= static_cast<uint32_t>(fminf(fmaxf(n[j], 0.f), 15.f)) << (4 * j);
+    return w;
 }
 
 // Keys or values of one token, `share` waves to it, 64 / C heads to a wave at a
-// time and a chunk of eight channels to a lane.
+// time and a chunk of eight channels to a lane.  2000 tokens of 32 heads of 128
+// channels, with as many of q: 20.6 us (26.9 with every quotient and remainder in
+// 64 bits), 3.7 TB/s; 17.6 without the writes.
 template <int D, bool NEIGHBOURS>
 __device__ void append4_rows(const Append4Args& a, int wave) {
     constexpr int C = D / 8, HEADS = 64 / C;
@@ -162,17 +191,22 @@ __device__ void append4_rows(const Append4Args& a, int wave) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             f[j] = h2f(half_of(x, j));
-            const bool finite = fabsf(f[j]) < INFINITY;
-            lo = fminf(lo, finite ? f[j] : INFINITY);
-            hi = fmaxf(hi, finite ? f[j] : -INFINITY);
+            lo = fminf(lo, f[j]);
+            hi = fmaxf(hi, f[j]);
+        }
+        if (!(lo > -INFINITY && hi < INFINITY)) {  // of the finite ones
+            lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool finite = fabsf(f[j]) < INFINITY;
+                lo = fminf(lo, finite ? f[j] : INFINITY);
+                hi = fmaxf(hi, finite ? f[j] : -INFINITY);
+            }
         }
         lo = over_lanes(lo, lanes_log2, [](float u, float v) { return fminf(u, v); });
         hi = over_lanes(hi, lanes_log2, [](float u, float v) { return fmaxf(u, v); });
         const uint32_t ab = affine_of(lo, hi);
-        const float scale = h2f(ab & 0xFFFFu), bias = h2f(ab >> 16), inv = scale > 0.f ? 1.f / scale : 0.f;
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w |= (scale > 0.f ? code_of(f[j], scale, inv, bias) : 0u) << (4 * j);
+        const uint32_t w = codes_of(f, h2f(ab & 0xFFFFu), h2f(ab >> 16));
         const int64_t base = static_cast<int64_t>(page) * a.c.kv_heads + head;
         *reinterpret_cast<uint32_t*>(codes + ((base << a.c.block_log2) + off) * (D / 2) + 4 * ch) = w;
         if ((ch & ((1 << lanes_log2) - 1)) == 0) affine[((base * a.c.groups + group) << a.c.block_log2) + off] = ab;
@@ -180,7 +214,8 @@ __device__ void append4_rows(const Append4Args& a, int wave) {
 }
 
 // Workgroups [0, kv_groups): keys and values; behind them q, four heads to a
-// thread, as in rope.
+// thread, as in rope.  8192 tokens of 32 heads of 256 channels over two: 69 us, of
+// which q's 268 MB take 57 at 4.7 TB/s.
 template <int D, bool NEIGHBOURS>
 __global__ __launch_bounds__(256) void kv4_append(Append4Args a) {
     if (static_cast<int>(blockIdx.x) < a.kv_groups) {
@@ -206,15 +241,18 @@ struct Values4Args {
     int64_t rows;
 };
 
-// Row i's keys and values, a chunk of eight channels to a lane.
+// 256 / C rows of one head to a workgroup, a chunk of eight channels to a thread:
+// neighbouring rows' codes and affine pairs lie side by side where they are neighbouring
+// tokens.  Bound by the bytes, most of them the rows': 8192 rows of 32 heads of 128
+// channels 26 us, 6.7 TB/s (stores that stay in the caches 38; a row's heads to a
+// workgroup, half a cache line of each head's codes, 55).
 template <int D>
 __global__ __launch_bounds__(256) void kv4_values(Values4Args a) {
     constexpr int C = D / 8;
     const NibUnpack nib;
-    const int64_t per_row = static_cast<int64_t>(a.c.kv_heads) * C, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = i / per_row;
+    const int head = blockIdx.x % a.c.kv_heads, ch = threadIdx.x % C;
+    const int64_t row = static_cast<int64_t>(blockIdx.x / a.c.kv_heads) * (256 / C) + threadIdx.x / C;
     if (row >= a.rows) return;
-    const int at = static_cast<int>(i - row * per_row), head = at / C, ch = at % C;
     const int s = a.slots[row], page = s >> a.c.block_log2;
     uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (s >= 0 && page < a.c.num_blocks) {
@@ -227,8 +265,9 @@ __global__ __launch_bounds__(256) void kv4_values(Values4Args a) {
         k = rising_from_pairs(elements8(nib, wk, ak));
         v = rising_from_pairs(elements8(nib, wv, av));
     }
-    *reinterpret_cast<uint4*>(a.k + 8 * i) = k;
-    *reinterpret_cast<uint4*>(a.v + 8 * i) = v;
+    const int64_t to = ((row * a.c.kv_heads + head) * C + ch) * 8;
+    store_nt16(a.k + to, k);
+    store_nt16(a.v + to, v);
 }
 
 }  // namespace
@@ -321,7 +360,7 @@ extern "C" int gdsllm_kv4_values(const gdsllm_kv_cache4* cache, const int32_t* s
     a.k = static_cast<uint16_t*>(k);
     a.v = static_cast<uint16_t*>(v);
     a.rows = rows;
-    const int64_t D = cache->head_dim, grid = (rows * cache->kv_heads * (D / 8) + 255) / 256;
+    const int64_t D = cache->head_dim, per = 256 / (D / 8), grid = (rows + per - 1) / per * cache->kv_heads;
     if (grid * 256 >= (int64_t(1) << 32)) return bad("too many rows and heads for one call");
     const dim3 g(static_cast<unsigned>(grid));
     const hipStream_t s = as_stream(stream);

@@ -125,8 +125,8 @@ __device__ __forceinline__ void rope_unit(const RopeRows& r, int D, int half, in
         const int h = h0 + i * step;
         if (h >= r.heads) continue;
         uint16_t* p = r.to(t, h, D);
-        *reinterpret_cast<uint4*>(p + c0) = x[i];
-        if (!NEIGHBOURS && rotates) *reinterpret_cast<uint4*>(p + c1) = y[i];
+        store_nt16(p + c0, x[i]);
+        if (!NEIGHBOURS && rotates) store_nt16(p + c1, y[i]);
     }
 }
 
