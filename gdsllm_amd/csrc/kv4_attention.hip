@@ -71,6 +71,7 @@ struct RowTile4 {
     // kBegin: 32 requests of up to 8192 tokens 43.0 us with 6 (47.7 with none, 45.1 with 4, 43.8 with 7), 32 of up
     // to 4000 of 256 channels 22.8 (26.9, 24.4, 24.3)
     static constexpr int kRows = 16, kD = D, kPerCu = per_cu(D), kBegin = 6;
+    static constexpr bool kRowJoin = false;
     static constexpr int kThreads = NW_ * 64;
     static constexpr int NT = 2;        // score tiles of an iteration
     static constexpr int NW = NW_;
@@ -351,6 +352,7 @@ template <int D, int SPLIT>
 struct PromptTile4 {
     typedef Args4 Args;
     static constexpr int kRows = 256 / SPLIT, kThreads = 512, kD = D, kPerCu = kPromptsPerCu, kBegin = 6;
+    static constexpr bool kRowJoin = true;
     static constexpr int BN = D == 256 ? 32 : D == 64 && SPLIT == 1 ? 128 : 64;
     static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
     static constexpr bool kQInLds = D == 256;
@@ -797,7 +799,7 @@ int launch_attend4(Args4 a, const Plan& p, int64_t blocks, int64_t max_rows, cha
     a.zero_other = p.few.on ? 0 : zero_other;
     char* ws = workspace + p.few.bytes;
     if constexpr (D <= 128)
-        if (p.many.rows == 256) return launch_part<PromptTile4<D, 1>, PromptTile4<D, 2>>(a, p.many, blocks, max_rows, ws, s, where);
+        if (p.many.rows == 256) return launch_part<PromptTile4<D, 1>, PromptTile4<D, 1>>(a, p.many, blocks, max_rows, ws, s, where);
     return launch_part<PromptTile4<D, 2>, PromptTile4<D, 2>>(a, p.many, blocks, max_rows, ws, s, where);
 }
 
@@ -809,7 +811,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv4_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                       int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len, kPromptsPerCu);
+    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len, {kPromptsPerCu, true});
 }
 
 extern "C" int gdsllm_kv4_attention(const gdsllm_kv_cache4* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
@@ -821,8 +823,8 @@ extern "C" int gdsllm_kv4_attention(const gdsllm_kv_cache4* cache, const void* q
     AttendCall c;
     if (int rc = kv4_cache_args(cache, "kv4_attention", &a.c)) return rc;
     if (int rc = attend_call("kv4_attention", cache, q, ldq, o, ldo, tokens, q_heads, block_tables, table_width, ld_table, lens,
-                             starts, requests, scale, max_new, max_len, zero_other, workspace, workspace_bytes, kPromptsPerCu, a,
-                             &c))
+                             starts, requests, scale, max_new, max_len, zero_other, workspace, workspace_bytes,
+                             {kPromptsPerCu, true}, a, &c))
         return rc;
     if (c.empty) return ok();
     const hipStream_t s = as_stream(stream);

@@ -286,6 +286,53 @@ __global__ __launch_bounds__(THREADS) void attend_join(Args a, int rows) {
     }
 }
 
+// The same where a tile has many rows and a sequence few parts: D/4 threads to a
+// row, which go over its parts in order, four of them under way at once.
+template <class Args, int RT, int D>
+__global__ __launch_bounds__(256) void attend_join_rows(Args a, int blocks) {
+    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    const int b = blockIdx.y, sequence = blockIdx.x / blocks, head = sequence % a.c.kv_heads, row0 = sequence / a.c.kv_heads * RT;
+    const int2 d = a.parts[static_cast<int64_t>(b) * a.tiles * a.c.kv_heads + sequence];
+    const Rows<RT> R(a, b);
+    const int count = min(RT, R.rows - row0), c = 4 * (threadIdx.x % TPR);
+    const int r0 = blockIdx.x % blocks * RPB + threadIdx.x / TPR;
+    if (r0 >= count || d.y == 0) return;  // no such row (d is not set where there is none), or whole
+    for (int r = r0; r < count; r += blocks * RPB) {
+        float m = -INFINITY, l = 0.f;
+        float4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < d.y; i0 += 4) {
+            float2 ml[4];
+            float4_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = min(i0 + k, d.y - 1);
+                const int64_t at = static_cast<int64_t>(i == 0 ? d.x : 2 * (d.x / 2 + i)) * RT + r;
+                ml[k] = a.part_ml[at];
+                o[k] = *reinterpret_cast<const float4_t*>(a.part_o + at * D + c);
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k].x);
+            const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m - ref);
+            l *= f;
+            acc *= f;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = i0 + k < d.y ? __builtin_amdgcn_exp2f(ml[k].x - ref) : 0.f;
+                l = fmaf(ml[k].y, w, l);
+                acc += o[k] * w;
+            }
+        }
+        const float inv = inverse(l);
+        uint16_t* out = a.o + (R.start + (row0 + r) / a.group) * a.ldo + (head * a.group + (row0 + r) % a.group) * D + c;
+        uint2 w;
+        w.x = pack_h2(static_cast<half_t>(acc[0] * inv), static_cast<half_t>(acc[1] * inv));
+        w.y = pack_h2(static_cast<half_t>(acc[2] * inv), static_cast<half_t>(acc[3] * inv));
+        *reinterpret_cast<uint2*>(out) = w;
+    }
+}
+
 // Workgroups of attend_shared that a compute unit holds at once (registers: 16
 // rows of accumulators, a tile of codes and Q grow with D).  At D = 256 one, so
 // that a long sequence leaves half as many parts: 131072 tokens 36.8 us against
@@ -334,15 +381,22 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
     p->bytes = part_bytes(p->groups, p->rows, p->sequences, head_dim);
 }
 
-// Workgroups that the device holds at once, of 16-row tiles and of many rows': a
-// compute unit holds `many` of those.
+// Workgroups of 16-row tiles that the device holds at once.
 int64_t resident_few(int64_t head_dim) { return per_cu(head_dim) * static_cast<int64_t>(kCus); }
+
+// What the kernels for many rows (prompts) are like: workgroups that a compute
+// unit holds at once, and whether work is shared out in 256-row tiles too.
+struct Prompts {
+    int per_cu;
+    bool shares_wide;
+};
 
 // One workgroup to a sequence where none is long or there are many of them, else
 // as many workgroups as the device holds at once, with even shares.  (256 requests
 // of up to 4000 tokens over 8 heads: 218 us whole, 236 shared out; a prompt of 500 tokens
 // behind 1500, 128 tiles: 62 whole, 66 shared out; one of 64 in 32 tiles: 57 and 34.)
-Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len, int many_per_cu) {
+Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len,
+                 const Prompts& prompts) {
     Plan p;
     const int64_t rows = max_new * (q_heads / kv_heads);
     const bool many = rows > 2 * kFewRows;
@@ -355,16 +409,26 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
                     max_len <= kWholeTokens || sequences >= (max_len <= 4 * kWholeTokens ? 2 : 8) * resident);
     }
     if (many) {
-        const int64_t resident = many_per_cu * static_cast<int64_t>(kCus);
-        // 256 rows to a tile (each wave converts half as much) where that still leaves
-        // two workgroups to a compute unit, one after the other: 4096 tokens of 32
-        // heads over the 8-bit cache 172 us against 188; 4 chunks of 300 tokens 167 against 161
-        const bool wide = head_dim <= 128 && requests * kv_heads * ((rows + 255) / 256) >= resident;
+        const int64_t resident = prompts.per_cu * static_cast<int64_t>(kCus);
+        const int64_t sequences = requests * kv_heads * ((rows + 127) / 128), wide_sequences = requests * kv_heads * ((rows + 255) / 256);
+        bool wide, whole;
+        if (prompts.shares_wide) {
+            // 256 rows to a tile (each wave converts half as much) where those are many; whole
+            // where two of them come to a compute unit, one after the other: 4 chunks of up
+            // to 300 tokens behind up to 5000 take 132 us shared out in 256-row tiles, 150 in
+            // 128-row ones and 148 whole, 500 tokens behind 1500 44, 43 and 46
+            wide = head_dim <= 128 && 2 * wide_sequences >= resident;
+            whole = max_len <= kWholeTokens || (wide ? wide_sequences : sequences) >= 2 * resident;
+        } else {
+            // 256 rows to a tile where that still leaves two workgroups to a compute unit, one
+            // after the other: 4096 tokens of 32 heads over the 8-bit cache 172 us against
+            // 188; 4 chunks of 300 tokens 167 against 161
+            wide = head_dim <= 128 && wide_sequences >= resident;
+            whole = wide || max_len <= (4 * sequences >= resident ? 2 : 1) * kWholeTokens || 2 * sequences >= resident;
+        }
         p.many.rows = wide ? 256 : 128;
         if (p.few.on) p.many.min_rows = kFewRows + 1;
-        const int64_t sequences = requests * kv_heads * ((rows + 127) / 128);
-        finish_part(&p.many, requests, kv_heads, head_dim, rows, max_len, resident,
-                    wide || max_len <= (4 * sequences >= resident ? 2 : 1) * kWholeTokens || 2 * sequences >= resident);
+        finish_part(&p.many, requests, kv_heads, head_dim, rows, max_len, resident, whole);
     }
     return p;
 }
@@ -373,9 +437,10 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
 // and max_len too, which need not be less: a prompt of 4096 tokens of 32 heads is
 // whole and needs none, 64 tokens behind as many share their work.  Work is
 // shared out past kWholeTokens alone, by up to 64 rows of fewer than 8 * resident
-// sequences and by 128-row tiles of fewer than resident / 2.
+// sequences and by 128-row tiles of fewer than resident / 2, or, with
+// shares_wide, by tiles of either size of fewer than 2 * resident.
 size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int64_t max_len,
-                       int many_per_cu) {
+                       const Prompts& prompts) {
     if (max_len <= kWholeTokens) return 0;
     const int64_t rows = max_new * (q_heads / kv_heads), units = (max_len + 255) / 256;
     auto part = [&](int64_t tile, int64_t most, int64_t limit, int64_t resident) {
@@ -383,7 +448,12 @@ size_t workspace_bound(int64_t requests, int64_t q_heads, int64_t kv_heads, int6
         return part_bytes(std::min(resident, sequences * units), tile, sequences, head_dim);
     };
     size_t bytes = part(16, std::min<int64_t>(rows, 2 * kFewRows), 8 * resident_few(head_dim), resident_few(head_dim));
-    if (rows > 2 * kFewRows) bytes += part(128, rows, many_per_cu * kCus / 2, many_per_cu * kCus);
+    if (rows > 2 * kFewRows) {
+        const int64_t resident = prompts.per_cu * static_cast<int64_t>(kCus);
+        size_t most = part(128, rows, prompts.shares_wide ? 2 * resident : resident / 2, resident);
+        if (prompts.shares_wide && head_dim <= 128) most = std::max(most, part(256, rows, 2 * resident, resident));
+        bytes += most;
+    }
     return bytes;
 }
 
@@ -412,6 +482,12 @@ int launch_part(typename S::Args a, const Part& p, int64_t blocks, int64_t max_r
     if (int rc = prepare_lds(reinterpret_cast<const void*>(&attend_shared<S>), lds)) return rc;
     hipLaunchKernelGGL(attend_shared<S>, dim3(a.groups), dim3(S::kThreads), lds, s, a);
     const int rows = static_cast<int>(std::min<int64_t>(S::kRows, std::max<int64_t>(1, max_rows)));
+    if constexpr (S::kRowJoin) {
+        constexpr int per = 1024 / S::kD;
+        const int n = (rows + per - 1) / per;
+        hipLaunchKernelGGL((attend_join_rows<typename S::Args, S::kRows, S::kD>), dim3(per_request * n, requests), dim3(256), 0, s, a, n);
+        return check_hip(hipGetLastError(), where);
+    }
     const dim3 join(per_request * rows, requests);
     // few sequences are long, in many parts each
     if (p.sequences * rows <= kCus)
@@ -438,7 +514,7 @@ template <class Args, class Desc>
 int attend_call(const std::string& n, const Desc* cache, const void* q, int64_t ldq, void* o, int64_t ldo, int64_t tokens,
                 int64_t q_heads, const int32_t* block_tables, int64_t table_width, int64_t ld_table, const int32_t* lens,
                 const int32_t* starts, int64_t requests, float scale, int64_t max_new, int64_t max_len, int zero_other,
-                void* workspace, size_t workspace_bytes, int many_per_cu, Args& a, AttendCall* call) {
+                void* workspace, size_t workspace_bytes, const Prompts& prompts, Args& a, AttendCall* call) {
     auto bad = [&](const std::string& m) { return set_error(GDSLLM_ERR_INVALID_ARGUMENT, n + ": " + m); };
     const int64_t D = cache->head_dim;
     if (tokens < 0 || tokens > (int64_t(1) << 30)) return bad("bad token count");
@@ -463,7 +539,7 @@ int attend_call(const std::string& n, const Desc* cache, const void* q, int64_t 
     if (max_len == 0 || max_len > most) max_len = most;
     if (!attend_sizes(requests, q_heads, cache->kv_heads, D, max_new, max_len)) return bad("sizes out of range");
     if (requests == 0) return bad("no requests for the tokens");
-    const Plan& p = call->plan = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len, many_per_cu);
+    const Plan& p = call->plan = plan_attend(requests, q_heads, cache->kv_heads, D, max_new, max_len, prompts);
     const size_t need = p.bytes();
     if (need > 0 && (!workspace || workspace_bytes < need))
         return bad("workspace of " + std::to_string(need) + " bytes needed, got " + std::to_string(workspace_bytes));

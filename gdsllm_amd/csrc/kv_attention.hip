@@ -57,7 +57,8 @@ constexpr int prompts_per_cu(int64_t D) { return D == 256 ? 1 : 2; }
 template <bool E4M3, int D, int NW_>
 struct RowTile {
     typedef Args8 Args;
-    static constexpr int kRows = 16, kD = D, kPerCu = per_cu(D), kBegin = 0;  // not tuned: 0 keeps the order of its sums
+    static constexpr int kRows = 16, kD = D, kPerCu = per_cu(D), kBegin = 0;
+    static constexpr bool kRowJoin = false;
     static constexpr int kThreads = NW_ * 64;
     static constexpr int NT = 2;        // score tiles of an iteration
     static constexpr int NW = NW_;
@@ -334,6 +335,7 @@ template <bool E4M3, int D, int NW>
 struct PromptTile {
     typedef Args8 Args;
     static constexpr int kRows = 32 * NW, kThreads = 64 * NW, kD = D, kPerCu = prompts_per_cu(D), kBegin = 0;
+    static constexpr bool kRowJoin = false;
     static constexpr int BN = D == 256 ? 32 : 64;
     static constexpr int ST = BN / 32, KS = D / 16, DT = D / 32, U = BN / 16;
     // 16-code chunks of K, and the ones a thread converts (the last threads none where there are fewer)
@@ -595,7 +597,7 @@ using namespace gdsllm;
 extern "C" size_t gdsllm_kv_attention_workspace_size(int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t max_new, int64_t max_len) {
     if (!attend_sizes(requests, q_heads, kv_heads, head_dim, max_new, max_len)) return 0;
-    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len, prompts_per_cu(head_dim));
+    return workspace_bound(requests, q_heads, kv_heads, head_dim, max_new, max_len, {prompts_per_cu(head_dim), false});
 }
 
 extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q, int64_t ldq, void* o, int64_t ldo,
@@ -608,7 +610,7 @@ extern "C" int gdsllm_kv_attention(const gdsllm_kv_cache8* cache, const void* q,
     if (int rc = kv_cache_args(cache, "kv_attention", &a.c)) return rc;
     if (int rc = attend_call("kv_attention", cache, q, ldq, o, ldo, tokens, q_heads, block_tables, table_width, ld_table, lens,
                              starts, requests, scale, max_new, max_len, zero_other, workspace, workspace_bytes,
-                             prompts_per_cu(cache->head_dim), a, &c))
+                             {prompts_per_cu(cache->head_dim), false}, a, &c))
         return rc;
     if (c.empty) return ok();
     const int64_t D = cache->head_dim;

@@ -215,6 +215,16 @@ def test_many_sequences_take_the_widest_tiles(gpu, dim, group):
     p.check(p.run(), [0, 77, 127])
 
 
+@pytest.mark.parametrize("dim,group,bs,lens,new", [(128, 64, 32, [1300, 900], [70, 65]), (64, 32, 16, [1100, 5, 1500], [80, 3, 33]),
+                                                   (128, 128, 256, [1029], [200]), (64, 64, 64, [70, 2100], [70, 129])])
+def test_the_widest_tiles_share_the_work(gpu, dim, group, bs, lens, new):
+    """128 to 511 (request, kv head, 256 rows) past 1024 tokens: parts of 256-row tiles, which begin and end inside
+    the tiles of tokens, rows that see none of a part, ragged last rows, a request with few rows beside them."""
+    p = Problem(gpu, group, dim, 256, 64, bs, lens, new, 1550 + dim + len(lens))
+    p.poison()
+    p.check(p.run(), [0, 31, 63])
+
+
 def test_whole_sequences_past_a_segment(gpu):
     """Many sequences, so that each has a workgroup of its own, longer than the block table it holds at once."""
     p = Problem(gpu, 128, 256, 1024, 1024, 64, [100, 3], [1, 1], 1600)

@@ -2,6 +2,7 @@
 before anything touches a device, with a message that names what is wrong."""
 
 import ctypes
+import re
 
 import pytest
 import torch
@@ -125,6 +126,24 @@ def test_attention_workspace_serves_smaller_calls(heads, kv_heads, dim):
         for small in steps:
             if all(a <= b for a, b in zip(small, big)):
                 assert sizes[small] <= sizes[big], (small, big)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 32, 128), (64, 8, 128), (32, 2, 256), (8, 1, 64), (256, 64, 64), (7, 7, 128)])
+def test_attention_workspace_covers_the_plan(heads, kv_heads, dim):
+    """What a call says that it needs is within the workspace's size for the same step, in every form of the plan (the
+    call is refused for its 2^30 tokens in any case)."""
+    size, c, shared = capi().gdsllm_kv4_attention_workspace_size, _cache(kv_heads=kv_heads, head_dim=dim, group_size=64), 0
+    for r in (1, 2, 3, 4, 5, 16, 40, 300):
+        for new in (1, 2, 9, 33, 64, 65, 70, 129, 300, 1000, 4096):
+            for length in (512, 1024, 1025, 1300, 2048, 2049, 5000, 131072):
+                assert attention(c=c, n=2 ** 30, hq=heads, ldq=heads * dim, ldo=heads * dim, w=8192, ldt=8192, b=r, new=new,
+                                 ml=length, ws=None, wb=0) == BAD
+                need = re.search(r"workspace of (\d+) bytes", _err())
+                assert need or "2^30" in _err(), _err()
+                if need:
+                    shared += 1
+                    assert int(need[1]) <= size(r, heads, kv_heads, dim, new, length), (r, new, length)
+    assert shared > 50
 
 
 def rope(q=16, ldq=128, qo=32, ldqo=128, hq=2, k=16, ldk=64, ko=48, ldko=64, hk=1, d=64, n=2, pos=16, cos=16, sin=16, rot=64,
