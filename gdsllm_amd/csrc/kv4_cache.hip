@@ -31,6 +31,7 @@ int kv4_cache_args(const gdsllm_kv_cache4* c, const std::string& where, Kv4Cache
     if (c->kv_heads < 1 || c->kv_heads > 1024) return bad("kv_heads must be in [1, 1024]");
     if (c->num_blocks < 1 || c->num_blocks > ((int64_t(1) << 31) - 1) / c->block_size)
         return bad("num_blocks must be positive and num_blocks * block_size below 2^31");
+    if (c->num_blocks * c->kv_heads >= int64_t(1) << 31) return bad("num_blocks * kv_heads must be below 2^31");
     if (!c->k || !c->v || !c->k_affine || !c->v_affine) return bad("null cache pointer");
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_affine) |
          reinterpret_cast<uintptr_t>(c->v_affine)) % 16)

@@ -560,7 +560,7 @@ int gdsllm_rope(const void* q, int64_t ldq, void* q_out, int64_t ldqo, int64_t q
  * as they are.  A row whose slot lies outside the cache (-1) or whose position
  * outside [0, max_pos) is padding: not written, zeros in q_out.  Of several rows with one
  * slot the last counts, where the tokens of a block stand in consecutive rows (as
- * kv_assign numbers them, no padding between them).                          */
+ * kv_assign numbers them, no padding between them); elsewhere no slot may occur twice.  */
 int gdsllm_kv4_append(const gdsllm_kv_cache4* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
                       const int32_t* slots, int64_t tokens, const void* q, int64_t ldq, void* q_out, int64_t q_heads,
                       const int32_t* positions, const float* cos, const float* sin, int64_t rotary, int64_t max_pos,

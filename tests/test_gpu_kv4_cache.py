@@ -150,6 +150,55 @@ def test_every_exponent(gpu):
     c.append(x, x.flip(0), torch.arange(n).int())
 
 
+def test_values_next_to_ties(gpu):
+    """Groups of values in the middle between two codes of theirs, or one fp16 step off it, of every range and offset;
+    signalling NaNs among them."""
+    g = gen(10)
+    n, dim, group = 4096, 64, 32
+    low = (torch.exp2(torch.randint(-24, 15, (n, 2, 1), generator=g).float()) * torch.randn(n, 2, 1, generator=g)).half().double()
+    span = 15 * torch.exp2(torch.randint(-24, 11, (n, 2, 1), generator=g).double()) * (1 + torch.rand(n, 2, 1, generator=g).double())
+    high = (low + span).clamp(max=65504).half().double()
+    scale = ((high - low) / 15).float().half().double()
+    x = (low + (torch.randint(0, 15, (n, 2, group), generator=g) + 0.5) * scale).clamp(-65504, 65504).half()
+    x = (x.view(torch.int16) + torch.randint(-1, 2, x.shape, generator=g).to(torch.int16)).view(torch.float16)
+    x = torch.minimum(torch.maximum(x.double(), low), high)
+    x[:, :, :1], x[:, :, 1:2] = low, high
+    x = x.half().reshape(n, 1, dim)
+    x.view(torch.int16)[::7, 0, 9] = 0x7C01
+    c = Cache(gpu, n // 64, 1, 64, dim, group, 11)
+    c.append(x, x.flip(0), torch.arange(n).int())
+
+
+def test_append_and_values_in_a_graph(gpu):
+    """A replay takes what its inputs hold then, as the eager calls do."""
+    g = gen(12)
+    n, heads, dim = 37, 3, 128
+    a, b = Cache(gpu, 6, heads, 16, dim, 64, 13), Cache(gpu, 6, heads, 16, dim, 64, 13)
+    cos, sin = (t.to(gpu) for t in angles(50, dim, g))
+    k, v, slots, pos = (torch.zeros(s, dtype=d, device=gpu) for s, d in (((n, heads, dim), torch.float16),) * 2 +
+                        (((n,), torch.int32),) * 2)
+
+    def step(c):
+        q = ext().kv4_append(k, v, slots, *c.dev, k, pos, cos, sin, True)
+        return (q, *ext().kv4_values(slots, *c.dev))
+
+    step(Cache(gpu, 6, heads, 16, dim, 64, 14))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(a)
+    for i in range(4):
+        k.copy_(rows(n, heads, dim, g))
+        v.copy_(rows(n, heads, dim, g))
+        slots.copy_(torch.randperm(96, generator=g)[:n].sort().values.int())
+        pos.copy_(torch.randint(-1, 51, (n,), generator=g).int())
+        graph.replay()
+        want = step(b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(got, want))
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a.dev, b.dev))
+
+
 def test_strided_rows_and_another_stream(gpu):
     """q, k and v inside one projection's rows, on a stream of the caller's."""
     g = gen(10)

@@ -25,7 +25,7 @@ def _cache(**kw):
 CACHES = [(dict(k=0), "null"), (dict(v_affine=0), "null"), (dict(k=8), "misaligned"), (dict(k_affine=24), "misaligned"),
           (dict(block_size=8), "block_size"), (dict(block_size=48), "block_size"), (dict(block_size=512), "block_size"),
           (dict(head_dim=80), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(kv_heads=0), "kv_heads"),
-          (dict(kv_heads=1025), "kv_heads"), (dict(num_blocks=0), "num_blocks"), (dict(num_blocks=2 ** 28), "num_blocks"),
+          (dict(kv_heads=1025), "kv_heads"), (dict(num_blocks=0), "num_blocks"), (dict(num_blocks=2 ** 28), "num_blocks"), (dict(num_blocks=2 ** 21, kv_heads=1024), "kv_heads"),
           (dict(group_size=16), "group_size"), (dict(group_size=48), "group_size"), (dict(group_size=128), "group_size")]
 
 
