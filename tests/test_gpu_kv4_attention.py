@@ -225,6 +225,14 @@ def test_the_widest_tiles_share_the_work(gpu, dim, group, bs, lens, new):
     p.check(p.run(), [0, 31, 63])
 
 
+@pytest.mark.parametrize("dim,max_new,max_len", [(128, 20, 0), (64, 20, 1500), (128, 0, 1100), (128, 30, 40000)])
+def test_the_widest_tiles_under_other_bounds(gpu, dim, max_new, max_len):
+    """More rows, and longer requests, than the caller said, over work that is shared out in 256-row tiles."""
+    p = Problem(gpu, 64, dim, 256, 64, 64, [1700, 1200, 3], [70, 130, 1], 1570 + dim)
+    p.poison()
+    p.check(p.run(max_new=max_new, max_len=max_len), [0, 31, 63])
+
+
 def test_whole_sequences_past_a_segment(gpu):
     """Many sequences, so that each has a workgroup of its own, longer than the block table it holds at once."""
     p = Problem(gpu, 128, 256, 1024, 1024, 64, [100, 3], [1, 1], 1600)
