@@ -2,7 +2,8 @@
 // request, the split of the work over workgroups, the join of its parts, the plan
 // of a call's launches and the checks of its arguments.  A tile class T (RowTile,
 // PromptTile) does a sequence: T::run(args, lds, ...), T::Args, T::Lds, T::kRows,
-// T::kD, T::kThreads, T::kPerCu.
+// T::kD, T::kThreads, T::kPerCu (of them to a compute unit), T::kBegin (blocks that
+// the beginning of a sequence counts as) and T::kRowJoin (parts are joined by rows).
 #pragma once
 
 #include <algorithm>
