@@ -228,12 +228,29 @@ def rope_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[dict
                 low) / (high - low)
       "yarn"    inv_freq / s for pairs past beta_slow turns in L positions, as it
                 is for those before beta_fast (32 and 1 where they are not given), a
-                line in i between them; factor = attention_factor, or 0.1 ln s + 1
+                line in i between them, from and to whole pairs unless truncate is
+                false; factor = attention_factor, or t(mscale) / t(mscale_all_dim)
+                with t(m) = 0.1 m ln s + 1 where both are given, or t(1).  (Models
+                that give mscale_all_dim also multiply the scale of their scores by
+                t(mscale_all_dim) ** 2: attend's `scale`.)
+    A key that its kind does not use is refused, but for those that say what the
+    arguments say or what the model is: rope_theta (must be theta),
+    partial_rotary_factor, original_max_position_embeddings, finetuned.  A key
+    with None is not given.
     """
     if rotary < 2 or rotary % 2:
         raise ValueError(f"rope_frequencies: rotary must be even and positive, got {rotary}")
-    scaling = scaling or {}
+    scaling = {key: v for key, v in (scaling or {}).items() if v is not None}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if scaling.get("type", kind) != kind:
+        raise ValueError(f"rope_frequencies: rope_type {kind!r} and type {scaling['type']!r} differ")
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rope_frequencies: unknown scaling {kind!r}")
+    other = sorted(set(scaling) - _SCALING_KEYS[kind] - _MODEL_KEYS)
+    if other:
+        raise ValueError(f"rope_frequencies: {kind} does not use {', '.join(map(repr, other))}")
+    if float(scaling.get("rope_theta", theta)) != theta:
+        raise ValueError(f"rope_frequencies: rope_theta is {scaling['rope_theta']}, theta {theta}")
     i = torch.arange(rotary // 2, dtype=torch.float64)
 
     def need(key: str, low: float) -> float:
@@ -249,8 +266,6 @@ def rope_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[dict
     f = theta ** (-2 * i / rotary)
     if kind == "default":
         return f, 1.0
-    if kind not in ("linear", "llama3", "yarn"):
-        raise ValueError(f"rope_frequencies: unknown scaling {kind!r}")
     s = need("factor", 1.0)
     if kind == "linear":
         return f / s, 1.0
@@ -269,10 +284,39 @@ def rope_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[dict
         return rotary * math.log(length / (2 * math.pi * turns)) / (2 * math.log(theta))
 
     fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
-    first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary - 1)
+    if not fast >= slow > 0:
+        raise ValueError(f"rope_frequencies: yarn needs beta_fast >= beta_slow > 0, got {fast} and {slow}")
+    first, last = pair_of(fast), pair_of(slow)
+    if scaling.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary - 1)
     slowed = ((i - first) / (last - first)).clamp(0, 1) if last > first else (i > first).double()
-    factor = scaling.get("attention_factor")
-    return slowed * f / s + (1 - slowed) * f, 0.1 * math.log(s) + 1 if factor is None else float(factor)
+    return slowed * f / s + (1 - slowed) * f, _yarn_factor(scaling, s)
+
+
+# Keys that a dictionary of any kind may hold, and those that a kind's formula reads.
+_MODEL_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings", "finetuned"}
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": {"factor"},
+    "ntk": {"factor"},
+    "llama3": {"factor", "low_freq_factor", "high_freq_factor"},
+    "yarn": {"factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"},
+}
+
+
+def _yarn_factor(scaling: dict, s: float) -> float:
+    """What yarn multiplies cos and sin by."""
+    if "attention_factor" in scaling:
+        return float(scaling["attention_factor"])
+    m, all_dim = float(scaling.get("mscale") or 0.0), float(scaling.get("mscale_all_dim") or 0.0)
+    if m < 0 or all_dim < 0:
+        raise ValueError("rope_frequencies: mscale and mscale_all_dim must not be negative")
+    if not all_dim and m in (0.0, 1.0):
+        return 0.1 * math.log(s) + 1
+    if not m or not all_dim:  # programs differ in what one without the other means
+        raise ValueError("rope_frequencies: yarn needs mscale and mscale_all_dim together")
+    return (0.1 * m * math.log(s) + 1) / (0.1 * all_dim * math.log(s) + 1)
 
 
 def rope_table(max_pos: int, rotary: int, theta: float = 10000.0, inv_freq: Optional[torch.Tensor] = None,

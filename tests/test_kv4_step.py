@@ -231,3 +231,52 @@ def test_rotary_refusals():
             kv_cache.rope_frequencies(r)
     with pytest.raises(ValueError, match="one pair"):
         kv_cache.rope_frequencies(2, 10000.0, dict(type="ntk", factor=2.0))
+
+
+YARN = dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("keys,want", [
+    (dict(mscale=1.0, mscale_all_dim=1.0), 1.0), (dict(mscale=0.707, mscale_all_dim=0.707), 1.0),
+    (dict(mscale=2.0, mscale_all_dim=0.5), (0.2 * math.log(40) + 1) / (0.05 * math.log(40) + 1)),
+    (dict(mscale=1.0), 0.1 * math.log(40) + 1), (dict(mscale=1.0, mscale_all_dim=0), 0.1 * math.log(40) + 1),
+    (dict(mscale=None, mscale_all_dim=None, attention_factor=None), 0.1 * math.log(40) + 1),
+    (dict(mscale=0.0, mscale_all_dim=0.0), 0.1 * math.log(40) + 1),
+    (dict(mscale=1.0, mscale_all_dim=1.0, attention_factor=0.75), 0.75)])
+def test_yarn_factor(keys, want):
+    f, m = kv_cache.rope_frequencies(64, 10000.0, dict(YARN, **keys))
+    assert abs(m - want) < 1e-15
+    assert torch.equal(f, kv_cache.rope_frequencies(64, 10000.0, YARN)[0])
+
+
+def test_yarn_between_whole_pairs_or_not():
+    """truncate: whether the line between the pairs that stay and those that are slowed begins and ends at whole pairs."""
+    turns = lambda i: 4096 * 10000.0 ** (-i / 32) / (2 * math.pi)  # noqa: E731
+    first, last = (32 * math.log(4096 / (2 * math.pi * b)) / math.log(10000.0) for b in (32, 1))
+    assert abs(turns(first) - 32) < 1e-9 and abs(turns(last) - 1) < 1e-9 and first % 1 and last % 1
+    for truncate, lo, hi in ((True, math.floor(first), math.ceil(last)), (False, first, last)):
+        f, _ = kv_cache.rope_frequencies(64, 10000.0, dict(YARN, truncate=truncate))
+        for i in range(32):
+            slowed = min(max((i - lo) / (hi - lo), 0), 1)
+            assert abs(f[i].item() / (10000.0 ** (-i / 32) * (slowed / 40 + 1 - slowed)) - 1) < 1e-12
+
+
+def test_keys_that_say_what_the_model_is():
+    own = {"rope_theta": 500000, "partial_rotary_factor": 0.5, "original_max_position_embeddings": 8192, "type": "linear",
+           "rope_type": "linear", "factor": 2.0, "finetuned": True, "beta_fast": None}
+    assert torch.equal(kv_cache.rope_frequencies(64, 500000.0, own)[0],
+                       kv_cache.rope_frequencies(64, 500000.0, dict(type="linear", factor=2.0))[0])
+
+
+@pytest.mark.parametrize("scaling,word", [
+    (dict(YARN, mscale=0.707), "together"), (dict(YARN, mscale_all_dim=1.0), "together"), (dict(YARN, mscale=-1.0), "negative"),
+    (dict(YARN, beta_fast=1.0, beta_slow=2.0), "beta_fast"), (dict(YARN, beta_slow=-1.0), "beta_slow"),
+    (dict(YARN, attn_factor=1.0), "attn_factor"), (dict(YARN, low_freq_factor=1.0), "low_freq_factor"),
+    (dict(type="linear", factor=2.0, mscale=1.0), "'mscale'"), (dict(type="ntk", factor=2.0, alpha=1.0), "'alpha'"),
+    (dict(rope_type="default", factor=2.0), "'factor'"), (dict(factor=2.0), "'factor'"),
+    (dict(rope_type="llama3", factor=2.0, original_max_position_embeddings=10, low_freq_factor=1, high_freq_factor=4, short_factor=[1.0]),
+     "short_factor"),
+    (dict(rope_type="linear", type="mrope", factor=2.0), "differ"), (dict(type="linear", factor=2.0, rope_theta=1e6), "rope_theta")])
+def test_scaling_keys_are_not_dropped(scaling, word):
+    with pytest.raises(ValueError, match=word):
+        kv_cache.rope_frequencies(64, 10000.0, scaling)
