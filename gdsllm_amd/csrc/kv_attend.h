@@ -29,6 +29,9 @@ constexpr float kSet = 7.f, kMost = 11.f;
 constexpr int kSegment = 4096;             // tokens whose block table a workgroup holds in LDS
 constexpr int kMaxPages = kSegment / 16;   // segments begin on a block of 64 tokens
 constexpr int kBlock = 64;                 // tokens of a unit of work
+// Tokens that a request's table may have places for: tiles count them in 32 bits,
+// up to a segment past the last one (a sum that wrapped round would be an index).
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - 2 * kSegment;
 
 template <class Cache>
 struct AttendArgs {
@@ -522,7 +525,7 @@ int attend_call(const std::string& n, const Desc* cache, const void* q, int64_t 
     if (q_heads < 1 || q_heads % cache->kv_heads) return bad("q_heads must be a multiple of kv_heads");
     if (requests < 0 || requests > 65535) return bad("requests must be in [0, 65535]");
     if (table_width < 1 || ld_table < table_width) return bad("ld_table < table_width or an empty table");
-    if (table_width > ((int64_t(1) << 31) - 1) / cache->block_size) return bad("table_width too large");
+    if (table_width > kMostTokens / cache->block_size) return bad("table_width * block_size must be at most 2^31 - 8192");
     if (max_new < 0 || max_len < 0) return bad("negative max_new or max_len");
     if (!(scale > 0.f) || scale > 1e30f) return bad("scale must be positive and finite");
     call->empty = tokens == 0;

@@ -40,6 +40,8 @@ class _PagedCache:
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"{me}: head_dim must be one of {HEAD_DIMS}, got {head_dim}")
         width = -(-max_len // block_size)
+        if width * block_size > 2 ** 31 - 8192:
+            raise ValueError(f"{me}: max_len must be at most 2^31 - 8192, got {max_len}")
         num_blocks = requests * width if num_blocks is None else num_blocks
         if not 1 <= num_blocks <= (2 ** 31 - 1) // block_size:
             raise ValueError(f"{me}: num_blocks must be positive and num_blocks * block_size below 2^31")

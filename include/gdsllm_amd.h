@@ -497,7 +497,7 @@ int gdsllm_kv_append(const gdsllm_kv_cache8* cache, const void* k, int64_t ldk, 
  * weight.  What the cache holds
  * behind a request's tokens is not read as a number.  A NaN among its values (e4m3
  * only) also reaches rows of its request that stand before it in the same call.
- * tokens * q_heads <= 2^30.
+ * tokens * q_heads <= 2^30, table_width * block_size <= 2^31 - 8192.
  * max_new and max_len: bounds on a request's rows and tokens, known to the host
  * (0: tokens, and table_width * block_size).  They set how the work is split;
  * larger requests than they say are computed all the same, more slowly.  The

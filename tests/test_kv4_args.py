@@ -192,3 +192,14 @@ def test_cache_refusals(kw, word):
     base = dict(layers=1, requests=3, max_len=64, kv_heads=2, head_dim=64, block_size=16, device="cpu")
     with pytest.raises(ValueError, match=word):
         kv_cache.KVCache4(**dict(base, **kw))
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_attention_tables_end_before_32_bits(bs):
+    """Kernels step up to 4096 tokens past a request's last one in 32 bits: a table that long has to end before."""
+    most = (2 ** 31 - 8192) // bs
+    assert attention(c=_cache(block_size=bs), w=most, ldt=most, o=None) == BAD and "null" in _err()
+    assert attention(c=_cache(block_size=bs), w=most + 1, ldt=most + 1, o=None) == BAD and "table_width" in _err()
+    with pytest.raises(ValueError, match="max_len"):
+        kv_cache.KVCache4(1, 1, bs * most + 1, 1, 64, bs, num_blocks=2, group_size=32, device="meta")
+    assert kv_cache.KVCache4(1, 1, bs * most, 1, 64, bs, num_blocks=2, group_size=32, device="meta").max_len == bs * most

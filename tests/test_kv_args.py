@@ -178,3 +178,15 @@ def test_assign_outputs_apart_from_every_input():
     for lens_out, state_out in ((16, 144), (32, 144), (80, 144), (144, 16), (144, 32), (144, 80), (144, 144)):
         assert capi().gdsllm_kv_assign(*base, lens_out, state_out, None) == BAD
         assert "must not be" in _err()
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_attention_tables_end_before_32_bits(bs):
+    """Kernels step up to 4096 tokens past a request's last one in 32 bits: a table that long has to end before."""
+    def call(w):
+        return capi().gdsllm_kv_attention(_cache(block_size=bs), 16, 128, None, 128, 1, 2, 16, w, w, 16, 16, 1, 1.0, 1, 16, 0, None,
+                                          0, None)
+
+    most = (2 ** 31 - 8192) // bs
+    assert call(most) == BAD and "null" in _err()
+    assert call(most + 1) == BAD and "table_width" in _err()
