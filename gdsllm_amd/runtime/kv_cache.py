@@ -30,11 +30,15 @@ GROUP_SIZES = (32, 64, 128)
 class _PagedCache:
     """What the caches share: the requests' lengths and blocks on the device."""
 
+    _MOST_RUNS = None  # of a block and a kv head, where the kernels count them in 32 bits
+
     def __init__(self, layers: int, requests: int, max_len: int, kv_heads: int, head_dim: int, block_size: int,
                  num_blocks: Optional[int], device):
         me = type(self).__name__
-        if layers < 1 or not 1 <= requests <= 8192 or max_len < 1 or kv_heads < 1:
-            raise ValueError(f"{me}: layers, max_len and kv_heads must be positive, requests in [1, 8192]")
+        if layers < 1 or not 1 <= requests <= 8192 or max_len < 1:
+            raise ValueError(f"{me}: layers and max_len must be positive, requests in [1, 8192]")
+        if not 1 <= kv_heads <= 1024:
+            raise ValueError(f"{me}: kv_heads must be in [1, 1024], got {kv_heads}")
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"{me}: block_size must be one of {BLOCK_SIZES}, got {block_size}")
         if head_dim not in HEAD_DIMS:
@@ -45,6 +49,8 @@ class _PagedCache:
         num_blocks = requests * width if num_blocks is None else num_blocks
         if not 1 <= num_blocks <= (2 ** 31 - 1) // block_size:
             raise ValueError(f"{me}: num_blocks must be positive and num_blocks * block_size below 2^31")
+        if self._MOST_RUNS and num_blocks * kv_heads > self._MOST_RUNS:
+            raise ValueError(f"{me}: num_blocks * kv_heads must be at most {self._MOST_RUNS}")
         self.layers, self.requests, self.max_len = layers, requests, width * block_size
         self.kv_heads, self.head_dim, self.block_size, self.num_blocks = kv_heads, head_dim, block_size, num_blocks
         i32 = dict(dtype=torch.int32, device=device)
@@ -165,6 +171,8 @@ class KVCache4(_PagedCache):
     each token and head with an fp16 scale and bias for every group_size (32, 64
     or 128) channels, 4.25 to 5 bits an element.  A token is quantized by itself: what other tokens of
     its block hold stays.  Same methods, and values()."""
+
+    _MOST_RUNS = 2 ** 31 - 1
 
     def __init__(self, layers: int, requests: int, max_len: int, kv_heads: int, head_dim: int, block_size: int = 64,
                  num_blocks: Optional[int] = None, group_size: int = 64, device="cuda"):

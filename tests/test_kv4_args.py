@@ -203,3 +203,16 @@ def test_attention_tables_end_before_32_bits(bs):
     with pytest.raises(ValueError, match="max_len"):
         kv_cache.KVCache4(1, 1, bs * most + 1, 1, 64, bs, num_blocks=2, group_size=32, device="meta")
     assert kv_cache.KVCache4(1, 1, bs * most, 1, 64, bs, num_blocks=2, group_size=32, device="meta").max_len == bs * most
+
+
+def test_caches_refuse_what_their_kernels_refuse():
+    """Before they allocate anything: more key heads than a call takes, more (block, head) than the 4-bit kernels count."""
+    for cls in (kv_cache.KVCache8, kv_cache.KVCache4):
+        with pytest.raises(ValueError, match="kv_heads"):
+            cls(1, 1, 64, 1025, 64, 16, device="meta")
+        assert cls(1, 1, 64, 1024, 64, 16, device="meta").kv_heads == 1024
+    with pytest.raises(ValueError, match="num_blocks . kv_heads"):
+        kv_cache.KVCache4(1, 1, 64, 1024, 64, 16, num_blocks=2 ** 21, group_size=32, device="meta")
+    with pytest.raises(ValueError, match="num_blocks . kv_heads"):
+        kv_cache.KVCache4(1, 8192, 4096, 1024, 64, 16, group_size=32, device="meta")
+    kv_cache.KVCache4(1, 1, 64, 1023, 64, 16, num_blocks=2 ** 21, group_size=32, device="meta")
