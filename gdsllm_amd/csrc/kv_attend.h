@@ -490,14 +490,14 @@ int launch_part(typename S::Args a, const Part& p, int64_t blocks, int64_t max_r
         constexpr int per = 1024 / S::kD;
         const int n = (rows + per - 1) / per;
         hipLaunchKernelGGL((attend_join_rows<typename S::Args, S::kRows, S::kD>), dim3(per_request * n, requests), dim3(256), 0, s, a, n);
-        return check_hip(hipGetLastError(), where);
+    } else {
+        const dim3 join(per_request * rows, requests);
+        // few sequences are long, in many parts each
+        if (p.sequences * rows <= kCus)
+            hipLaunchKernelGGL((attend_join<typename S::Args, S::kRows, S::kD, 1024>), join, dim3(1024), 0, s, a, rows);
+        else
+            hipLaunchKernelGGL((attend_join<typename S::Args, S::kRows, S::kD, 256>), join, dim3(256), 0, s, a, rows);
     }
-    const dim3 join(per_request * rows, requests);
-    // few sequences are long, in many parts each
-    if (p.sequences * rows <= kCus)
-        hipLaunchKernelGGL((attend_join<typename S::Args, S::kRows, S::kD, 1024>), join, dim3(1024), 0, s, a, rows);
-    else
-        hipLaunchKernelGGL((attend_join<typename S::Args, S::kRows, S::kD, 256>), join, dim3(256), 0, s, a, rows);
     return check_hip(hipGetLastError(), where);
 }
 

@@ -47,3 +47,14 @@ def test_no_kernel_uses_scratch(device_asm):
                 spills.append(f"{name}: {m.group(1)} ({m.group(2)} bytes)")
     assert kernels > 50, f"found only {kernels} kernels in the assembly"
     assert not spills, "kernels with scratch:\n" + "\n".join(spills)
+
+
+def test_parts_of_a_tile_have_one_join(device_asm):
+    """Attention over a paged cache builds the joins that a launch can take and no others: in 4 bits by rows for tiles
+    of 128 and 256 rows, else a workgroup to a row."""
+    join = re.compile(r"\.amdhsa_kernel\s+\S*?(attend_join(?:_rows)?)I\S*?Cache\S*?Li(\d+)ELi(\d+)E")
+    four = {m.groups() for m in join.finditer(device_asm["kv4_attention.hip"])}
+    assert four == {("attend_join", "16", d) for d in ("64", "128", "256")} | {
+        ("attend_join_rows", r, d) for r, d in (("256", "64"), ("256", "128"), ("128", "64"), ("128", "128"), ("128", "256"))}
+    eight = {m.groups() for m in join.finditer(device_asm["kv_attention.hip"])}
+    assert eight == {("attend_join", r, d) for r in ("16", "128") for d in ("64", "128", "256")}
