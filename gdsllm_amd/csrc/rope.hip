@@ -66,6 +66,25 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs a) {
     }
 }
 
+// `tokens` rows of `width` halves, ld apart.
+struct Span {
+    const void* p;
+    int64_t ld, width;
+};
+
+// Whether two of them share a byte.  Rows of one distance may lie between each
+// other's (q and k in the rows of one projection); of different ones they are
+// taken to meet where the memory from the first row to the last does.
+bool meet(const Span& a, const Span& b, int64_t tokens) {
+    const uint64_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+    auto bytes = [&](const Span& s) { return 2 * (static_cast<uint64_t>(tokens - 1) * s.ld + s.width); };
+    if (pa >= pb + bytes(b) || pb >= pa + bytes(a)) return false;
+    if (tokens == 1 || a.ld != b.ld) return true;
+    const uint64_t period = 2 * static_cast<uint64_t>(a.ld);
+    const uint64_t d = pb >= pa ? (pb - pa) % period : (period - (pa - pb) % period) % period;  // of b's row from one of a
+    return d < 2 * static_cast<uint64_t>(a.width) || d + 2 * static_cast<uint64_t>(b.width) > period;
+}
+
 }  // namespace
 }  // namespace gdsllm
 
@@ -97,6 +116,10 @@ extern "C" int gdsllm_rope(const void* q, int64_t ldq, void* q_out, int64_t ldqo
         return bad("misaligned pointer");
     if ((q == q_out && tokens > 1 && ldq != ldqo) || (has_k && k == k_out && tokens > 1 && ldk != ldko))
         return bad("in place the strides must be equal");
+    const Span qs{q, ldq, q_heads * head_dim}, qos{q_out, ldqo, qs.width}, ks{k, ldk, k_heads * head_dim}, kos{k_out, ldko, ks.width};
+    if ((q != q_out && meet(qos, qs, tokens)) ||
+        (has_k && ((k != k_out && meet(kos, ks, tokens)) || meet(qos, ks, tokens) || meet(kos, qs, tokens) || meet(qos, kos, tokens))))
+        return bad("q_out and k_out must overlap neither each other nor q and k, but for q_out = q and k_out = k");
     RopeArgs a{};
     a.r = {static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<uint16_t*>(q_out),
            static_cast<uint16_t*>(k_out), ldq, ldk, ldqo, ldko, static_cast<int>(q_heads), static_cast<int>(q_heads + k_heads)};

@@ -543,7 +543,8 @@ typedef struct gdsllm_kv_cache4 {
  * [max_pos][rotary/2] at positions[t], in 64 bits, rounded to fp32 and then to
  * fp16; the channels past `rotary` are copied.  A row whose position lies outside
  * [0, max_pos) is zero.  head_dim in [2, 1024], rotary even.  q_out may be q with the same
- * stride, k_out k (in place); otherwise the outputs overlap neither input.  Fast
+ * stride, k_out k (in place); otherwise the outputs overlap neither input nor each
+ * other, which is checked (so in place k must not be q).  Fast
  * for head_dim % 8 == 0, rotary % 16 == 0 (neighbours: % 8) and everything on the
  * 16-byte grid.  Replaces the rotation of runtime/llama.py:60-103.             */
 int gdsllm_rope(const void* q, int64_t ldq, void* q_out, int64_t ldqo, int64_t q_heads, const void* k, int64_t ldk,

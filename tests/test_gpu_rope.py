@@ -129,3 +129,24 @@ def test_refusals(gpu):
     for args, word in bad:
         with pytest.raises(RuntimeError, match=word):
             ext().rope(*args)
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+def test_in_place_k_is_not_q(gpu, neighbours):
+    """q and k that share memory are refused in place; rows between each other's, from either side, are not."""
+    q, _, pos, cos, sin = problem(9, 4, 4, 64, 64, 17)
+    d = [t.to(gpu) for t in (q, pos, cos, sin)]
+    with pytest.raises(RuntimeError, match="overlap"):
+        ext().rope(d[0], d[0], *d[1:], neighbours, True)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ext().rope(d[0][:, :3], d[0][:, 2:], *d[1:], neighbours, True)
+    assert torch.equal(d[0].cpu(), q)
+    want = s4.rotate(q, pos, cos, sin, neighbours)[0]
+    for cut in (1, 2, 3):
+        for first in (True, False):
+            x = q.to(gpu)
+            a, b = (x[:, :cut], x[:, cut:]) if first else (x[:, cut:], x[:, :cut])
+            ext().rope(a, b, *d[1:], neighbours, True)
+            assert torch.equal(x.cpu(), want)
+    # the same heads twice, into new tensors
+    assert all(torch.equal(y.cpu(), want) for y in ext().rope(d[0], d[0], *d[1:], neighbours))

@@ -216,3 +216,19 @@ def test_caches_refuse_what_their_kernels_refuse():
     with pytest.raises(ValueError, match="num_blocks . kv_heads"):
         kv_cache.KVCache4(1, 8192, 4096, 1024, 64, 16, group_size=32, device="meta")
     kv_cache.KVCache4(1, 1, 64, 1023, 64, 16, num_blocks=2 ** 21, group_size=32, device="meta")
+
+
+def test_rope_outputs_apart():
+    """Rows of 128 and 64 halves (256 and 128 bytes) 512 bytes apart: outputs may lie between the inputs' rows, not on them."""
+    ld = dict(ldq=256, ldqo=256, ldk=256, ldko=256, n=3)
+    far = dict(q=2 ** 20, qo=2 ** 21, k=2 ** 22, ko=2 ** 23)
+    def refused(**kw):
+        return rope(**{**ld, **far, **kw}) == BAD and "overlap" in _err()
+
+    q = far["q"]
+    assert refused(qo=q + 16) and refused(qo=q - 16) and refused(qo=q + 240) and refused(qo=q + 512) and refused(qo=q + 2 * 512 + 240)
+    assert refused(ko=q) and refused(ko=q + 240) and refused(k=q, qo=q) and refused(k=q, ko=q, qo=q)
+    assert refused(k=q + 128, ko=q + 128, qo=q) and refused(ko=far["qo"]) and refused(ko=far["qo"] + 512 - 112)
+    assert refused(ko=far["k"] + 64) and refused(k=far["qo"] + 128)
+    # rows of other distances, in the same memory; a single row
+    assert refused(ldqo=384, qo=q + 256) and refused(n=1, qo=q + 16) and refused(n=1, k=q + 128, ko=q + 128, qo=q)
