@@ -1032,6 +1032,17 @@ py::object kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torc
     return has_q ? py::cast(out) : py::none();
 }
 
+// Operators without a backward pass refuse what autograd would follow through them:
+// their results would pass for constants.
+void no_gradient(const torch::Tensor& t, const char* what, const char* where) {
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        throw std::runtime_error(std::string(where) + ": " + what + " needs a gradient, which there is none of (no_grad or detach)");
+}
+// A tensor that a kernel writes: autograd learns of it, as of torch's own operators in place.
+void written(const torch::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // What an attention call over a paged cache brings besides the cache.
 struct AttentionRows {
     torch::Tensor q, lens, starts, out;
@@ -1125,6 +1136,8 @@ py::tuple rope(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor po
     const int64_t n = q.size(0), dim = q.size(2);
     torch::Tensor qr = rope_rows(q, dev, n, dim, inplace, "q"), kr;
     if (k.has_value()) kr = rope_rows(*k, dev, n, dim, inplace, "k");
+    no_gradient(q, "q", "rope");
+    if (k.has_value()) no_gradient(*k, "k", "rope");
     const Rotation r(positions, cos, sin, dev, n, "rope");
     const bool has_k = kr.defined() && kr.size(1) > 0;
     torch::Tensor qo = inplace ? qr : torch::empty(qr.sizes(), qr.options()), ko;
@@ -1135,6 +1148,10 @@ py::tuple rope(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor po
                       has_k ? kr.size(1) : 0, dim, n, r.positions_ptr(), r.cos_ptr(), r.sin_ptr(), r.rotary, r.max_pos,
                       neighbours ? 1 : 0, OnDevice(dev).stream()),
           "rope");
+    if (inplace) {
+        written(qr);
+        if (has_k) written(kr);
+    }
     return py::make_tuple(qo, ko.defined() ? py::cast(ko) : py::none());
 }
 
@@ -1169,6 +1186,9 @@ py::object kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, tor
     torch::Tensor vr = head_rows(v, dev, c.kv_heads, c.head_dim, "v", where);
     const int64_t n = kr.size(0);
     if (vr.size(0) != n) throw std::runtime_error("kv4_append: k and v differ in tokens");
+    no_gradient(k, "k", where);
+    no_gradient(v, "v", where);
+    if (q.has_value()) no_gradient(*q, "q", where);
     torch::Tensor s = flat(slots, torch::kInt32, dev, n, "slots", where);
     if (cos.has_value() != sin.has_value()) throw std::runtime_error("kv4_append: cos and sin come together");
     if (q.has_value() && !cos.has_value()) throw std::runtime_error("kv4_append: q is given without cos and sin");
@@ -1210,6 +1230,7 @@ torch::Tensor kv4_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tenso
     const char* where = "kv4_attention";
     const gdsllm_kv_cache4 c = kv4_cache_of(k_cache, v_cache, k_affine, v_affine, where);
     const int dev = k_cache.get_device();
+    no_gradient(q, "q", where);
     const AttentionRows r(q, block_tables, lens, starts, output, dev, c.head_dim, c.block_size, max_new, max_len, where);
     torch::Tensor ws = r.workspace(
         gdsllm_kv4_attention_workspace_size(r.requests, r.heads, c.kv_heads, c.head_dim, r.most_new, r.most_len));
@@ -1219,6 +1240,7 @@ torch::Tensor kv4_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tenso
                                max_new, max_len, output.has_value() ? 0 : 1, ws.defined() ? ws.data_ptr() : nullptr,
                                ws.defined() ? ws.numel() : 0, OnDevice(dev).stream()),
           where);
+    if (output.has_value()) written(r.out);
     return r.out;
 }
 

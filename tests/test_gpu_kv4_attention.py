@@ -430,3 +430,20 @@ def test_refusals(gpu):
         ext().kv4_attention(q, k, v, ka, va, t, n, st, 0.0)
     with pytest.raises(RuntimeError, match="output"):
         ext().kv4_attention(q, k, v, ka, va, t, n, st, 0.1, output=torch.empty_like(q)[:1])
+
+
+def test_gradients_and_versions(gpu):
+    """There is no backward pass: a q that autograd would follow is refused, and it learns of a written output."""
+    p = Problem(gpu, 32, 64, 4, 2, 16, [20, 20], [1, 1], 2700)
+    a = p.args()
+    for q in (a[0].clone().requires_grad_(), a[0].clone().requires_grad_() * 1.0):
+        with pytest.raises(RuntimeError, match="kv4_attention: q needs a gradient"):
+            ext().kv4_attention(q, *a[1:], p.scale)
+        with torch.no_grad():
+            p.check(ext().kv4_attention(q, *a[1:], p.scale))
+    out = torch.ones_like(a[0])
+    z = out * torch.ones(64, dtype=torch.float16, device=gpu, requires_grad=True)
+    ext().kv4_attention(*a, p.scale, output=out)
+    p.check(out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.float().sum().backward()

@@ -276,3 +276,21 @@ def test_refusals(gpu):
     with pytest.raises(RuntimeError, match="slots"):
         ext().kv4_values(s.long(), *c.dev)
     c.check()
+
+
+def test_gradients_are_refused(gpu):
+    """There is no backward pass: rows that autograd would follow are refused before anything is written."""
+    g = gen(71)
+    c = Cache(gpu, 3, 2, 16, 64, 32, 72)
+    k, v, q = (rows(3, h, 64, g).to(gpu) for h in (2, 2, 4))
+    slots, pos = (torch.tensor(t, dtype=torch.int32, device=gpu) for t in ([5, 6, 7], [0, 1, 2]))
+    cos, sin = (t.to(gpu) for t in angles(9, 64, g))
+    for i, name in enumerate("kvq"):
+        rows_ = [k, v, q]
+        rows_[i] = rows_[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match=f"kv4_append: {name} needs a gradient"):
+            ext().kv4_append(*rows_[:2], slots, *c.dev, rows_[2], pos, cos, sin)
+        c.check()
+    with torch.no_grad():
+        ext().kv4_append(k.clone().requires_grad_(), v, slots, *c.dev, q, pos, cos, sin)
+    c.append(k.cpu(), v.cpu(), slots.cpu(), q.cpu(), pos.cpu(), cos.cpu(), sin.cpu())

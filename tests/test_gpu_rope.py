@@ -150,3 +150,32 @@ def test_in_place_k_is_not_q(gpu, neighbours):
             assert torch.equal(x.cpu(), want)
     # the same heads twice, into new tensors
     assert all(torch.equal(y.cpu(), want) for y in ext().rope(d[0], d[0], *d[1:], neighbours))
+
+
+def test_gradients_and_versions(gpu):
+    """There is no backward pass: what autograd would follow is refused, and in place it learns of the write."""
+    q, k, pos, cos, sin = problem(5, 3, 1, 64, 64, 19)
+    d = [t.to(gpu) for t in (q, k, pos, cos, sin)]
+    for i, name in enumerate("qk"):
+        for inplace in (False, True):
+            a = list(d)
+            a[i] = (a[i].clone().requires_grad_() * 1.0)
+            with pytest.raises(RuntimeError, match=f"rope: {name} needs a gradient"):
+                ext().rope(*a, False, inplace)
+            with torch.no_grad():
+                got = ext().rope(*a)
+            assert not got[i].requires_grad and torch.equal(got[i].cpu(), s4.rotate((q, k)[i], pos, cos, sin)[0])
+    w = torch.ones(64, dtype=torch.float16, device=gpu, requires_grad=True)
+    x, y = d[0].clone(), d[1].clone()
+    z, u = x * w, y * w
+    ext().rope(x, y, *d[2:], False, True)
+    for t in (z, u):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            t.float().sum().backward()
+    z = d[0] * w
+    ext().rope(d[0], d[1], *d[2:])  # into new tensors: q stays
+    z.float().sum().backward()
+    with torch.inference_mode():
+        x = d[0] * 1.0
+    ext().rope(x, None, *d[2:], False, True)
+    assert torch.equal(x.cpu(), s4.rotate(q, pos, cos, sin)[0])
