@@ -76,7 +76,7 @@ def values(slots, packed, affine):
 
 def attention(q, k_val, v_val, tables, lens, starts, scale, heads=None):
     """q fp16 [T, Hq, D]; k_val, v_val float64 [N, Hkv, bs, D].  (out, bound), float64 [T, Hq, D]: zero where nothing is
-    seen and in rows of no request; bound, how far a row computed with fp32 sums, fp16 weights and an fp16 result may be off:
+    seen and in rows of no request; a block outside the cache has no weight; bound, how far a row computed with fp32 sums, fp16 weights and an fp16 result may be off:
       * scores: D products summed in fp32 and scaled: |dx| <= D 2^-24 sum|q k| scale + 3 * 2^-24 |x|, the exponential
         2^-22 more; so dp / p <= d = that, twice (numerator, sum)
       * a weight in the product with v: half an fp16 step, 2^-11 of itself, or 2^-25 where the largest is 2^7 at least
@@ -95,9 +95,10 @@ def attention(q, k_val, v_val, tables, lens, starts, scale, heads=None):
             continue
         ids = tables[b, :blocks(held, bs)].long()
         last = held - n + torch.arange(n)
-        see = torch.arange(held) <= last[:, None]  # [n, held]
+        there = (ids >= 0) & (ids < k_val.shape[0])
+        see = (torch.arange(held) <= last[:, None]) & there.repeat_interleave(bs)[:held]  # [n, held]
         for h in range(Hkv) if heads is None else heads:
-            k, v = (t[ids, h].reshape(-1, D)[:held] for t in (k_val, v_val))
+            k, v = (t[torch.where(there, ids, 0), h].reshape(-1, D)[:held] for t in (k_val, v_val))
             for j in range(h * G, (h + 1) * G):
                 qq = q[lo:hi, j].double()
                 x = (qq @ k.T * scale).masked_fill(~see, -torch.inf)

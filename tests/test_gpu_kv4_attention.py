@@ -447,3 +447,124 @@ def test_gradients_and_versions(gpu):
     p.check(out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.float().sum().backward()
+
+
+BAD_IDS = (-1, 10 ** 9, -2 ** 31)
+
+
+def lose(p, *places):
+    """Table entries (request, block) that name no block of the cache.  Block 0, which lies where a bad index is taken
+    to, is nobody's and its pairs are no numbers."""
+    used = set(p.tables[p.tables >= 0].tolist())
+    free = next((i for i in range(1, p.k.shape[0]) if i not in used), 1)  # (blocks that occur again and again: any)
+    if 0 in used and free not in used:
+        for t in (p.k, p.v, p.ka, p.va):
+            t[free] = t[0]
+    p.tables[p.tables == 0] = free
+    p.ka[0], p.va[0] = float("nan"), float("inf")
+    for i, (b, block) in enumerate(places):
+        p.tables[b, block] = (*BAD_IDS, p.k.shape[0])[i % 4]
+
+
+# dim, heads, kv_heads, bs, group, lens, new, max_len, lost (request, block)
+LOST = {
+    "decode": (128, 4, 1, 64, 64, [300, 64, 17, 140], [1] * 4, None, [(0, 2), (1, 0), (2, 0), (3, 2), (0, 4)]),
+    "decode_256": (256, 4, 2, 16, 128, [300, 16, 33], [1] * 3, None, [(0, 0), (1, 0), (2, 2), (0, 7)]),
+    "decode_shared": (128, 4, 1, 32, 32, [2100, 513], [1, 1], None, [(0, 0), (0, 9), (0, 40), (0, 65), (1, 16), (1, 3)]),
+    "decode_shared_256": (256, 4, 2, 128, 64, [2100, 700], [1, 2], None, [(0, 3), (0, 16), (1, 0), (1, 5)]),
+    "decode_segments": (64, 8, 8, 16, 32, [4500], [1], 500, [(0, 255), (0, 256), (0, 270)]),
+    "prompt_64": (64, 4, 1, 16, 32, [300, 129, 20], [200, 100, 20], None, [(0, 0), (0, 5), (0, 12), (0, 18), (1, 0), (1, 1), (2, 1)]),
+    "prompt_128": (128, 6, 2, 64, 128, [300, 129], [200, 100], None, [(0, 1), (0, 4), (1, 0)]),
+    "prompt_256": (256, 6, 2, 32, 64, [300, 129], [200, 100], None, [(0, 0), (0, 4), (0, 8), (1, 2), (1, 4)]),
+    "prompt_wide_64": (64, 512, 128, 16, 64, [130, 65, 7], [100, 65, 2], None, [(0, 0), (0, 5), (0, 8), (1, 0), (2, 0)]),
+    "prompt_wide_128": (128, 512, 128, 64, 64, [130, 65, 7], [100, 65, 2], None, [(0, 1), (1, 1)]),
+    "prompt_shared_64": (64, 4, 2, 16, 64, [2300, 70, 2100, 180], [150, 2, 1, 180], None,
+                         [(0, 0), (0, 60), (0, 64), (0, 140), (1, 4), (2, 7), (3, 1)]),
+    "prompt_shared_128": (128, 2, 2, 128, 32, [2300, 70, 2100, 180], [150, 2, 1, 180], None, [(0, 0), (0, 8), (0, 17), (2, 16), (3, 0)]),
+    "prompt_shared_256": (256, 6, 2, 32, 128, [2300, 70, 2100, 180], [150, 2, 1, 180], None, [(0, 2), (0, 33), (0, 71), (2, 0), (3, 5)]),
+    "prompt_wide_shared_64": (64, 256, 64, 16, 32, [1100, 5, 1500], [80, 3, 33], None, [(0, 0), (0, 33), (0, 68), (2, 50), (2, 93)]),
+    "prompt_wide_shared_128": (128, 256, 64, 32, 64, [1300, 900], [70, 65], None, [(0, 0), (0, 20), (0, 40), (1, 27), (1, 3)]),
+}
+
+
+@pytest.mark.parametrize("case", LOST.values(), ids=LOST)
+def test_lost_blocks(gpu, case):
+    """Blocks outside the cache, the first, the last and some between, have no weight in any kind of tile, whole or
+    shared out; rows that see no other block are zero."""
+    dim, heads, kv_heads, bs, group, lens, new, max_len, lost = case
+    p = Problem(gpu, group, dim, heads, kv_heads, bs, lens, new, 2800 + len(lost))
+    p.poison()
+    lose(p, *lost)
+    p.check(p.run(max_len=max_len), None if kv_heads < 64 else [0, 31, kv_heads - 1])
+
+
+def mark(p, blocks):
+    """Equal keys, and no values but 1024 in one block, request r's number blocks[r]: a row that sees m of its tokens
+    among n gets 1024 m / n.  Gives those: [rows, 1, 1]."""
+    p.q.zero_()
+    p.va.zero_()
+    marked = p.k.shape[0] - 1
+    p.va[marked, ..., 1] = 1024.0
+    p.tables[p.tables == marked] = 0
+    want = []
+    for r, block in enumerate(blocks):
+        p.tables[r, block] = marked
+        n = int(p.starts[r + 1] - p.starts[r])
+        seen = torch.arange(int(p.lens[r]) - n + 1, int(p.lens[r]) + 1).double()
+        want.append(1024 * (seen - block * p.bs).clamp(0, p.bs) / seen)
+    return torch.cat(want)[:, None, None]
+
+
+def check_marks(p, blocks, **kw):
+    """Weights are equal powers of two and sums whole numbers of them, exact in fp32; the quotient and its product are
+    off by 2^-22, the result by half an fp16 step."""
+    want = mark(p, blocks)
+    got = p.run(**kw).cpu().double()
+    assert bool(((got - want).abs() <= (2.0 ** -11 + 2.0 ** -21) * want + 2.0 ** -25).all()), blocks
+
+
+SEGMENTS = [(64, 2, 32), (128, 2, 64), (256, 2, 128), (64, 64, 64), (128, 64, 128)]
+
+
+@pytest.mark.parametrize("bs", [16, 256])
+@pytest.mark.parametrize("dim,kv_heads,group", SEGMENTS, ids=[f"d{d}_{'wide' if h > 2 else 'tall'}" for d, h, _ in SEGMENTS])
+def test_prompts_past_a_segment(gpu, dim, kv_heads, group, bs):
+    """Prompt tiles, of 128 rows (tall) and of 256 (wide), over more tokens than a workgroup holds a block table of at
+    once: twice and three times as many.  (The bound of 1000 tokens leaves each sequence to one workgroup.)"""
+    lens, new = [4200, 8300, 4096, 4097], [70, 66, 33, 40]
+    p = Problem(gpu, group, dim, 2 * kv_heads, kv_heads, bs, [2 * bs] * 4, new, 2900 + dim + bs)
+    repeated(p, lens, new, 2901)
+    p.check(p.run(max_len=1000), [0, kv_heads - 1])
+    lose(p, (0, 4096 // bs), (1, 4096 // bs + 1), (1, 8192 // bs), (3, 0), (2, 4095 // bs))
+    p.check(p.run(max_len=1000), [0, kv_heads - 1])
+
+
+@pytest.mark.parametrize("max_len", [1000, 0], ids=["whole", "shared"])
+@pytest.mark.parametrize("bs", [16, 256])
+@pytest.mark.parametrize("dim,kv_heads,group", SEGMENTS, ids=[f"d{d}_{'wide' if h > 2 else 'tall'}" for d, h, _ in SEGMENTS])
+def test_every_block_counts_once(gpu, dim, kv_heads, group, bs, max_len):
+    """In prompt tiles, whole and shared out: the first block, those about a segment's edge, the last, and others
+    between count by their share, each row's by the tokens that it sees."""
+    lens, new = [4200, 8300, 4097, 8190, 300], [70, 66, 40, 35, 34]
+    p = Problem(gpu, group, dim, 2 * kv_heads, kv_heads, bs, [2 * bs] * 5, new, 3000 + dim + bs)
+    repeated(p, lens, new, 3001)
+    tables, at = p.tables.clone(), [sv.blocks(n, bs) for n in lens]
+    edge = 4096 // bs
+    for blocks in ([0] * 5, [n - 1 for n in at], [edge - 1, edge - 1, edge, edge, 0], [edge, 2 * edge, 1, edge - 1, at[4] - 1],
+                   [at[0] - 2, 2 * edge - 1, edge - 2, edge + 1, at[4] // 2], [at[0] // 2, at[1] // 3, 3, at[3] - 3, 0]):
+        p.tables = tables.clone()
+        check_marks(p, blocks, max_len=max_len)
+
+
+def test_every_part_of_a_long_sequence_counts_once(gpu):
+    """Hundreds of parts of 256 tokens, a block each, joined by 256 threads (one long sequence among short ones) and by
+    1024 (alone): parts about the 256th and the 512th, the first and the last."""
+    for lens, blocks in (([120000] + list(range(1, 32)), (0, 1, 63, 64, 255, 256, 257, 300, 467, 468)),
+                         ([131000], (0, 1, 16, 255, 256, 257, 500, 510, 511))):
+        n = len(lens)
+        p = Problem(gpu, 64, 64, 16, 1, 256, [1000] * n, [1] * n, 3100)
+        repeated(p, lens, [1] * n, 3101)
+        tables = p.tables.clone()
+        for block in blocks:
+            p.tables = tables.clone()
+            check_marks(p, [block] + [0] * (n - 1))

@@ -112,3 +112,22 @@ def test_attention():
     assert torch.allclose(out[0, 3], want, rtol=1e-12)
     assert bool((out[1] == 0).all()) and torch.allclose(out[2, 0], v[1, 0, 0])  # four rows of three tokens: the first sees none
     assert bool((bound >= 0).all()) and float((bound / out.abs().clamp(min=0.05)).max()) < 0.02
+
+
+def test_attention_without_blocks_outside_the_cache():
+    """A block that is not there has no weight: the same as a table without it, for rows that stand behind it; nothing
+    but zeros where no other is seen."""
+    g = gen(9)
+    k, v = torch.randn(2, 6, 2, 4, 8, generator=g).double()
+    q = torch.randn(5, 4, 8, generator=g).half()
+    tables, i32 = torch.tensor([[3, 1, 5, 0]], dtype=torch.int32), dict(dtype=torch.int32)
+    starts = torch.tensor([0, 5], **i32)
+    for lost in (-1, 6, 10 ** 9, -2 ** 31):
+        t = tables.clone()
+        t[0, 1] = lost
+        got = s4.attention(q, k, v, t, torch.tensor([15], **i32), starts, 0.3)
+        want = s4.attention(q, k, v, tables[:, [0, 2, 3]], torch.tensor([11], **i32), starts, 0.3)
+        assert torch.allclose(got[0], want[0], rtol=1e-12, atol=1e-14) and bool((got[1] >= want[1] * (1 - 1e-12)).all())
+        t = torch.tensor([[lost, 2]], **i32)
+        got = s4.attention(q, k, v, t, torch.tensor([6], **i32), starts, 0.3)[0]
+        assert bool((got[:3] == 0).all()) and bool((got[3:].abs().amax(-1) > 0).all())
