@@ -794,12 +794,21 @@ int launch_attend4(Args4 a, const Plan& p, int64_t blocks, int64_t max_rows, cha
     const char* where = "kv4_attention launch";
     const int zero_other = a.zero_other;
     a.zero_other = p.few.on ? zero_other : 0;
-    // D = 256: one workgroup to a compute unit, of eight waves, for the bytes under way (131072 tokens 29.3 us, with
-    // four waves 30.7; 4 requests of up to 20000 tokens over 8 heads 33.6 and 38.0; 32 of up to 4000 23.7 and 22.7)
-    constexpr int kWaves = D == 256 ? 8 : 4;
-    if (int rc = launch_part<RowTile4<D, 8>, RowTile4<D, kWaves>>(a, p.few, blocks, p.many.on ? kFewRows : max_rows, workspace, s,
-                                                                 where))
-        return rc;
+    const int64_t few_rows = p.many.on ? kFewRows : max_rows;
+    auto few = [&](auto tile) { return launch_part<RowTile4<D, 8>, decltype(tile)>(a, p.few, blocks, few_rows, workspace, s, where); };
+    int rc = GDSLLM_OK;
+    if constexpr (D == 256) {
+        // One workgroup to a compute unit.  Eight waves for the bytes under way; four, whose sums meet
+        // sooner, where tiles are full and a workgroup has few tokens (32 requests over 2 key heads of 16
+        // query heads each, up to 2000 tokens 22.1 us with four and 23.0 with eight, 4000 22.7 and 23.5,
+        // 8000 31.1 and 31.0, 16000 51.5 and 45.5; one of 40000 19.8 and 20.1, of 131072 30.9 and 29.5.
+        // Half full, 4 requests over 4 key heads of 8, up to 4000 20.7 and 19.8, 16000 22.3 and 21.7).
+        if (few_rows >= 16 && p.few.sequences * p.few.longest < 1024 * static_cast<int64_t>(p.few.groups)) rc = few(RowTile4<D, 4>{});
+        else rc = few(RowTile4<D, 8>{});
+    } else {
+        rc = few(RowTile4<D, 4>{});
+    }
+    if (rc) return rc;
     a.zero_other = p.few.on ? 0 : zero_other;
     char* ws = workspace + p.few.bytes;
     if constexpr (D <= 128)

@@ -349,6 +349,7 @@ struct Part {
     bool on = false;
     int rows = 0, min_rows = 0, max_rows = INT_MAX, tiles = 0;
     int64_t sequences = 0;  // (request, row tile, kv head)
+    int64_t longest = 0;    // tokens that one may have
     int groups = 0;         // workgroups that share them; 0: one to a sequence
     size_t sums = 0, bytes = 0;
 };
@@ -380,6 +381,7 @@ void finish_part(Part* p, int64_t requests, int64_t kv_heads, int64_t head_dim, 
     p->on = true;
     p->tiles = static_cast<int>(std::max<int64_t>(1, (max_rows + p->rows - 1) / p->rows));
     p->sequences = requests * kv_heads * p->tiles;
+    p->longest = max_len;
     p->groups = whole ? 0 : static_cast<int>(std::min<int64_t>(resident, p->sequences * ((max_len + 255) / 256)));
     p->sums = static_cast<size_t>(p->groups) * 2 * p->rows;
     p->bytes = part_bytes(p->groups, p->rows, p->sequences, head_dim);

@@ -568,3 +568,23 @@ def test_every_part_of_a_long_sequence_counts_once(gpu):
         for block in blocks:
             p.tables = tables.clone()
             check_marks(p, [block] + [0] * (n - 1))
+
+
+@pytest.mark.parametrize("lens,new", [([2100, 700, 5], [1, 1, 1]), ([1500, 0, 1100], [2, 0, 3]), ([1300, 1030], [4, 1])])
+def test_full_tiles_of_wide_heads(gpu, lens, new):
+    """16 and more rows of 256 channels over sequences that are shared out, in workgroups of four waves."""
+    p = Problem(gpu, 128, 256, 32, 2, 64, lens, new, 3200 + sum(new))
+    p.poison()
+    p.check(p.run())
+    p.check(p.run(max_len=0))
+
+
+def test_full_tiles_of_wide_heads_in_four_and_eight_waves(gpu):
+    """On both sides of 1024 tokens to a workgroup: every part counts once."""
+    for longest, blocks in ((30000, (0, 1, 58, 116, 117)), (140000, (0, 4, 5, 273, 545, 546))):
+        p = Problem(gpu, 64, 256, 32, 2, 256, [300, 300], [1, 1], 3300)
+        repeated(p, [longest, 999], [1, 1], 3301)
+        tables = p.tables.clone()
+        for block in blocks:
+            p.tables = tables.clone()
+            check_marks(p, [block, 3])
