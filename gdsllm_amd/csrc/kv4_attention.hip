@@ -8,7 +8,11 @@
 // Elements k, v = fp16(code * scale + bias) enter the matrix cores as the fp16
 // values that they are by definition: nothing of the format is left for the sums.
 // Weights are rounded to fp16 for the product with v and for it alone: half an
-// fp16 step of a weight, and 2^-25 at least where the largest is 2^7 to 2^11.
+// fp16 step of a weight, and 2^-25 at least where the largest is 2^7 to 2^11.  The
+// matrix instructions take fp16 on both sides; a weight as the sum of two such
+// operands costs a 4096-token prompt 232 us instead of 172 and 32 decoding requests
+// 47.8 instead of 44.8, for results 2.0e-4 (their own rounding) instead of 2.6e-4 from
+// those in 64 bits.
 //
 // A code becomes an element in three packed instructions for two of them: below
 // the exponent of 1024 (64 for the high one of two neighbours) it is a number, less
@@ -68,8 +72,8 @@ __device__ __forceinline__ void token_pairs(const NibUnpack& n, uint32_t t0, uin
 template <int D, int NW_>
 struct RowTile4 {
     typedef Args4 Args;
-    // kBegin: 32 requests of up to 8192 tokens 43.0 us with 6 (47.7 with none, 45.1 with 4, 43.8 with 7), 32 of up
-    // to 4000 of 256 channels 22.8 (26.9, 24.4, 24.3)
+    // kBegin: 32 requests of up to 8192 tokens 43.6 us with 6 (49.4 with none, 44.8 with 4, 45.1 with 7), 32 of up
+    // to 4000 of 256 channels 22.7 (26.9, 24.2, 24.4)
     static constexpr int kRows = 16, kD = D, kPerCu = per_cu(D), kBegin = 6;
     static constexpr bool kRowJoin = false;
     static constexpr int kThreads = NW_ * 64;

@@ -421,8 +421,8 @@ Plan plan_attend(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t he
         if (prompts.shares_wide) {
             // 256 rows to a tile (each wave converts half as much) where those are many; whole
             // where two of them come to a compute unit, one after the other: 4 chunks of up
-            // to 300 tokens behind up to 5000 take 132 us shared out in 256-row tiles, 150 in
-            // 128-row ones and 148 whole, 500 tokens behind 1500 44, 43 and 46
+            // to 300 tokens behind up to 5000 take 129 us shared out in 256-row tiles, 160 in
+            // 128-row ones and 147 whole, 500 tokens behind 1500 44, 42 and 63
             wide = head_dim <= 128 && 2 * wide_sequences >= resident;
             whole = max_len <= kWholeTokens || (wide ? wide_sequences : sequences) >= 2 * resident;
         } else {
