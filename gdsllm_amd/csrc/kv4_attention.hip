@@ -803,11 +803,13 @@ int launch_attend4(Args4 a, const Plan& p, int64_t blocks, int64_t max_rows, cha
     int rc = GDSLLM_OK;
     if constexpr (D == 256) {
         // One workgroup to a compute unit.  Eight waves for the bytes under way; four, whose sums meet
-        // sooner, where tiles are full and a workgroup has few tokens (32 requests over 2 key heads of 16
-        // query heads each, up to 2000 tokens 22.1 us with four and 23.0 with eight, 4000 22.7 and 23.5,
-        // 8000 31.1 and 31.0, 16000 51.5 and 45.5; one of 40000 19.8 and 20.1, of 131072 30.9 and 29.5.
-        // Half full, 4 requests over 4 key heads of 8, up to 4000 20.7 and 19.8, 16000 22.3 and 21.7).
-        if (few_rows >= 16 && p.few.sequences * p.few.longest < 1024 * static_cast<int64_t>(p.few.groups)) rc = few(RowTile4<D, 4>{});
+        // sooner, where tiles are full and a workgroup has few tokens.  (2 key heads of 16 query heads
+        // each, four waves and eight: 32 requests of up to 2000 tokens 22.1 us and 23.0, 4000 22.7 and 23.5,
+        // 8000 31.1 and 31.0, 16000 51.5 and 45.5; one of 60000 25.2 and 26.4, 80000 24.3 and 24.1, 100000 31.1
+        // and 30.2, 160000 37.3 and 33.6.  Of several the longest says about twice what they have.  Half full,
+        // 4 requests over 4 key heads of 8, up to 4000 20.7 and 19.8, 16000 22.3 and 21.7.)
+        const int64_t most = (a.requests > 1 ? 1024 : 640) * static_cast<int64_t>(p.few.groups);
+        if (few_rows >= 16 && p.few.sequences * p.few.longest < most) rc = few(RowTile4<D, 4>{});
         else rc = few(RowTile4<D, 8>{});
     } else {
         rc = few(RowTile4<D, 4>{});

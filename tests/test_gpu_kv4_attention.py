@@ -580,11 +580,13 @@ def test_full_tiles_of_wide_heads(gpu, lens, new):
 
 
 def test_full_tiles_of_wide_heads_in_four_and_eight_waves(gpu):
-    """On both sides of 1024 tokens to a workgroup: every part counts once."""
-    for longest, blocks in ((30000, (0, 1, 58, 116, 117)), (140000, (0, 4, 5, 273, 545, 546))):
-        p = Problem(gpu, 64, 256, 32, 2, 256, [300, 300], [1, 1], 3300)
-        repeated(p, [longest, 999], [1, 1], 3301)
+    """On both sides of the number of tokens to a workgroup that the choice goes by: every part counts once."""
+    for lens, blocks in (([30000, 999], (0, 1, 58, 116, 117)), ([140000, 999], (0, 4, 5, 273, 545, 546)),
+                         ([60000], (0, 1, 2, 117, 233, 234)), ([100000], (0, 1, 3, 4, 200, 389, 390))):
+        n = len(lens)
+        p = Problem(gpu, 64, 256, 32, 2, 256, [300] * n, [1] * n, 3300)
+        repeated(p, lens, [1] * n, 3301)
         tables = p.tables.clone()
         for block in blocks:
             p.tables = tables.clone()
-            check_marks(p, [block, 3])
+            check_marks(p, [block, 3][:n])
